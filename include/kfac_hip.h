@@ -498,6 +498,38 @@ int kfac_unpack_batched(int count, float* const* arrays, const int64_t* numel,
                         const int* dims, const int* triangular, const float* buffer,
                         int64_t offset, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Orthogonalised updates ---------------------------------------------- */
+
+/* Newton-Schulz orthogonalisation of a list of matrices (HOST arrays of length `count`):
+ *   X = in[i] / (|in[i]| + eps)                       (Frobenius norm)
+ *   `steps` times:  A = X X^T,  X = (a I + b A + c A A) X
+ *   out[i] = X
+ * rows[i] x cols[i], contiguous row-major, of the element type `type` (0 float32, 1 bfloat16,
+ * 2 float16), inputs and results alike; a matrix with more rows than columns is iterated on
+ * transposed; a matrix without elements is skipped.  in[i] == out[i] is allowed.  coefficients:
+ * HOST array of `steps` triples (a, b, c) under which |X| in the spectral norm stays below 7: a product's
+ * operands are kept as fp16 numbers in two parts (22 bits; absolute error 2^-38) times 2^13.
+ * late_steps: in as many steps at the end they are kept in one part (11 bits).  The update that a
+ * layer takes in the place of the preconditioning of optim/secondorder.py:195-209 of the reference
+ * where its Kronecker factors are too large to invert. */
+size_t kfac_orthogonalize_workspace_bytes(int count, const int* rows, const int* cols);
+int kfac_orthogonalize_batched(int count, const int* rows, const int* cols, int type, const void* const* in,
+                               void* const* out, int steps, const float* coefficients, float eps,
+                               int late_steps, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Muon's update of a list of matrices, with the workspace of kfac_orthogonalize_workspace_bytes:
+ *   buffers[i] = momentum * buffers[i] + grads[i]                              (float32)
+ *   U = nesterov ? grads[i] + momentum * buffers[i] : buffers[i]
+ *   params[i] = keep[i] * params[i] - step[i] * orthogonalised(U)
+ * params and grads are of `type`; the sums are formed in float32 and rounded once.  Stands where
+ * optim/secondorder.py:225-312 of the reference applies momentum, weight decay and the update to
+ * a preconditioned gradient. */
+int kfac_muon_update_batched(int count, const int* rows, const int* cols, int type, void* const* params,
+                             const void* const* grads, float* const* buffers, const float* step,
+                             const float* keep, float momentum, int nesterov, int steps,
+                             const float* coefficients, float eps, int late_steps, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

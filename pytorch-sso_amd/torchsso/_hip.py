@@ -129,7 +129,15 @@ _SIGNATURES = {
     'kfac_bn_diag_cov_batched_workspace_bytes': (c_size, [c_int]),
     'kfac_bn_diag_cov_batched': (c_int, [c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
                                          c_ptr, c_ptr, c_size, c_ptr]),
+    'kfac_orthogonalize_workspace_bytes': (c_size, [c_int, c_ptr, c_ptr]),
+    'kfac_orthogonalize_batched': (c_int, [c_int, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_int, c_ptr, c_f32,
+                                           c_int, c_ptr, c_size, c_ptr]),
+    'kfac_muon_update_batched': (c_int, [c_int, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
+                                         c_f32, c_int, c_int, c_ptr, c_f32, c_int, c_ptr, c_size, c_ptr]),
 }
+
+# element types of the entry points that take more than float32
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def int_array(values):
@@ -223,6 +231,22 @@ def dev_ptr(t, what='tensor'):
                            '(no CPU path exists in this package)' % (what, t.device))
     if t.dtype != torch.float32:
         raise KfacHipError('%s has dtype %s, expected float32' % (what, t.dtype))
+    if not t.is_contiguous():
+        raise KfacHipError('%s is not contiguous' % what)
+    return t.data_ptr()
+
+
+def typed_ptr(t, dtype, device, what='tensor'):
+    """Device address of a contiguous tensor of that type on that device (loud otherwise)."""
+    if not isinstance(t, torch.Tensor):
+        raise KfacHipError('%s: expected a torch.Tensor' % what)
+    if not t.is_cuda:
+        raise KfacHipError('%s is on %s: the kernels run on a HIP device only '
+                           '(no CPU path exists in this package)' % (what, t.device))
+    if t.device != device:
+        raise KfacHipError('%s is on %s, expected %s' % (what, t.device, device))
+    if t.dtype != dtype:
+        raise KfacHipError('%s has dtype %s, expected %s' % (what, t.dtype, dtype))
     if not t.is_contiguous():
         raise KfacHipError('%s is not contiguous' % what)
     return t.data_ptr()

@@ -772,3 +772,78 @@ def _pack_call(arrays, buf, offset, unpack):
             _ws_ptr(ws), ws_bytes, _hip.stream_ptr(dev))
     _hip.check(st, 'kfac_unpack_batched' if unpack else 'kfac_pack_batched')
     return offset + total
+
+
+def _element_type(t, what):
+    code = _hip.ELEMENT_TYPES.get(t.dtype)
+    if code is None:
+        raise _hip.KfacHipError('%s has dtype %s, expected float32, bfloat16 or float16'
+                                % (what, t.dtype))
+    return code
+
+
+def _addresses(tensors, like, what, dtype=None):
+    """Device addresses (host array) of contiguous tensors of one type on the device of `like`."""
+    dtype = like.dtype if dtype is None else dtype
+    return (ctypes.c_void_p * len(tensors))(
+        *[_hip.typed_ptr(t, dtype, like.device, '%s %d' % (what, i)) for i, t in enumerate(tensors)])
+
+
+def _matrix_dims(mats, what):
+    for i, m in enumerate(mats):
+        if m.dim() != 2:
+            raise _hip.KfacHipError('%s %d is not a matrix: %s' % (what, i, tuple(m.shape)))
+    return _hip.ints([m.shape[0] for m in mats]), _hip.ints([m.shape[1] for m in mats])
+
+
+# In as many steps at the end of an orthogonalisation operands are kept in 11 bits instead of 22.
+# What a step rounds away grows by the slope of the iteration at zero (3.4) with every step behind
+# it, where a direction of the gradient is weak; of the last two at most 12 * 2^-12 is left where
+# a bfloat16 result rounds by 2^-9, and no step is late where the result holds more bits.
+LATE_STEPS = {torch.float32: 0, torch.float16: 0, torch.bfloat16: 2}
+
+
+def orthogonalize_batched(mats, outs, coefficients, eps):
+    """outs[i] = Newton-Schulz iterate of mats[i] (contiguous 2-D tensors of one type);
+    coefficients: flat list of a, b, c of every step."""
+    lib = _hip.load()
+    if len(mats) == 0:
+        return
+    first = mats[0]
+    kind = _element_type(first, 'matrix 0')
+    rows, cols = _matrix_dims(mats, 'matrix')
+    for i, (m, o) in enumerate(zip(mats, outs)):
+        if m.shape != o.shape:
+            raise _hip.KfacHipError('result %d has shape %s, expected %s' % (i, tuple(o.shape), tuple(m.shape)))
+    ins, results = _addresses(mats, first, 'matrix'), _addresses(outs, first, 'result')
+    ws, ws_bytes = _hip.workspace(first.device, lib.kfac_orthogonalize_workspace_bytes(len(mats), rows, cols))
+    st = lib.kfac_orthogonalize_batched(
+        len(mats), rows, cols, kind, ins, results, len(coefficients) // 3, _hip.floats(coefficients),
+        float(eps), LATE_STEPS[first.dtype], _ws_ptr(ws), ws_bytes, _hip.stream_ptr(first.device))
+    _hip.check(st, 'kfac_orthogonalize_batched')
+
+
+def muon_update_batched(params, grads, buffers, step_sizes, keeps, momentum, nesterov, coefficients, eps):
+    """buffers = momentum * buffers + grads, params = keeps * params - step_sizes * the iterate of the
+    direction, in place, for contiguous matrices of one type (buffers: float32)."""
+    lib = _hip.load()
+    if len(params) == 0:
+        return
+    first = params[0]
+    kind = _element_type(first, 'parameter 0')
+    rows, cols = _matrix_dims(params, 'parameter')
+    for i, (p, g, b) in enumerate(zip(params, grads, buffers)):
+        if g.shape != p.shape or b.shape != p.shape:
+            raise _hip.KfacHipError('parameter %d is %s, its gradient %s and its momentum buffer %s'
+                                    % (i, tuple(p.shape), tuple(g.shape), tuple(b.shape)))
+    ps, gs = _addresses(params, first, 'parameter'), _addresses(grads, first, 'gradient')
+    bs = _addresses(buffers, first, 'momentum buffer', torch.float32)
+    written = [t.data_ptr() for t in list(params) + list(buffers) if t.numel() > 0]
+    if len(set(written)) != len(written):
+        raise _hip.KfacHipError('a parameter or momentum buffer is in the list twice')
+    ws, ws_bytes = _hip.workspace(first.device, lib.kfac_orthogonalize_workspace_bytes(len(params), rows, cols))
+    st = lib.kfac_muon_update_batched(
+        len(params), rows, cols, kind, ps, gs, bs, _hip.floats(step_sizes), _hip.floats(keeps),
+        float(momentum), int(bool(nesterov)), len(coefficients) // 3, _hip.floats(coefficients),
+        float(eps), LATE_STEPS[first.dtype], _ws_ptr(ws), ws_bytes, _hip.stream_ptr(first.device))
+    _hip.check(st, 'kfac_muon_update_batched')
