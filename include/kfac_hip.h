@@ -530,6 +530,34 @@ int kfac_muon_update_batched(int count, const int* rows, const int* cols, int ty
                              const float* coefficients, float eps, int late_steps, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* ---- Root-mean-square norm ------------------------------------------------- */
+
+/* h = x + residual, rounded to its type;  y = h / sqrt(mean(h^2) + eps) * gain  for `rows` rows of
+ * `dim` elements of `type` (0 float32, 1 bfloat16, 2 float16), rows of x and residual ldx and ldr
+ * elements apart, those of y and h contiguous.  residual may be NULL (h is x then, and may be NULL);
+ * gain is of `type`, or float32 with gain_is_float, or NULL for ones.  scale != NULL: y is in 8 bits
+ * (float8 e4m3fn), scale[row] = max |y| / 448 (1 for a row of zeros) and y holds y / scale.
+ * The normalisation in front of the layers of a decoder, as the reference has BatchNorm in front of
+ * its (curv/cov/batchnorm.py:10-49). */
+int kfac_rms_norm(int type, int gain_is_float, int64_t rows, int dim, const void* x, int64_t ldx,
+                  const void* residual, int64_t ldr, const void* gain, float eps, void* y, void* h, float* scale,
+                  void* stream);
+
+/* Backward pass of kfac_rms_norm from the gradient dy of y and dh of h (NULL: none):
+ *   dx = dh + r (gain dy - h r^2 mean(gain dy h)),  r = 1 / sqrt(mean(h^2) + eps)   (also the
+ *        residual's gradient; NULL: not wanted)
+ *   s_n = sum over the rows of sample n of dy h r        (rows / samples consecutive ones)
+ *   dgain = sum_n s_n                 (of the gain's type; NULL: not wanted)
+ *   curvature = samples * sum_n s_n^2 (float32; NULL: not wanted), the diagonal curvature of the
+ *        gain: mean of squared per-sample gradients with the n^2 rescale of curvature.py:154-158.
+ * The sums over rows are formed in an order that depends on the sizes alone.  `squares` of the
+ * workspace query: whether a curvature is wanted; without dgain and curvature no workspace is. */
+size_t kfac_rms_norm_backward_workspace_bytes(int type, int64_t rows, int dim, int samples, int squares);
+int kfac_rms_norm_backward(int type, int gain_is_float, int64_t rows, int dim, int samples, const void* dy,
+                           int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh, const void* gain,
+                           float eps, void* dx, void* dgain, float* curvature, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

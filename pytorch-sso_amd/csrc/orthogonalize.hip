@@ -6,11 +6,10 @@
 // renews the momentum and sums the squares, a second one normalises and writes the operands; then
 // three launches a step, each over the tiles of all matrices.  The last one writes the result in
 // its own type, or decays and updates the parameters.
+#include "element_types.h"
 #include "orth_core.h"
 #include "orth_plan.h"
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <string.h>
 
 #include <exception>
@@ -35,25 +34,6 @@ struct OrthMat {
 constexpr int SUM_ELEMS = 16384;                 // a workgroup of the first pass
 constexpr int SUM_MAX = 1024;                    // ... at most as many for a matrix
 constexpr int PACK_R = 64, PACK_C = 128;         // a workgroup of the second pass
-
-template <class V> struct Type;
-template <> struct Type<float> {
-  static __device__ __forceinline__ float get(float v) { return v; }
-  static __device__ __forceinline__ float put(float v) { return v; }
-};
-template <> struct Type<__hip_bfloat16> {
-  static __device__ __forceinline__ float get(__hip_bfloat16 v) { return __bfloat162float(v); }
-  static __device__ __forceinline__ __hip_bfloat16 put(float v) { return __float2bfloat16(v); }
-};
-template <> struct Type<half_t> {
-  static __device__ __forceinline__ float get(half_t v) { return (float)v; }
-  static __device__ __forceinline__ half_t put(float v) { return (half_t)v; }
-};
-
-template <class V, int N>
-struct alignas(sizeof(V) * N) Pack {
-  V v[N];
-};
 
 struct Momentum {
   float mu;
@@ -95,22 +75,22 @@ __global__ __launch_bounds__(256) void orth_sum_kernel(const OrthMat* mats, int 
         Pack<float, 4> b0 = at[0], b1 = at[1];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          b[e] = b0.v[e] = fmaf(mom.mu, b0.v[e], Type<V>::get(g.v[e]));
-          b[e + 4] = b1.v[e] = fmaf(mom.mu, b1.v[e], Type<V>::get(g.v[e + 4]));
+          b[e] = b0.v[e] = fmaf(mom.mu, b0.v[e], Element<V>::get(g.v[e]));
+          b[e + 4] = b1.v[e] = fmaf(mom.mu, b1.v[e], Element<V>::get(g.v[e + 4]));
         }
         at[0] = b0;
         at[1] = b1;
       }
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        float u = Type<V>::get(g.v[e]);
+        float u = Element<V>::get(g.v[e]);
         if (MUON) u = mom.nesterov ? fmaf(mom.mu, b[e], u) : b[e];
         s = fma((double)u, (double)u, s);
       }
     }
   } else {
     for (long i = (long)local * 256 + threadIdx.x; i < m.numel; i += (long)m.sums * 256) {
-      float u = Type<V>::get(in[i]);
+      float u = Element<V>::get(in[i]);
       if (MUON) {
         const float b = fmaf(mom.mu, m.buf[i], u);
         m.buf[i] = b;
@@ -150,7 +130,7 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
   const int R = g.R, C = g.C;
   const V* const in = (const V*)m.in;
   const auto value = [&](long i) {
-    float u = Type<V>::get(in[i]);
+    float u = Element<V>::get(in[i]);
     if (MUON) u = mom.nesterov ? fmaf(mom.mu, m.buf[i], u) : m.buf[i];
     return u * scale;
   };
@@ -184,7 +164,7 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float u = Type<V>::get(p.v[e]);
+        float u = Element<V>::get(p.v[e]);
         if (MUON) u = mom.nesterov ? fmaf(mom.mu, b[e], u) : b[e];
         v[e] = u * scale;
       }
@@ -205,7 +185,6 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
 }
 
 enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
-enum { OUT_F32 = 0, OUT_BF16 = 1, OUT_F16 = 2 };
 
 struct OrthProduct {
   half_t* base;
@@ -222,8 +201,8 @@ static_assert(sizeof(OrthProduct) <= 4096, "kernel arguments");
 template <class V>
 __device__ __forceinline__ void orth_store(const OrthMat& m, long at, float o, int update) {
   V* const out = (V*)m.out;
-  if (update) o = m.keep * Type<V>::get(out[at]) - m.step * o;
-  out[at] = Type<V>::put(o);
+  if (update) o = m.keep * Element<V>::get(out[at]) - m.step * o;
+  out[at] = Element<V>::put(o);
 }
 
 template <int T, bool SPLIT, int MODE>
@@ -294,8 +273,8 @@ __global__ __launch_bounds__(ORTH_THREADS, 2) void orth_product_kernel(const Ort
           if (row >= g.r || col >= g.c) continue;
           const long at = tall ? (long)col * g.r + row : (long)row * g.c + col;
           const float o = acc[i][j][e] * (INV * INV);
-          if (p.type == OUT_F32) orth_store<float>(m, at, o, p.update);
-          else if (p.type == OUT_BF16) orth_store<__hip_bfloat16>(m, at, o, p.update);
+          if (p.type == TYPE_F32) orth_store<float>(m, at, o, p.update);
+          else if (p.type == TYPE_BF16) orth_store<__hip_bfloat16>(m, at, o, p.update);
           else orth_store<half_t>(m, at, o, p.update);
         }
     return;
@@ -416,7 +395,7 @@ struct Call {
 int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (!sizes_ok(c.count, c.rows, c.cols)) return KFAC_ERR_ARG;
   if (c.count == 0) return KFAC_OK;
-  if (!c.in || !c.out || !c.coeffs || c.steps < 1 || c.late < 0 || c.type < OUT_F32 || c.type > OUT_F16)
+  if (!c.in || !c.out || !c.coeffs || c.steps < 1 || c.late < 0 || c.type < TYPE_F32 || c.type > TYPE_F16)
     return KFAC_ERR_ARG;
   OrthPlan plan = orth_plan(c.count, c.rows, c.cols);
   if (plan.order.empty()) return KFAC_OK;
@@ -426,7 +405,7 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
   if (!workspace || workspace_bytes < l.bytes) return KFAC_ERR_WORKSPACE;
   std::vector<OrthMat> table(plan.order.size());
   std::vector<int> sum_blocks, pack_blocks;
-  const size_t size = c.type == OUT_F32 ? 4 : 2;
+  const size_t size = type_size(c.type);
   for (OrthBatch& b : plan.batches) {
     int sum0 = 0, pack0 = 0, gi = 0, index = 0;
     for (int at = b.first; at < b.first + b.count; ++at) {
@@ -472,8 +451,8 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
       if (c.buf) launch_passes<V, true>(mats, b, c.mom, sums, sum_blocks[bi], pack_blocks[bi], c.eps, base, low, stream);
       else launch_passes<V, false>(mats, b, c.mom, sums, sum_blocks[bi], pack_blocks[bi], c.eps, base, low, stream);
     };
-    if (c.type == OUT_F32) passes((float*)nullptr);
-    else if (c.type == OUT_BF16) passes((__hip_bfloat16*)nullptr);
+    if (c.type == TYPE_F32) passes((float*)nullptr);
+    else if (c.type == TYPE_BF16) passes((__hip_bfloat16*)nullptr);
     else passes((half_t*)nullptr);
     OrthProduct p;
     memset(&p, 0, sizeof(p));

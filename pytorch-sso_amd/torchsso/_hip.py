@@ -134,6 +134,12 @@ _SIGNATURES = {
                                            c_int, c_ptr, c_size, c_ptr]),
     'kfac_muon_update_batched': (c_int, [c_int, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
                                          c_f32, c_int, c_int, c_ptr, c_f32, c_int, c_ptr, c_size, c_ptr]),
+    'kfac_rms_norm': (c_int, [c_int, c_int, c_i64, c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_f32,
+                              c_ptr, c_ptr, c_ptr, c_ptr]),
+    'kfac_rms_norm_backward_workspace_bytes': (c_size, [c_int, c_i64, c_int, c_int, c_int]),
+    'kfac_rms_norm_backward': (c_int, [c_int, c_int, c_i64, c_int, c_int, c_ptr, c_i64, c_ptr, c_i64,
+                                       c_ptr, c_i64, c_ptr, c_f32, c_ptr, c_ptr, c_ptr, c_ptr, c_size,
+                                       c_ptr]),
 }
 
 # element types of the entry points that take more than float32

@@ -847,3 +847,111 @@ def muon_update_batched(params, grads, buffers, step_sizes, keeps, momentum, nes
         float(momentum), int(bool(nesterov)), len(coefficients) // 3, _hip.floats(coefficients),
         float(eps), LATE_STEPS[first.dtype], _ws_ptr(ws), ws_bytes, _hip.stream_ptr(first.device))
     _hip.check(st, 'kfac_muon_update_batched')
+
+
+def _rows(t, dim):
+    """(2-D tensor [rows, dim] with its elements of a row side by side, elements between rows)."""
+    t = t.reshape(-1, dim)
+    if dim > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _row_ptr(t, like, what):
+    """Device address of rows of the type and on the device of `like`."""
+    if not t.is_cuda:
+        raise _hip.KfacHipError('%s is on %s: the kernels run on a HIP device only '
+                                '(no CPU path exists in this package)' % (what, t.device))
+    if t.device != like.device or t.dtype != like.dtype:
+        raise _hip.KfacHipError('%s is %s on %s, expected %s on %s'
+                                % (what, t.dtype, t.device, like.dtype, like.device))
+    return t.data_ptr()
+
+
+def _gain_args(gain, x, dim):
+    """(is float32 beside rows of another type, address) of a gain."""
+    if gain is None:
+        return 0, None
+    if tuple(gain.shape) != (dim,):
+        raise _hip.KfacHipError('gain has shape %s, expected (%d,)' % (tuple(gain.shape), dim))
+    is_float = gain.dtype == torch.float32
+    return int(is_float), _hip.typed_ptr(gain, torch.float32 if is_float else x.dtype, x.device, 'gain')
+
+
+def _norm_dim(x):
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise _hip.KfacHipError('cannot normalise a tensor of shape %s' % (tuple(x.shape),))
+    return x.shape[-1]
+
+
+def rms_norm(x, residual, gain, eps, eight_bit=False):
+    """(y, h, scale): h = x + residual (None without a residual), y = h / rms(h) * gain, in the type
+    of x or, with a float32 scale per row, in 8 bits (scale is None otherwise)."""
+    lib = _hip.load()
+    dim = _norm_dim(x)
+    kind = _element_type(x, 'input')
+    if residual is not None and residual.shape != x.shape:
+        raise _hip.KfacHipError('residual has shape %s, expected %s'
+                                % (tuple(residual.shape), tuple(x.shape)))
+    is_float, gain_ptr = _gain_args(gain, x, dim)
+    rows, ldx = _rows(x, dim)
+    x_ptr = _row_ptr(rows, x, 'input')
+    h = r_ptr = None
+    ldr = 0
+    if residual is not None:
+        res, ldr = _rows(residual, dim)
+        r_ptr = _row_ptr(res, x, 'residual')
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if eight_bit else x.dtype, device=x.device)
+    scale = None
+    if eight_bit:
+        scale = torch.empty(x.shape[:-1] + (1,), dtype=torch.float32, device=x.device)
+    st = lib.kfac_rms_norm(kind, is_float, rows.shape[0], dim, x_ptr, ldx, r_ptr, ldr, gain_ptr, float(eps),
+                           y.data_ptr(), None if h is None else h.data_ptr(),
+                           None if scale is None else scale.data_ptr(), _hip.stream_ptr(x.device))
+    _hip.check(st, 'kfac_rms_norm')
+    return y, h, scale
+
+
+def rms_norm_backward(dy, dh, h, gain, eps, samples, want_dx=True, want_dgain=True, curvature=None):
+    """(dx, dgain) of rms_norm from the gradients of y and of h (None: none), either None where it is
+    not wanted; `curvature`: a float32 tensor that receives the gain's diagonal curvature over
+    `samples` samples."""
+    lib = _hip.load()
+    dim = _norm_dim(h)
+    kind = _element_type(h, 'stream')
+    is_float, gain_ptr = _gain_args(gain, h, dim)
+    stream_rows, ldh = _rows(h, dim)
+    rows = stream_rows.shape[0]
+    for what, g in (('gradient', dy), ('stream gradient', dh)):
+        if g is not None and g.shape != h.shape:
+            raise _hip.KfacHipError('%s has shape %s, expected %s' % (what, tuple(g.shape), tuple(h.shape)))
+    if rows > 0 and (samples < 1 or rows % samples != 0):
+        raise _hip.KfacHipError('%d rows are not %d samples' % (rows, samples))
+    c_ptr = None
+    if curvature is not None:
+        if tuple(curvature.shape) != (dim,):
+            raise _hip.KfacHipError('curvature has shape %s, expected (%d,)' % (tuple(curvature.shape), dim))
+        c_ptr = _hip.typed_ptr(curvature, torch.float32, h.device, 'curvature')
+    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device) if want_dx else None
+    dgain = torch.empty_like(gain) if want_dgain and gain is not None else None
+    if rows == 0:
+        for t in (dgain, curvature):
+            if t is not None:
+                t.zero_()
+        return dx, dgain
+    dy, lddy = _rows(dy, dim)
+    args = [_row_ptr(dy, h, 'gradient'), lddy, None, 0]
+    if dh is not None:
+        dh, lddh = _rows(dh, dim)
+        args[2:] = [_row_ptr(dh, h, 'stream gradient'), lddh]
+    ws, ws_bytes = None, 0
+    if dgain is not None or curvature is not None:
+        ws, ws_bytes = _hip.workspace(h.device, lib.kfac_rms_norm_backward_workspace_bytes(
+            kind, rows, dim, samples, int(curvature is not None)))
+    st = lib.kfac_rms_norm_backward(
+        kind, is_float, rows, dim, samples, *args, _row_ptr(stream_rows, h, 'stream'), ldh, gain_ptr, float(eps),
+        None if dx is None else dx.data_ptr(), None if dgain is None else dgain.data_ptr(), c_ptr,
+        _ws_ptr(ws), ws_bytes, _hip.stream_ptr(h.device))
+    _hip.check(st, 'kfac_rms_norm_backward')
+    return dx, dgain
