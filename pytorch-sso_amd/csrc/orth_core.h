@@ -9,10 +9,12 @@
 // three v_mfma_f32_16x16x32_f16 with exact products and float32 sums, where three bf16 parts, which
 // hold any float32, take six.
 //
-// One workgroup of 256 threads (4 waves, 2 x 2) computes a T x T tile D[m][n] = sum_k P[m][k] Q[n][k].
-// Operands go from memory to LDS directly (16 bytes a lane), 32 reduction steps a stage, two stages.
+// A workgroup computes a tile D[m][n] = sum_k P[m][k] Q[n][k].  Operands go from memory to LDS
+// directly (16 bytes a lane) in stages of two planes of 32 reduction steps: the high and the low parts
+// of the same steps, or of operands in one part two successive pieces of 32.
 //   rows of an operand with k along them ("KC"): 64 bytes a row; the 16-byte groups of a row are
-//     exchanged by (row / 4) % 4, so that the 16 rows that lanes read at once lie in different banks;
+//     exchanged by its number, so that the lanes that read at once fall on different banks (they are
+//     0-3, 12-15, 20-27 and so on);
 //   an operand with k down its rows ("KM"): T columns a row, read by the transposing LDS loads, 16
 //     columns (32 bytes) of 4 rows at a time; the 32-byte groups of a row are exchanged by its number.
 #pragma once
@@ -29,84 +31,91 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr float ORTH_SCALE = 8192.f;             // 2^13
-constexpr int ORTH_THREADS = 256, ORTH_BK = 32;
+constexpr int ORTH_BK = 32;                      // reduction steps of a stage
 
-template <int T>
-struct OrthCfg {
-  static constexpr int PLANE = T * ORTH_BK * 2;         // bytes of a stage of one plane
-  static constexpr int LOADS = PLANE / 4096;            // 16-byte loads of a lane for it
-  static constexpr int NF = T / 32;                     // 16-row fragments of a wave's half
-  template <bool SPLIT>
-  static constexpr int stage() { return (SPLIT ? 4 : 2) * PLANE; }
-  template <bool SPLIT>
-  static constexpr int lds() { return 2 * stage<SPLIT>(); }
+// A TM x TN tile on WM x WN waves, STAGES of its operands in LDS.  PAIR: see orth_pair_product.
+template <int TM_, int TN_, int WM_, int WN_, int STAGES_, bool PAIR_ = false>
+struct OrthTile {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int STAGES = STAGES_;
+  static constexpr bool PAIR = PAIR_;
+  static constexpr int FM = TM / WM / 16, FN = TN / WN / 16;        // 16-row fragments of a wave
+  static constexpr int P_PLANE = TM * ORTH_BK * 2, Q_PLANE = TN * ORTH_BK * 2;
+  static constexpr int Q_AT = 2 * P_PLANE, STAGE = Q_AT + 2 * Q_PLANE;            // bytes
+  static constexpr int LDS = STAGES * STAGE;
 };
 
-// 64 lanes times 16 bytes from `base` + voff to LDS at `dst` (lane i at dst + 16 i).
-__device__ __forceinline__ void lds_load(const char* base, unsigned voff, lds_char* dst) {
-  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(base + voff),
-                                   (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+// 64 lanes times 16 bytes from `base` + voff to LDS at `dst` (lane i at dst + 16 i).  M0 holds the
+// LDS address and is written right in front of its use, here as in what the compiler makes of its
+// builtin; the builtin itself would have every transposing read wait for all loads in flight.
+__device__ __forceinline__ void lds_load(const char* base, unsigned voff, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(dst), "v"(voff), "s"(base) : "memory");
 }
-// This wave's loads into LDS have landed and its reads are done, and so it is with all others'.
+// Of this wave's loads into LDS all but the last N have landed, its reads are done, and so it is with
+// all other waves.
+template <int N>
 __device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  static_assert(N < 64, "loads in flight");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 
 // exchange of the 32-byte groups of row k of a KM stage: the 16 rows that a transposing load reads
 // at once (k, k+8, k+16, k+24 for four successive k) fall on all banks evenly
 template <int T>
 __device__ __forceinline__ int km_swap(int k) {
-  return T == 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
+  return T >= 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
 }
 
-// What a lane needs to load and read one operand of a tile.
-template <int T, bool KM>
+// What a lane needs to load and read one operand of a tile: T rows (KM: columns) of it, loaded by
+// WAVES waves, F fragments of them read by each.
+template <int T, int WAVES, int F, bool KM>
 struct OrthOperand {
-  using Cfg = OrthCfg<T>;
-  unsigned voff[Cfg::LOADS];       // byte offsets of its loads from the operand's corner
+  static constexpr int PLANE = T * ORTH_BK * 2, LOADS = PLANE / (1024 * WAVES);
+  static_assert(LOADS >= 1, "waves");
+  unsigned voff[LOADS];            // byte offsets of its loads from the operand's corner
   const char* base;                // the corner, at the next stage
   long step;                       // bytes to the next stage
-  long lo;                         // bytes from the high to the low plane
-  unsigned frag[KM ? Cfg::NF : 1]; // LDS byte offsets of its fragments
+  long second;                     // bytes from the first to the second plane
+  unsigned frag[KM ? F : 1];       // LDS byte offsets of its fragments
 
-  // rows [row0, row0 + T) (KM: columns) of a plane with row length ld; `side`: which half of them
-  // this wave computes
+  // rows [row0, row0 + T) (KM: columns) of a matrix with row length ld, its low parts lo_halves behind
+  // its high ones (0: it has one part); `side`: which F fragments of them this wave computes
   __device__ __forceinline__ void init(const half_t* plane, long lo_halves, int ld, int row0, int side, int wave,
                                        int lane) {
-    lo = 2 * lo_halves;
+    const long piece = (long)ORTH_BK * 2 * (KM ? ld : 1);
+    second = lo_halves ? 2 * lo_halves : piece;
+    step = lo_halves ? piece : 2 * piece;
 #pragma unroll
-    for (int j = 0; j < Cfg::LOADS; ++j) {
-      const int i = wave * Cfg::LOADS + j;               // which KiB of the stage
+    for (int j = 0; j < LOADS; ++j) {
+      const int i = wave * LOADS + j;               // which KiB of the stage
       if (KM) {
         constexpr int LANES = T / 8, ROWS = 64 / LANES;  // lanes a row, rows a load
         const int k = i * ROWS + lane / LANES, slot = lane % LANES;
         voff[j] = (unsigned)k * ld * 2 + ((slot ^ (km_swap<T>(k) << 1)) << 4);
       } else {
-        const int row = i * 16 + (lane >> 2), group = (lane & 3) ^ ((row >> 2) & 3);
+        const int row = i * 16 + (lane >> 2), group = (lane & 3) ^ (-(row >> 2) & 3);
         voff[j] = (unsigned)row * ld * 2 + (group << 4);
       }
     }
     if (KM) {
       base = (const char*)(plane + row0);
-      step = (long)ORTH_BK * ld * 2;
       const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
 #pragma unroll
-      for (int f = 0; f < Cfg::NF; ++f)
-        frag[f] = k * T * 2 + (((side * Cfg::NF + f) ^ km_swap<T>(k)) << 5) + ((lane & 3) << 3);
+      for (int f = 0; f < F; ++f)
+        frag[f] = k * T * 2 + (((side * F + f) ^ km_swap<T>(k)) << 5) + ((lane & 3) << 3);
     } else {
       base = (const char*)(plane + (long)row0 * ld);
-      step = ORTH_BK * 2;
-      frag[0] = side * Cfg::NF * 1024 + (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) << 4);
+      frag[0] = side * F * 1024 + (lane & 15) * 64 + (((lane >> 4) ^ (-(lane >> 2) & 3)) << 4);
     }
   }
 
-  template <bool SPLIT>
-  __device__ __forceinline__ void load(lds_char* dst, int wave) {
+  __device__ __forceinline__ void load(unsigned dst, int wave) {
 #pragma unroll
-    for (int p = 0; p < (SPLIT ? 2 : 1); ++p)
+    for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int j = 0; j < Cfg::LOADS; ++j)
-        lds_load(base + p * lo, voff[j], dst + p * Cfg::PLANE + (wave * Cfg::LOADS + j) * 1024);
+      for (int j = 0; j < LOADS; ++j)
+        lds_load(base + p * second, voff[j], dst + p * PLANE + (wave * LOADS + j) * 1024);
     base += step;
   }
 
@@ -121,54 +130,118 @@ struct OrthOperand {
   }
 };
 
-// acc[i][j]: 16 x 16 block of fragment i of P against fragment j of Q; of each block lane l holds
-// D[4 (l / 16) + 0..3][l % 16].
-template <int T, bool SPLIT, bool P_KM>
-__device__ __forceinline__ void orth_tile_product(OrthOperand<T, P_KM>& P, OrthOperand<T, false>& Q, int steps,
-                                                  lds_char* lds, int wave,
-                                                  f4 (&acc)[OrthCfg<T>::NF][OrthCfg<T>::NF]) {
-  using Cfg = OrthCfg<T>;
-  constexpr int NF = Cfg::NF, STAGE = Cfg::template stage<SPLIT>(), Q_AT = (SPLIT ? 2 : 1) * Cfg::PLANE;
+// The blocks of fragments i0 ... i0 + N - 1 of P against all of Q.
+template <bool SPLIT, int N, int FM, int FN>
+__device__ __forceinline__ void orth_mfma(const h8 (&p)[2][N], const h8 (&q)[2][FN], f4 (&acc)[FM][FN], int i0) {
 #pragma unroll
-  for (int i = 0; i < NF; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int j = 0; j < NF; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-  P.template load<SPLIT>(lds, wave);
-  Q.template load<SPLIT>(lds + Q_AT, wave);
-  stage_barrier();
-  for (int s = 0; s < steps; ++s) {
-    const int cur = (s & 1) * STAGE, next = STAGE - cur;
-    lds_char* const ps = lds + cur;
-    lds_char* const qs = ps + Q_AT;
-    h8 ph[NF], pl[NF], qh[NF], ql[NF];
-    // (P first: a transposing read behind a load into LDS would wait for it)
-#pragma unroll
-    for (int f = 0; f < NF; ++f) ph[f] = P.read(ps, f);
-    if (SPLIT) {
-#pragma unroll
-      for (int f = 0; f < NF; ++f) pl[f] = P.read(ps + Cfg::PLANE, f);
-    }
-    if (s + 1 < steps) {
-      P.template load<SPLIT>(lds + next, wave);
-      Q.template load<SPLIT>(lds + next + Q_AT, wave);
-    }
-#pragma unroll
-    for (int f = 0; f < NF; ++f) qh[f] = Q.read(qs, f);
-    if (SPLIT) {
-#pragma unroll
-      for (int f = 0; f < NF; ++f) ql[f] = Q.read(qs + Cfg::PLANE, f);
-    }
-#pragma unroll
-    for (int i = 0; i < NF; ++i)
-#pragma unroll
-      for (int j = 0; j < NF; ++j) {
-        if (SPLIT) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
-        }
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+    for (int j = 0; j < FN; ++j) {
+      f4& d = acc[i0 + i][j];
+      if (SPLIT) {
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[1][i], q[0][j], d, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0][i], q[1][j], d, 0, 0, 0);
+      } else {
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[1][i], q[1][j], d, 0, 0, 0);
       }
-    stage_barrier();
+      d = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0][i], q[0][j], d, 0, 0, 0);
+    }
+}
+
+template <int N, class OP>
+__device__ __forceinline__ void orth_read(const OP& op, lds_char* stage, int f0, h8 (&v)[2][N]) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int f = 0; f < N; ++f) v[p][f] = op.read(stage + p * OP::PLANE, f0 + f);
+}
+
+template <class TILE>
+__device__ __forceinline__ void orth_clear(f4 (&acc)[TILE::FM][TILE::FN]) {
+#pragma unroll
+  for (int i = 0; i < TILE::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < TILE::FN; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+}
+
+// acc[i][j]: 16 x 16 block of fragment i of P against fragment j of Q over `steps` stages; of each
+// block lane l holds D[4 (l / 16) + 0..3][l % 16].  One barrier a stage, behind which the stage that
+// is STAGES - 1 ahead is asked for.
+template <class TILE, bool SPLIT, class OP_P, class OP_Q>
+__device__ __forceinline__ void orth_product(OP_P& P, OP_Q& Q, int steps, lds_char* lds, int wave,
+                                             f4 (&acc)[TILE::FM][TILE::FN]) {
+  constexpr int S = TILE::STAGES, LOADS = 2 * (OP_P::LOADS + OP_Q::LOADS);
+  orth_clear<TILE>(acc);
+  const unsigned at = (unsigned)(uintptr_t)lds;
+  const auto load = [&](int stage) {
+    P.load(at + stage * TILE::STAGE, wave);
+    Q.load(at + stage * TILE::STAGE + TILE::Q_AT, wave);
+  };
+  int ahead = 0;                           // stages asked for
+  for (; ahead < S - 1 && ahead < steps; ++ahead) load(ahead);
+  int cur = 0, into = S - 1;
+  for (int s = 0; s < steps; ++s) {
+    if (ahead - s == S - 1) stage_barrier<(S - 2) * LOADS>();
+    else stage_barrier<0>();
+    if (ahead < steps) {
+      load(into);
+      ++ahead;
+    }
+    lds_char* const stage = lds + cur * TILE::STAGE;
+    h8 p[2][TILE::FM], q[2][TILE::FN];
+    orth_read(P, stage, 0, p);
+    orth_read(Q, stage + TILE::Q_AT, 0, q);
+    orth_mfma<SPLIT>(p, q, acc, 0);
+    into = cur;
+    cur = cur + 1 == S ? 0 : cur + 1;
+  }
+}
+
+// The same for a workgroup of eight waves that has the compute unit to itself, two waves on every
+// SIMD: while one reads its fragments of a stage, the other multiplies those that it has read, and
+// they change places at a barrier.  Stage s is read by the first four waves in phase 2s and by the
+// others in phase 2s + 1, so that its successor, in the other half of the LDS, may be asked for from
+// phase 2s on and has to be there at the end of phase 2s + 1.
+template <class TILE, bool SPLIT, class OP_P, class OP_Q>
+__device__ __forceinline__ void orth_pair_product(OP_P& P, OP_Q& Q, int steps, lds_char* lds, int wave,
+                                                  f4 (&acc)[TILE::FM][TILE::FN]) {
+  static_assert(TILE::WAVES == 8 && TILE::STAGES == 2, "waves");
+  orth_clear<TILE>(acc);
+  const unsigned at = (unsigned)(uintptr_t)lds;
+  const auto load = [&](int stage) {
+    P.load(at + stage * TILE::STAGE, wave);
+    Q.load(at + stage * TILE::STAGE + TILE::Q_AT, wave);
+  };
+  h8 p[2][TILE::FM], q[2][TILE::FN];
+  const auto read = [&](int stage) {
+    orth_read(P, lds + stage * TILE::STAGE, 0, p);
+    orth_read(Q, lds + stage * TILE::STAGE + TILE::Q_AT, 0, q);
+  };
+  constexpr int LOADS = 2 * (OP_P::LOADS + OP_Q::LOADS);
+  load(0);
+  stage_barrier<0>();
+  if (wave < 4) {
+    for (int s = 0; s < steps; ++s) {
+      read(s & 1);
+      if (s + 1 < steps) load((s + 1) & 1);
+      stage_barrier<LOADS>();
+      __builtin_amdgcn_sched_barrier(0);
+      orth_mfma<SPLIT>(p, q, acc, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      stage_barrier<0>();
+    }
+  } else {
+    if (steps > 1) load(1);
+    stage_barrier<LOADS>();
+    for (int s = 0; s < steps; ++s) {
+      read(s & 1);
+      stage_barrier<0>();
+      if (s + 2 < steps) load(s & 1);
+      __builtin_amdgcn_sched_barrier(0);
+      orth_mfma<SPLIT>(p, q, acc, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (s + 1 < steps) stage_barrier<LOADS>();
+    }
   }
 }
 

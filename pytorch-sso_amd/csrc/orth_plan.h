@@ -43,9 +43,9 @@ constexpr long ORTH_BATCH_HALVES = 1L << 29;     // a batch is closed when it ne
 
 inline int orth_pad(int n, int tile) { return (n + tile - 1) / tile * tile; }
 
-// 64-wide tiles where the smaller side is at most this
-constexpr int ORTH_SMALL_SIDE = 128;
-inline int orth_tile(int r) { return r <= ORTH_SMALL_SIDE ? 64 : 128; }
+// sides are padded to multiples of 64, 128 or 256 by the smaller of them
+constexpr int ORTH_SMALL_SIDE = 128, ORTH_MID_SIDE = 512;
+inline int orth_tile(int r) { return r <= ORTH_SMALL_SIDE ? 64 : r <= ORTH_MID_SIDE ? 128 : 256; }
 
 inline OrthPlan orth_plan(int count, const int* rows, const int* cols) {
   OrthPlan p;
@@ -93,22 +93,37 @@ inline OrthPlan orth_plan(int count, const int* rows, const int* cols) {
 }
 
 // Tiles of one matrix: of a symmetric product those on and below the diagonal, or all of B X.
-inline int orth_symmetric_tiles(const OrthGroup& g) {
-  const int t = g.R / g.tile;
-  return t * (t + 1) / 2;
+inline long orth_tiles(const OrthGroup& g, int tile, bool symmetric) {
+  const long t = g.R / tile;
+  return symmetric ? t * (t + 1) / 2 : t * (g.C / tile);
 }
-inline int orth_full_tiles(const OrthGroup& g) { return (g.R / g.tile) * (g.C / g.tile); }
 
 // Workgroups of a launch over the groups; sets their tile0 and tiles.  Workgroups go to the eight
 // dies in turn, and a group starts at a multiple of eight.
-inline int orth_launch(std::vector<OrthGroup>& groups, bool symmetric) {
+inline int orth_launch(std::vector<OrthGroup>& groups, int tile, bool symmetric) {
   int at = 0;
   for (OrthGroup& g : groups) {
     g.tile0 = at;
-    g.tiles = g.count * (symmetric ? orth_symmetric_tiles(g) : orth_full_tiles(g));
+    g.tiles = (int)(g.count * orth_tiles(g, tile, symmetric));
     at += (g.tiles + 7) / 8 * 8;
   }
   return at;
+}
+
+// The tiles that a product of the batch is computed in: 256 wide, one workgroup to a compute unit; 128
+// wide, two to a unit or, where there are not as many tiles, one with more stages in flight; 64 wide.
+enum { ORTH_LARGE, ORTH_MID, ORTH_DEEP, ORTH_SMALL };
+constexpr long ORTH_UNITS = 256;
+inline int orth_pick_tile(const OrthBatch& b, bool symmetric) {
+  const auto tiles = [&](int tile) {
+    long n = 0;
+    for (const OrthGroup& g : b.groups) n += g.count * orth_tiles(g, tile, symmetric);
+    return n;
+  };
+  if (b.tile == 64) return ORTH_SMALL;
+  if (b.tile == 256 && tiles(256) >= ORTH_UNITS / 2) return ORTH_LARGE;
+  const long n = tiles(128);
+  return n > ORTH_UNITS ? ORTH_MID : n > ORTH_UNITS / 2 ? ORTH_DEEP : ORTH_SMALL;
 }
 
 }  // namespace kfac

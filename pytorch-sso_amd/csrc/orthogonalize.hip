@@ -205,11 +205,16 @@ __device__ __forceinline__ void orth_store(const OrthMat& m, long at, float o, i
   out[at] = Element<V>::put(o);
 }
 
-template <int T, bool SPLIT, int MODE>
-__global__ __launch_bounds__(ORTH_THREADS, 2) void orth_product_kernel(const OrthProduct p) {
+typedef OrthTile<64, 64, 2, 2, 4> SmallTile;
+typedef OrthTile<128, 128, 2, 2, 2> MidTile;
+typedef OrthTile<128, 128, 2, 2, 4> DeepTile;
+typedef OrthTile<256, 256, 2, 4, 2, true> LargeTile;
+
+template <class TILE, bool SPLIT, int MODE>
+__global__ __launch_bounds__(TILE::THREADS, 2) void orth_product_kernel(const OrthProduct p) {
   extern __shared__ __align__(16) char smem[];
-  using Cfg = OrthCfg<T>;
-  constexpr int NF = Cfg::NF;
+  constexpr int T = TILE::TM, FM = TILE::FM, FN = TILE::FN;
+  static_assert(TILE::TM == TILE::TN, "symmetric products");
   constexpr bool SYM = MODE == GRAM || MODE == POLY;
   int gi = 0;
   while (gi + 1 < p.n && p.g[gi + 1].tile0 <= (int)blockIdx.x) ++gi;
@@ -233,40 +238,42 @@ __global__ __launch_bounds__(ORTH_THREADS, 2) void orth_product_kernel(const Ort
     tn = u % rt;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / TILE::WN, wn = wave % TILE::WN;
   const long XS = (long)R * C, AS = (long)R * R;
   half_t* const x = p.base + g.x[p.from] + k * 2 * XS;
   half_t* const a = p.base + g.a + k * 2 * AS;
   half_t* const b = p.base + g.b + k * 2 * AS;
-  OrthOperand<T, !SYM> P;
-  OrthOperand<T, false> Q;
+  OrthOperand<TILE::TM, TILE::WAVES, FM, !SYM> P;
+  OrthOperand<TILE::TN, TILE::WAVES, FN, false> Q;
   int steps;
   if (MODE == GRAM) {
-    P.init(x, XS, C, tm * T, wm, wave, lane);
-    Q.init(x, XS, C, tn * T, wn, wave, lane);
-    steps = C / ORTH_BK;
+    P.init(x, SPLIT ? XS : 0, C, tm * T, wm, wave, lane);
+    Q.init(x, SPLIT ? XS : 0, C, tn * T, wn, wave, lane);
+    steps = C;
   } else if (MODE == POLY) {
-    P.init(a, AS, R, tm * T, wm, wave, lane);
-    Q.init(a, AS, R, tn * T, wn, wave, lane);
-    steps = R / ORTH_BK;
+    P.init(a, SPLIT ? AS : 0, R, tm * T, wm, wave, lane);
+    Q.init(a, SPLIT ? AS : 0, R, tn * T, wn, wave, lane);
+    steps = R;
   } else {
-    P.init(x, XS, C, tm * T, wm, wave, lane);          // (columns of X)
-    Q.init(b, AS, R, tn * T, wn, wave, lane);
-    steps = R / ORTH_BK;
+    P.init(x, SPLIT ? XS : 0, C, tm * T, wm, wave, lane);          // (columns of X)
+    Q.init(b, SPLIT ? AS : 0, R, tn * T, wn, wave, lane);
+    steps = R;
   }
+  steps /= SPLIT ? ORTH_BK : 2 * ORTH_BK;
   lds_char* const lds = (lds_char*)smem;
-  f4 acc[NF][NF];
-  orth_tile_product<T, SPLIT, !SYM>(P, Q, steps, lds, wave, acc);
+  f4 acc[FM][FN];
+  if constexpr (TILE::PAIR) orth_pair_product<TILE, SPLIT>(P, Q, steps, lds, wave, acc);
+  else orth_product<TILE, SPLIT>(P, Q, steps, lds, wave, acc);
 
   constexpr float INV = 1.f / ORTH_SCALE;
-  const int m0 = tm * T + wm * (T / 2) + 4 * (lane >> 4), n0 = tn * T + wn * (T / 2) + (lane & 15);
+  const int m0 = tm * T + wm * FM * 16 + 4 * (lane >> 4), n0 = tn * T + wn * FN * 16 + (lane & 15);
   if (MODE == LAST) {
     const OrthMat m = p.mats[g.first + k];
     const bool tall = m.rows > m.cols;
 #pragma unroll
-    for (int i = 0; i < NF; ++i)
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < NF; ++j)
+      for (int j = 0; j < FN; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = n0 + 16 * j, col = m0 + 16 * i + e;
@@ -284,9 +291,9 @@ __global__ __launch_bounds__(ORTH_THREADS, 2) void orth_product_kernel(const Ort
   const int ld = SYM ? R : C;
   half_t* const out = MODE == GRAM ? a : MODE == POLY ? b : p.base + g.x[1 - p.from] + k * 2 * XS;
 #pragma unroll
-  for (int i = 0; i < NF; ++i)
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
+    for (int j = 0; j < FN; ++j) {
       const int m = m0 + 16 * i, n = n0 + 16 * j;
       f4 v = acc[i][j] * INV;
       if (MODE == POLY) {
@@ -315,33 +322,42 @@ __global__ __launch_bounds__(ORTH_THREADS, 2) void orth_product_kernel(const Ort
     }
 }
 
-template <int T, bool SPLIT, int MODE>
-bool launch_product(OrthProduct& p, OrthBatch& b, hipStream_t stream) {
-  const int grid = orth_launch(b.groups, MODE == GRAM || MODE == POLY);
+template <class TILE, bool SPLIT, int MODE>
+bool launch_tiles(OrthProduct& p, OrthBatch& b, hipStream_t stream) {
+  const int grid = orth_launch(b.groups, TILE::TM, MODE == GRAM || MODE == POLY);
   p.n = (int)b.groups.size();
   std::copy(b.groups.begin(), b.groups.end(), p.g);
-  constexpr int lds = OrthCfg<T>::template lds<SPLIT>();
-  const auto kernel = orth_product_kernel<T, SPLIT, MODE>;
+  constexpr int lds = TILE::LDS;
+  const auto kernel = orth_product_kernel<TILE, SPLIT, MODE>;
   if (!enable_large_lds((const void*)kernel, lds)) return false;
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(ORTH_THREADS), lds, stream, p);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(TILE::THREADS), lds, stream, p);
   return true;
 }
 
-template <int T>
+template <class TILE, int MODE>
+bool launch_parts(OrthProduct& p, OrthBatch& b, bool split, hipStream_t stream) {
+  return split ? launch_tiles<TILE, true, MODE>(p, b, stream) : launch_tiles<TILE, false, MODE>(p, b, stream);
+}
+
+template <int MODE>
+bool launch_product(OrthProduct& p, OrthBatch& b, bool split, hipStream_t stream) {
+  switch (orth_pick_tile(b, MODE == GRAM || MODE == POLY)) {
+    case ORTH_SMALL: return launch_parts<SmallTile, MODE>(p, b, split, stream);
+    case ORTH_DEEP: return launch_parts<DeepTile, MODE>(p, b, split, stream);
+    case ORTH_MID: return launch_parts<MidTile, MODE>(p, b, split, stream);
+    default: return launch_parts<LargeTile, MODE>(p, b, split, stream);
+  }
+}
+
 bool launch_step(OrthProduct& p, OrthBatch& b, const float* coeffs, bool split, bool next_split, bool last,
                  hipStream_t stream) {
   p.ca = coeffs[0];
   p.cb = coeffs[1];
   p.cc = coeffs[2];
   p.low = split;
-  if (!(split ? launch_product<T, true, GRAM>(p, b, stream) : launch_product<T, false, GRAM>(p, b, stream)))
-    return false;
-  if (!(split ? launch_product<T, true, POLY>(p, b, stream) : launch_product<T, false, POLY>(p, b, stream)))
-    return false;
+  if (!launch_product<GRAM>(p, b, split, stream) || !launch_product<POLY>(p, b, split, stream)) return false;
   p.low = next_split;
-  if (last)
-    return split ? launch_product<T, true, LAST>(p, b, stream) : launch_product<T, false, LAST>(p, b, stream);
-  return split ? launch_product<T, true, APPLY>(p, b, stream) : launch_product<T, false, APPLY>(p, b, stream);
+  return last ? launch_product<LAST>(p, b, split, stream) : launch_product<APPLY>(p, b, split, stream);
 }
 
 template <class V, bool MUON>
@@ -463,9 +479,7 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
     for (int k = 0; k < c.steps; ++k) {
       const bool split = c.steps - k > c.late, next = c.steps - k - 1 > c.late, last = k + 1 == c.steps;
       p.from = k & 1;
-      const bool ok = b.tile == 64 ? launch_step<64>(p, b, c.coeffs + 3 * k, split, next, last, stream)
-                                   : launch_step<128>(p, b, c.coeffs + 3 * k, split, next, last, stream);
-      if (!ok) return KFAC_ERR_LAUNCH;
+      if (!launch_step(p, b, c.coeffs + 3 * k, split, next, last, stream)) return KFAC_ERR_LAUNCH;
     }
   }
   return launch_status();

@@ -96,7 +96,7 @@ int main() {
       }
       if (end > p.halves || count != b.count) return 7;
       for (int sym = 0; sym < 2; ++sym) {
-        const int grid = orth_launch(b.groups, sym);
+        const int grid = orth_launch(b.groups, b.tile, sym);
         int to = 0;
         for (auto& g : b.groups) {
           if (g.tile0 != to || g.tile0 % 8) return 8;
