@@ -9,12 +9,16 @@
 // three v_mfma_f32_16x16x32_f16 with exact products and float32 sums, where three bf16 parts, which
 // hold any float32, take six.
 //
+// In memory a row of a matrix in two parts is made of pieces of 32 elements, 64 bytes of high parts and
+// 64 of low ones, so that what a tile reads of a row at a time, both parts of 32 elements, is one cache
+// line; in one part it is just a row (a line is 64 elements).
+//
 // A workgroup computes a tile D[m][n] = sum_k P[m][k] Q[n][k].  Operands go from memory to LDS
-// directly (16 bytes a lane) in stages of two planes of 32 reduction steps: the high and the low parts
-// of the same steps, or of operands in one part two successive pieces of 32.
-//   rows of an operand with k along them ("KC"): 64 bytes a row; the 16-byte groups of a row are
-//     exchanged by its number, so that the lanes that read at once fall on different banks (they are
-//     0-3, 12-15, 20-27 and so on);
+// directly (16 bytes a lane, whole cache lines) in stages of two planes of 32 reduction steps: the high
+// and the low parts of the same steps, or of operands in one part two successive pieces of 32.
+//   rows of an operand with k along them ("KC"): 128 bytes a row, both planes; the 16-byte groups of a
+//     row are exchanged by half its number, so that the lanes that read at once fall on different banks
+//     (they are 0-3, 12-15, 20-27 and so on);
 //   an operand with k down its rows ("KM"): T columns a row, read by the transposing LDS loads, 16
 //     columns (32 bytes) of 4 rows at a time; the 32-byte groups of a row are exchanged by its number.
 #pragma once
@@ -33,16 +37,22 @@ typedef __attribute__((address_space(3))) char lds_char;
 constexpr float ORTH_SCALE = 8192.f;             // 2^13
 constexpr int ORTH_BK = 32;                      // reduction steps of a stage
 
-// A TM x TN tile on WM x WN waves, STAGES of its operands in LDS.  PAIR: see orth_pair_product.
-template <int TM_, int TN_, int WM_, int WN_, int STAGES_, bool PAIR_ = false>
+// A TM x TN tile on WM x WN waves, STAGES of its operands in LDS.  PAIR: see orth_pair_product.  WK: as
+// many teams of WM x WN waves, each with stages of its own and every WK-th piece of the reduction.
+template <int TM_, int TN_, int WM_, int WN_, int STAGES_, bool PAIR_ = false, int WK_ = 1>
 struct OrthTile {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WK = WK_, WAVES = WM * WN, TEAM = 64 * WAVES, THREADS = TEAM * WK;
   static constexpr int STAGES = STAGES_;
   static constexpr bool PAIR = PAIR_;
   static constexpr int FM = TM / WM / 16, FN = TN / WN / 16;        // 16-row fragments of a wave
   static constexpr int P_PLANE = TM * ORTH_BK * 2, Q_PLANE = TN * ORTH_BK * 2;
   static constexpr int Q_AT = 2 * P_PLANE, STAGE = Q_AT + 2 * Q_PLANE;            // bytes
-  static constexpr int LDS = STAGES * STAGE;
+  static constexpr int LDS = WK * STAGES * STAGE;
+  // behind the product: the sums of the other teams, then a piece for each wave that writes the tile
+  static constexpr int SUMS = (WK - 1) * FM * FN * TEAM * 16;
+  static constexpr int M_PITCH = FM * 64 + 16, N_PITCH = FN * 64 + 16;
+  static constexpr int WRITE = 16 * (M_PITCH > N_PITCH ? M_PITCH : N_PITCH);
+  static_assert(SUMS + WAVES * WRITE <= LDS, "room to write a tile");
 };
 
 // 64 lanes times 16 bytes from `base` + voff to LDS at `dst` (lane i at dst + 16 i).  M0 holds the
@@ -60,100 +70,95 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 
-// exchange of the 32-byte groups of row k of a KM stage: the 16 rows that a transposing load reads
-// at once (k, k+8, k+16, k+24 for four successive k) fall on all banks evenly
-template <int T>
+// exchange of the 32-byte groups of row k of a KM stage of rows of BYTES: the 16 rows that a transposing
+// load reads at once (k, k+8, k+16, k+24 for four successive k) fall on all banks evenly
+template <int BYTES>
 __device__ __forceinline__ int km_swap(int k) {
-  return T >= 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
+  return BYTES >= 256 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
 }
 
 // What a lane needs to load and read one operand of a tile: T rows (KM: columns) of it, loaded by
 // WAVES waves, F fragments of them read by each.
-template <int T, int WAVES, int F, bool KM>
+template <int T, int WAVES, int F, bool KM, bool SPLIT>
 struct OrthOperand {
-  static constexpr int PLANE = T * ORTH_BK * 2, LOADS = PLANE / (1024 * WAVES);
+  static constexpr int STAGE = T * ORTH_BK * 4, LOADS = STAGE / (1024 * WAVES);
   static_assert(LOADS >= 1, "waves");
+  // KM: bytes of a row, which holds both parts (pieces of 32 columns of each in turn) or one
+  static constexpr int ROW = T * (SPLIT ? 4 : 2);
+  static constexpr int SECOND = KM ? (SPLIT ? 64 : ORTH_BK * ROW) : 64;      // from the first plane to the second
   unsigned voff[LOADS];            // byte offsets of its loads from the operand's corner
   const char* base;                // the corner, at the next stage
   long step;                       // bytes to the next stage
-  long second;                     // bytes from the first to the second plane
-  unsigned frag[KM ? F : 1];       // LDS byte offsets of its fragments
+  unsigned frag[KM ? 2 * F : 2];   // LDS byte offsets of its fragments in the planes (KC: of the first ones)
 
-  // rows [row0, row0 + T) (KM: columns) of a matrix with row length ld, its low parts lo_halves behind
-  // its high ones (0: it has one part); `side`: which F fragments of them this wave computes
-  __device__ __forceinline__ void init(const half_t* plane, long lo_halves, int ld, int row0, int side, int wave,
-                                       int lane) {
-    const long piece = (long)ORTH_BK * 2 * (KM ? ld : 1);
-    second = lo_halves ? 2 * lo_halves : piece;
-    step = lo_halves ? piece : 2 * piece;
+  // rows [row0, row0 + T) (KM: columns) of a matrix of rows of `ld` elements; `side`: which F fragments
+  // of them this wave computes
+  __device__ __forceinline__ void init(const half_t* matrix, int ld, int row0, int side, int wave, int lane) {
+    const int row_bytes = ld * (SPLIT ? 4 : 2);
+    step = !KM ? 128 : (long)(SPLIT ? 1 : 2) * ORTH_BK * row_bytes;
+    base = (const char*)matrix + (KM ? (long)row0 * (SPLIT ? 4 : 2) : (long)row0 * row_bytes);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-      const int i = wave * LOADS + j;               // which KiB of the stage
-      if (KM) {
-        constexpr int LANES = T / 8, ROWS = 64 / LANES;  // lanes a row, rows a load
-        const int k = i * ROWS + lane / LANES, slot = lane % LANES;
-        voff[j] = (unsigned)k * ld * 2 + ((slot ^ (km_swap<T>(k) << 1)) << 4);
-      } else {
-        const int row = i * 16 + (lane >> 2), group = (lane & 3) ^ (-(row >> 2) & 3);
-        voff[j] = (unsigned)row * ld * 2 + (group << 4);
-      }
+      const int at = ((wave * LOADS + j) * 64 + lane) * 16;           // where this lane's bytes go
+      constexpr int BYTES = KM ? ROW : 128;
+      const int row = at / BYTES, group = at % BYTES / 16;
+      voff[j] = (unsigned)row * row_bytes + 16 * (group ^ (KM ? km_swap<ROW>(row) << 1 : (row >> 1) & 7));
     }
-    if (KM) {
-      base = (const char*)(plane + row0);
-      const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
 #pragma unroll
-      for (int f = 0; f < F; ++f)
-        frag[f] = k * T * 2 + (((side * F + f) ^ km_swap<T>(k)) << 5) + ((lane & 3) << 3);
-    } else {
-      base = (const char*)(plane + (long)row0 * ld);
-      frag[0] = side * F * 1024 + (lane & 15) * 64 + (((lane >> 4) ^ (-(lane >> 2) & 3)) << 4);
+    for (int p = 0; p < 2; ++p) {
+      if (KM) {
+        const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+          const int c = side * F + f;                                 // which 16 columns
+          const int group = SPLIT ? (c >> 1) * 4 + 2 * p + (c & 1) : c;
+          frag[p * F + f] = (SPLIT ? 0 : p * SECOND) + k * ROW + ((group ^ km_swap<ROW>(k)) << 5) + ((lane & 3) << 3);
+        }
+      } else {
+        const int row = lane & 15, group = 4 * p + (lane >> 4);
+        frag[p] = side * F * 2048 + row * 128 + ((group ^ ((row >> 1) & 7)) << 4);
+      }
     }
   }
 
   __device__ __forceinline__ void load(unsigned dst, int wave) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j)
-        lds_load(base + p * second, voff[j], dst + p * PLANE + (wave * LOADS + j) * 1024);
+    for (int j = 0; j < LOADS; ++j) lds_load(base, voff[j], dst + (wave * LOADS + j) * 1024);
     base += step;
   }
 
-  __device__ __forceinline__ h8 read(lds_char* stage, int f) const {
+  __device__ __forceinline__ h8 read(lds_char* stage, int plane, int f) const {
     if (KM) {
-      lds_char* const at = stage + frag[f];
+      lds_char* const at = stage + frag[plane * F + f];
       const h4s u = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) h4s*)at);
-      const h4s v = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) h4s*)(at + 4 * T * 2));
+      const h4s v = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) h4s*)(at + 4 * ROW));
       return __builtin_bit_cast(h8, (h8s)__builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    return *(__attribute__((address_space(3))) h8*)(stage + frag[0] + f * 1024);
+    return *(__attribute__((address_space(3))) h8*)(stage + frag[plane] + f * 2048);
   }
 };
 
-// The blocks of fragments i0 ... i0 + N - 1 of P against all of Q.
+// The blocks of fragments i0 ... i0 + N - 1 of P against all of Q, one of the partial products after
+// the other: an instruction waits for the one before it that adds to the same block.
 template <bool SPLIT, int N, int FM, int FN>
 __device__ __forceinline__ void orth_mfma(const h8 (&p)[2][N], const h8 (&q)[2][FN], f4 (&acc)[FM][FN], int i0) {
+  constexpr int TERMS = SPLIT ? 3 : 2;
+  constexpr int PP[3] = {1, 0, 0}, QQ[3] = {SPLIT ? 0 : 1, SPLIT ? 1 : 0, 0};
 #pragma unroll
-  for (int i = 0; i < N; ++i)
+  for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      f4& d = acc[i0 + i][j];
-      if (SPLIT) {
-        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[1][i], q[0][j], d, 0, 0, 0);
-        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0][i], q[1][j], d, 0, 0, 0);
-      } else {
-        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[1][i], q[1][j], d, 0, 0, 0);
-      }
-      d = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0][i], q[0][j], d, 0, 0, 0);
-    }
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[i0 + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[PP[t]][i], q[QQ[t]][j], acc[i0 + i][j], 0, 0, 0);
 }
 
 template <int N, class OP>
-__device__ __forceinline__ void orth_read(const OP& op, lds_char* stage, int f0, h8 (&v)[2][N]) {
+__device__ __forceinline__ void orth_read(const OP& op, lds_char* stage, h8 (&v)[2][N]) {
 #pragma unroll
   for (int p = 0; p < 2; ++p)
 #pragma unroll
-    for (int f = 0; f < N; ++f) v[p][f] = op.read(stage + p * OP::PLANE, f0 + f);
+    for (int f = 0; f < N; ++f) v[p][f] = op.read(stage, p, f);
 }
 
 template <class TILE>
@@ -166,34 +171,59 @@ __device__ __forceinline__ void orth_clear(f4 (&acc)[TILE::FM][TILE::FN]) {
 
 // acc[i][j]: 16 x 16 block of fragment i of P against fragment j of Q over `steps` stages; of each
 // block lane l holds D[4 (l / 16) + 0..3][l % 16].  One barrier a stage, behind which the stage that
-// is STAGES - 1 ahead is asked for.
+// is STAGES - 1 ahead is asked for.  With several teams the first one ends up with the sum.
 template <class TILE, bool SPLIT, class OP_P, class OP_Q>
-__device__ __forceinline__ void orth_product(OP_P& P, OP_Q& Q, int steps, lds_char* lds, int wave,
+__device__ __forceinline__ void orth_product(OP_P& P, OP_Q& Q, int steps, lds_char* lds, int wave, int team,
                                              f4 (&acc)[TILE::FM][TILE::FN]) {
-  constexpr int S = TILE::STAGES, LOADS = 2 * (OP_P::LOADS + OP_Q::LOADS);
+  constexpr int S = TILE::STAGES, LOADS = OP_P::LOADS + OP_Q::LOADS, WK = TILE::WK;
   orth_clear<TILE>(acc);
-  const unsigned at = (unsigned)(uintptr_t)lds;
+  lds_char* const mine = lds + team * S * TILE::STAGE;
+  const unsigned at = (unsigned)(uintptr_t)mine;
+  if (WK > 1) {
+    P.base += team * P.step;
+    Q.base += team * Q.step;
+    P.step *= WK;
+    Q.step *= WK;
+  }
+  const int own = (steps + WK - 1 - team) / WK, all = (steps + WK - 1) / WK;
   const auto load = [&](int stage) {
     P.load(at + stage * TILE::STAGE, wave);
     Q.load(at + stage * TILE::STAGE + TILE::Q_AT, wave);
   };
   int ahead = 0;                           // stages asked for
-  for (; ahead < S - 1 && ahead < steps; ++ahead) load(ahead);
+  for (; ahead < S - 1 && ahead < own; ++ahead) load(ahead);
   int cur = 0, into = S - 1;
-  for (int s = 0; s < steps; ++s) {
+  for (int s = 0; s < all; ++s) {
     if (ahead - s == S - 1) stage_barrier<(S - 2) * LOADS>();
     else stage_barrier<0>();
-    if (ahead < steps) {
+    if (ahead < own) {
       load(into);
       ++ahead;
     }
-    lds_char* const stage = lds + cur * TILE::STAGE;
-    h8 p[2][TILE::FM], q[2][TILE::FN];
-    orth_read(P, stage, 0, p);
-    orth_read(Q, stage + TILE::Q_AT, 0, q);
-    orth_mfma<SPLIT>(p, q, acc, 0);
+    if (WK == 1 || s < own) {
+      lds_char* const stage = mine + cur * TILE::STAGE;
+      h8 p[2][TILE::FM], q[2][TILE::FN];
+      orth_read(P, stage, p);
+      orth_read(Q, stage + TILE::Q_AT, q);
+      orth_mfma<SPLIT>(p, q, acc, 0);
+    }
     into = cur;
     cur = cur + 1 == S ? 0 : cur + 1;
+  }
+  if constexpr (WK > 1) {
+    typedef __attribute__((address_space(3))) f4 lds_f4;
+    constexpr int PER = TILE::FM * TILE::FN, TEAM = TILE::TEAM;
+    stage_barrier<0>();
+    lds_f4* const sums = (lds_f4*)lds + (threadIdx.x & (TEAM - 1));
+    if (team > 0)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sums[((team - 1) * PER + i) * TEAM] = acc[i / TILE::FN][i % TILE::FN];
+    stage_barrier<0>();
+    if (team == 0)
+#pragma unroll
+      for (int w = 0; w < WK - 1; ++w)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i / TILE::FN][i % TILE::FN] += sums[(w * PER + i) * TEAM];
   }
 }
 
@@ -214,10 +244,10 @@ __device__ __forceinline__ void orth_pair_product(OP_P& P, OP_Q& Q, int steps, l
   };
   h8 p[2][TILE::FM], q[2][TILE::FN];
   const auto read = [&](int stage) {
-    orth_read(P, lds + stage * TILE::STAGE, 0, p);
-    orth_read(Q, lds + stage * TILE::STAGE + TILE::Q_AT, 0, q);
+    orth_read(P, lds + stage * TILE::STAGE, p);
+    orth_read(Q, lds + stage * TILE::STAGE + TILE::Q_AT, q);
   };
-  constexpr int LOADS = 2 * (OP_P::LOADS + OP_Q::LOADS);
+  constexpr int LOADS = OP_P::LOADS + OP_Q::LOADS;
   load(0);
   stage_barrier<0>();
   if (wave < 4) {
@@ -243,6 +273,18 @@ __device__ __forceinline__ void orth_pair_product(OP_P& P, OP_Q& Q, int steps, l
       if (s + 1 < steps) stage_barrier<LOADS>();
     }
   }
+}
+
+// Where element c of a row of `ld` elements lies (in halves, from the start of the matrix); its low part
+// is 32 behind.
+__device__ __forceinline__ long orth_at(int row, int c, int ld, bool split) {
+  return split ? (long)row * 2 * ld + ((c >> 5) << 6) + (c & 31) : (long)row * ld + c;
+}
+
+// What this wave has written to LDS can be read by its other lanes, and the other way round.
+__device__ __forceinline__ void wave_fence() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // four scaled values -> their high halves, and the low ones

@@ -12,20 +12,18 @@ namespace kfac {
 // The iteration runs on matrices of r rows and c >= r columns (a taller matrix is read and written
 // transposed).  Matrices of one shape, with their sides padded by zeros to whole tiles: R, C.
 // Offsets are in halves from the start of the operands; of matrix k of the group
-//   x[p] + k * 2RC   X, row-major [R][C]: the high halves, then the low ones (two of them: a step
-//                    reads one and writes the other)
+//   x[p] + k * 2RC   X, [R][C], room for two parts (two of them: a step reads one and writes the other)
 //   a    + k * 2RR   A = X X^T, in the same form
 //   b    + k * 2RR   B = aI + bA + cAA
 struct OrthGroup {
   int R, C, r, c;
   int count, first;      // matrices, and the first of them in the table
-  int tile;              // side of the tiles its products are computed in
-  int tile0, tiles;      // of the launch: first workgroup, and workgroups with a tile
+  int pad;               // R and C are multiples of it
   long x[2], a, b;
 };
 
 struct OrthBatch {
-  int tile;
+  int pad;               // of its largest matrices
   std::vector<OrthGroup> groups;
   long halves;           // scratch for the operands
   int first, count;      // matrices of the table
@@ -43,9 +41,14 @@ constexpr long ORTH_BATCH_HALVES = 1L << 29;     // a batch is closed when it ne
 
 inline int orth_pad(int n, int tile) { return (n + tile - 1) / tile * tile; }
 
-// sides are padded to multiples of 64, 128 or 256 by the smaller of them
-constexpr int ORTH_SMALL_SIDE = 128, ORTH_MID_SIDE = 512;
-inline int orth_tile(int r) { return r <= ORTH_SMALL_SIDE ? 64 : r <= ORTH_MID_SIDE ? 128 : 256; }
+// Sides are padded to multiples of 64 where the smaller one is at most this, else of 128, or of 256
+// where the smaller one is more than ORTH_MID_SIDE and such matrices hold as many 256-wide tiles as
+// half of the chip takes (they are in batches of their own then).
+constexpr int ORTH_SMALL_SIDE = 64, ORTH_MID_SIDE = 512;
+constexpr long ORTH_UNITS = 256;           // compute units
+
+// tiles on and below the diagonal
+inline long orth_triangle(long t) { return t * (t + 1) / 2; }
 
 inline OrthPlan orth_plan(int count, const int* rows, const int* cols) {
   OrthPlan p;
@@ -53,26 +56,34 @@ inline OrthPlan orth_plan(int count, const int* rows, const int* cols) {
     if (rows[i] > 0 && cols[i] > 0) p.order.push_back(i);
   const auto lo = [&](int i) { return std::min(rows[i], cols[i]); };
   const auto hi = [&](int i) { return std::max(rows[i], cols[i]); };
+  long large = 0;
+  for (int i : p.order)
+    if (lo(i) > ORTH_MID_SIDE) large += orth_triangle(orth_pad(lo(i), 256) / 256);
+  const auto pad = [&](int i) {
+    const int r = lo(i);
+    return r <= ORTH_SMALL_SIDE ? 64 : r <= ORTH_MID_SIDE || large < ORTH_UNITS / 2 ? 128 : 256;
+  };
   // longest reductions first, so that a launch does not end with them; equal shapes side by side
   std::stable_sort(p.order.begin(), p.order.end(), [&](int i, int j) {
-    const int ti = orth_tile(lo(i)), tj = orth_tile(lo(j));
-    if (ti != tj) return ti > tj;
+    const bool li = pad(i) == 256, lj = pad(j) == 256;
+    if (li != lj) return li;
     if (hi(i) != hi(j)) return hi(i) > hi(j);
     return lo(i) > lo(j);
   });
   for (size_t at = 0; at < p.order.size(); ++at) {
-    const int i = p.order[at], r = lo(i), c = hi(i), tile = orth_tile(r);
-    const long R = orth_pad(r, tile), C = orth_pad(c, tile), need = 4 * R * C + 4 * R * R;
+    const int i = p.order[at], r = lo(i), c = hi(i), side = pad(i);
+    const bool is_large = side == 256;
+    const long R = orth_pad(r, side), C = orth_pad(c, side), need = 4 * R * C + 4 * R * R;
     OrthBatch* b = p.batches.empty() ? nullptr : &p.batches.back();
-    const bool same = b && !b->groups.empty() && b->tile == tile && b->groups.back().r == r &&
-                      b->groups.back().c == c;
-    if (!b || b->tile != tile || b->halves + need > ORTH_BATCH_HALVES ||
+    const bool same = b && b->groups.back().r == r && b->groups.back().c == c;
+    if (!b || (b->pad == 256) != is_large || b->halves + need > ORTH_BATCH_HALVES ||
         (!same && (int)b->groups.size() == ORTH_GROUPS)) {
-      p.batches.push_back(OrthBatch{tile, {}, 0, (int)at, 0});
+      p.batches.push_back(OrthBatch{0, {}, 0, (int)at, 0});
       b = &p.batches.back();
     }
     if (b->groups.empty() || b->groups.back().r != r || b->groups.back().c != c)
-      b->groups.push_back(OrthGroup{(int)R, (int)C, r, c, 0, (int)at, tile, 0, 0, {0, 0}, 0, 0});
+      b->groups.push_back(OrthGroup{(int)R, (int)C, r, c, 0, (int)at, side, {0, 0}, 0, 0});
+    b->pad = std::max(b->pad, side);
     b->groups.back().count++;
     b->halves += need;
     b->count++;
@@ -92,38 +103,175 @@ inline OrthPlan orth_plan(int count, const int* rows, const int* cols) {
   return p;
 }
 
-// Tiles of one matrix: of a symmetric product those on and below the diagonal, or all of B X.
-inline long orth_tiles(const OrthGroup& g, int tile, bool symmetric) {
+// ---------------------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------------------
+
+// The kernels' tiles: 256 wide, one workgroup to a compute unit; 128 wide, two to a unit (in such a launch
+// matrices padded to 64 have 64-wide tiles); 64 wide, one to a unit with more stages of its operands in
+// flight (DEEP), or two.
+enum { ORTH_LARGE, ORTH_MID, ORTH_DEEP, ORTH_SMALL, ORTH_KINDS };
+struct OrthKind {
+  int tile, slots;       // workgroups at a time
+  float unit;            // us for 64 reduction steps of a tile, in two parts, with all slots taken
+};
+constexpr OrthKind ORTH_KIND[ORTH_KINDS] = {{256, 256, 4.4f}, {128, 512, 2.9f}, {64, 256, 0.6f}, {64, 512, 0.9f}};
+constexpr float ORTH_ENDS = 1.5f;          // what starting and ending a tile takes, in units
+
+enum { ORTH_GRAM, ORTH_POLY, ORTH_APPLY };
+
+// What a launch does for a group.  Of its tiles the first `whole` are a workgroup each, from workgroup
+// tile0 on; every other one is cut along the reduction into `cuts` pieces of `len` (in units of 64
+// steps; the last may be shorter), a workgroup each from piece0 on, whose sums a second launch adds up.
+struct OrthSlice {
+  int tile, tiles, whole, cuts, len, tile0, piece0, fix0;
+};
+struct OrthLaunch {
+  int kind = 0;
+  std::vector<OrthSlice> slices;
+  int pieces0 = 0, blocks = 0, fixes = 0;      // first piece, all workgroups, cut tiles
+};
+
+inline long orth_tiles(const OrthGroup& g, int tile, int product) {
   const long t = g.R / tile;
-  return symmetric ? t * (t + 1) / 2 : t * (g.C / tile);
+  return g.count * (product == ORTH_APPLY ? t * (g.C / tile) : orth_triangle(t));
 }
+inline int orth_length(const OrthGroup& g, int product) { return (product == ORTH_GRAM ? g.C : g.R) / 64; }
 
-// Workgroups of a launch over the groups; sets their tile0 and tiles.  Workgroups go to the eight
-// dies in turn, and a group starts at a multiple of eight.
-inline int orth_launch(std::vector<OrthGroup>& groups, int tile, bool symmetric) {
-  int at = 0;
-  for (OrthGroup& g : groups) {
-    g.tile0 = at;
-    g.tiles = (int)(g.count * orth_tiles(g, tile, symmetric));
-    at += (g.tiles + 7) / 8 * 8;
+struct OrthItems {
+  float length;
+  long n;
+};
+// When the last of the items is done, each taken by the slot that is free first, in order.
+struct OrthClock {
+  std::vector<std::pair<float, long>> free;     // (time, slots), earliest first
+  float end = 0.f;
+  explicit OrthClock(long slots) { free.push_back({0.f, slots}); }
+  // items that a slot can end by `until`; the rest is not taken
+  long take(float length, long n, float until = 1e30f) {
+    long taken = 0;
+    while (taken < n) {
+      const float t = free.front().first + length;
+      if (t > until) break;
+      const long k = std::min(n - taken, free.front().second);
+      if ((free.front().second -= k) == 0) free.erase(free.begin());
+      const auto at = std::lower_bound(free.begin(), free.end(), t,
+                                       [](const std::pair<float, long>& f, float v) { return f.first < v; });
+      if (at != free.end() && at->first == t) at->second += k;
+      else free.insert(at, {t, k});
+      end = std::max(end, t);
+      taken += k;
+    }
+    return taken;
   }
-  return at;
+};
+
+constexpr int ORTH_MIN_PIECE = 4;                 // a shorter one writes its sums for too little work
+constexpr long ORTH_PARTIAL_BYTES = 64L << 20;    // of all pieces
+
+// The schedule of one kind, and its time: whole tiles as long as they keep all slots busy, the rest cut
+// if that gains more than the second launch and the pieces' sums cost.
+inline float orth_schedule(const OrthBatch& b, int product, int kind, OrthLaunch& out) {
+  const OrthKind& K = ORTH_KIND[kind];
+  const int n = (int)b.groups.size();
+  out.kind = kind;
+  out.slices.assign(n, OrthSlice{});
+  std::vector<float> length(n);                   // of a tile, in this kind's units
+  std::vector<int> order(n);
+  double work = 0.;
+  float longest = 0.f;
+  for (int i = 0; i < n; ++i) {
+    const OrthGroup& g = b.groups[i];
+    OrthSlice& s = out.slices[i];
+    s.tile = std::min(K.tile, g.pad);
+    s.tiles = s.whole = (int)orth_tiles(g, s.tile, product);
+    length[i] = orth_length(g, product) * (s.tile < K.tile ? 0.6f : 1.f) + ORTH_ENDS;
+    work += (double)length[i] * s.tiles;
+    longest = std::max(longest, length[i]);
+    order[i] = i;
+  }
+  std::stable_sort(order.begin(), order.end(), [&](int i, int j) { return length[i] > length[j]; });
+  OrthClock plain(K.slots);
+  for (int i : order) plain.take(length[i], out.slices[i].tiles);
+  const float even = (float)(work / K.slots);
+  float best = plain.end * K.unit;
+  if (plain.end > 1.1f * even && plain.end * K.unit > 8.f) {
+    OrthClock full(K.slots);
+    std::vector<long> whole(n, 0);
+    for (int i : order) {
+      whole[i] = full.take(length[i], out.slices[i].tiles, 1.02f * even);
+      if (whole[i] < out.slices[i].tiles) break;
+    }
+    int last = 0;
+    for (int d : {2, 3, 4, 6, 8, 12, 16}) {
+      const int piece = std::max(ORTH_MIN_PIECE, (int)((longest + d - 1) / d));
+      if (piece == last) continue;
+      last = piece;
+      OrthClock clock = full;
+      long pieces = 0;
+      std::vector<OrthSlice> cut = out.slices;
+      for (int i : order) {
+        OrthSlice& s = cut[i];
+        const int all = orth_length(b.groups[i], product), c = (all + piece - 1) / piece;
+        s.cuts = 0;
+        s.whole = s.tiles;
+        if (whole[i] == s.tiles) continue;
+        if (c < 2) {
+          clock.take(length[i], s.tiles - whole[i]);
+          continue;
+        }
+        s.whole = (int)whole[i];
+        s.cuts = c;
+        s.len = (all + c - 1) / c;
+        const long m = (long)(s.tiles - s.whole) * c;
+        clock.take((length[i] - ORTH_ENDS) * s.len / all + ORTH_ENDS, m);
+        pieces += m;
+      }
+      const long bytes = pieces * K.tile * K.tile * 4;
+      const float t = clock.end * K.unit + 5.f + 2.f * bytes / 3.5e6f;
+      if (bytes <= ORTH_PARTIAL_BYTES && t < best - 10.f) {
+        best = t;
+        out.slices = cut;
+      }
+    }
+  }
+  // workgroups: whole tiles from multiples of eight on (workgroups go to the eight dies in turn), then
+  // the pieces, longest first throughout
+  int at = 0, fixes = 0;
+  for (int i : order) {
+    OrthSlice& s = out.slices[i];
+    s.tile0 = at;
+    at += (s.whole + 7) / 8 * 8;
+  }
+  out.pieces0 = at;
+  for (int i : order) {
+    OrthSlice& s = out.slices[i];
+    s.piece0 = at;
+    s.fix0 = fixes;
+    if (s.cuts > 0) {
+      // (a last piece without anything to do is left out)
+      s.cuts = (orth_length(b.groups[i], product) + s.len - 1) / s.len;
+      at += (s.tiles - s.whole) * s.cuts;
+      fixes += s.tiles - s.whole;
+    }
+  }
+  out.blocks = at;
+  out.fixes = fixes;
+  return best;
 }
 
-// The tiles that a product of the batch is computed in: 256 wide, one workgroup to a compute unit; 128
-// wide, two to a unit or, where there are not as many tiles, one with more stages in flight; 64 wide.
-enum { ORTH_LARGE, ORTH_MID, ORTH_DEEP, ORTH_SMALL };
-constexpr long ORTH_UNITS = 256;
-inline int orth_pick_tile(const OrthBatch& b, bool symmetric) {
-  const auto tiles = [&](int tile) {
-    long n = 0;
-    for (const OrthGroup& g : b.groups) n += g.count * orth_tiles(g, tile, symmetric);
-    return n;
-  };
-  if (b.tile == 64) return ORTH_SMALL;
-  if (b.tile == 256 && tiles(256) >= ORTH_UNITS / 2) return ORTH_LARGE;
-  const long n = tiles(128);
-  return n > ORTH_UNITS ? ORTH_MID : n > ORTH_UNITS / 2 ? ORTH_DEEP : ORTH_SMALL;
+inline OrthLaunch orth_launch(const OrthBatch& b, int product) {
+  OrthLaunch best;
+  float time = 1e30f;
+  for (int kind = b.pad == 256 ? ORTH_LARGE : b.pad == 128 ? ORTH_MID : ORTH_DEEP; kind < ORTH_KINDS; ++kind) {
+    OrthLaunch l;
+    const float t = orth_schedule(b, product, kind, l);
+    if (t < time) {
+      time = t;
+      best = l;
+    }
+  }
+  return best;
 }
 
 }  // namespace kfac

@@ -10,9 +10,11 @@
 #include "orth_core.h"
 #include "orth_plan.h"
 
+#include <limits.h>
 #include <string.h>
 
 #include <exception>
+#include <type_traits>
 
 namespace kfac {
 namespace {
@@ -28,7 +30,8 @@ struct OrthMat {
   int sum0, sums;        // its partial sums, and the workgroups that make them
   int pack0;             // first workgroup of the second pass (within the batch)
   float step, keep;      // parameter = keep * parameter - step * result
-  int vec;               // in, out and buf are 16-byte aligned, and so are all rows
+  int vec;               // in and buf can be read 8 elements at a time
+  int wide;              // out can be written 4 elements at a time
 };
 
 constexpr int SUM_ELEMS = 16384;                 // a workgroup of the first pass
@@ -178,53 +181,67 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
       h[e] = (half_t)v[e];
       l[e] = (half_t)(v[e] - (float)h[e]);
     }
-    half_t* const to = x + (long)(r0 + r) * C + c0 + c;
+    half_t* const to = x + orth_at(r0 + r, c0 + c, C, low);
     *(h8*)to = h;
-    if (low) *(h8*)(to + (long)R * C) = l;
+    if (low) *(h8*)(to + 32) = l;
   }
 }
 
-enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
+enum { GRAM = ORTH_GRAM, POLY = ORTH_POLY, APPLY = ORTH_APPLY, LAST };
 
 struct OrthProduct {
   half_t* base;
+  float* partial;        // sums of the pieces, a tile each
   const OrthMat* mats;
   float ca, cb, cc;      // of this step
   int from;              // which X is read (the other one is written)
-  int low;               // the low halves of the result are wanted
+  int low;               // APPLY: the next step reads X in two parts
   int type, update;      // LAST: type of the result; parameters are updated with it
-  int n;
+  int n, pieces0;
+  int tile0[ORTH_GROUPS], piece0[ORTH_GROUPS], fix0[ORTH_GROUPS];     // (beyond any workgroup: no group)
   OrthGroup g[ORTH_GROUPS];
+  OrthSlice s[ORTH_GROUPS];
 };
 static_assert(sizeof(OrthProduct) <= 4096, "kernel arguments");
 
-template <class V>
-__device__ __forceinline__ void orth_store(const OrthMat& m, long at, float o, int update) {
-  V* const out = (V*)m.out;
-  if (update) o = m.keep * Element<V>::get(out[at]) - m.step * o;
-  out[at] = Element<V>::put(o);
+// the last group that starts at or before `at` (the starts grow)
+__device__ __forceinline__ int orth_find(const int (&starts)[ORTH_GROUPS], int at) {
+  int gi = -1;
+#pragma unroll
+  for (int i = 0; i < ORTH_GROUPS; ++i) gi += starts[i] <= at;
+  return __builtin_amdgcn_readfirstlane(gi);
 }
 
-typedef OrthTile<64, 64, 2, 2, 4> SmallTile;
-typedef OrthTile<128, 128, 2, 2, 2> MidTile;
-typedef OrthTile<128, 128, 2, 2, 4> DeepTile;
+// Four elements of a result, columns c ... c + 3 of row r of the matrix as it is stored.
+template <class V>
+__device__ __forceinline__ void orth_store(const OrthMat& mat, int r, int c, f4 v, int update) {
+  if (r >= mat.rows || c >= mat.cols) return;
+  V* const out = (V*)mat.out + (long)r * mat.cols + c;
+  if (mat.wide) {
+    Pack<V, 4> o;
+    if (update) o = *(const Pack<V, 4>*)out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o.v[e] = Element<V>::put(update ? mat.keep * Element<V>::get(o.v[e]) - mat.step * v[e] : v[e]);
+    *(Pack<V, 4>*)out = o;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < mat.cols)
+      out[e] = Element<V>::put(update ? mat.keep * Element<V>::get(out[e]) - mat.step * v[e] : v[e]);
+}
+
+typedef OrthTile<64, 64, 2, 2, 2, false, 2> SmallTile;
+typedef OrthTile<64, 64, 2, 2, 4, false, 2> DeepTile;
+typedef OrthTile<128, 128, 2, 4, 2, true> MidTile;
 typedef OrthTile<256, 256, 2, 4, 2, true> LargeTile;
 
-template <class TILE, bool SPLIT, int MODE>
-__global__ __launch_bounds__(TILE::THREADS, 2) void orth_product_kernel(const OrthProduct p) {
-  extern __shared__ __align__(16) char smem[];
-  constexpr int T = TILE::TM, FM = TILE::FM, FN = TILE::FN;
-  static_assert(TILE::TM == TILE::TN, "symmetric products");
-  constexpr bool SYM = MODE == GRAM || MODE == POLY;
-  int gi = 0;
-  while (gi + 1 < p.n && p.g[gi + 1].tile0 <= (int)blockIdx.x) ++gi;
-  const OrthGroup& g = p.g[gi];
-  const int local = blockIdx.x - g.tile0, each = (g.tiles + 7) / 8;
-  const int t = (local & 7) * each + (local >> 3);     // neighbours in the tile order share a die's cache
-  if (t >= g.tiles) return;
-  const int R = g.R, C = g.C, rt = R / T, ct = C / T;
-  int tm, tn, k;
-  if (SYM) {
+// A tile of a group: of matrix k, rows tm of P and tn of Q.
+template <int MODE>
+__device__ __forceinline__ void orth_place(const OrthGroup& g, int tile, int t, int& k, int& tm, int& tn) {
+  const int rt = g.R / tile;
+  if (MODE == GRAM || MODE == POLY) {
     const int per = rt * (rt + 1) / 2, u = t % per;
     k = t / per;
     tm = (int)((sqrtf(8.f * u + 1.f) - 1.f) * 0.5f);
@@ -232,132 +249,328 @@ __global__ __launch_bounds__(TILE::THREADS, 2) void orth_product_kernel(const Or
     while ((tm + 1) * (tm + 2) / 2 <= u) ++tm;
     tn = u - tm * (tm + 1) / 2;
   } else {
-    const int per = rt * ct, u = t % per;
+    const int per = rt * (g.C / tile), u = t % per;
     k = t / per;
     tm = u / rt;
     tn = u % rt;
   }
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / TILE::WN, wn = wave % TILE::WN;
-  const long XS = (long)R * C, AS = (long)R * R;
-  half_t* const x = p.base + g.x[p.from] + k * 2 * XS;
-  half_t* const a = p.base + g.a + k * 2 * AS;
-  half_t* const b = p.base + g.b + k * 2 * AS;
-  OrthOperand<TILE::TM, TILE::WAVES, FM, !SYM> P;
-  OrthOperand<TILE::TN, TILE::WAVES, FN, false> Q;
-  int steps;
-  if (MODE == GRAM) {
-    P.init(x, SPLIT ? XS : 0, C, tm * T, wm, wave, lane);
-    Q.init(x, SPLIT ? XS : 0, C, tn * T, wn, wave, lane);
-    steps = C;
-  } else if (MODE == POLY) {
-    P.init(a, SPLIT ? AS : 0, R, tm * T, wm, wave, lane);
-    Q.init(a, SPLIT ? AS : 0, R, tn * T, wn, wave, lane);
-    steps = R;
-  } else {
-    P.init(x, SPLIT ? XS : 0, C, tm * T, wm, wave, lane);          // (columns of X)
-    Q.init(b, SPLIT ? AS : 0, R, tn * T, wn, wave, lane);
-    steps = R;
-  }
-  steps /= SPLIT ? ORTH_BK : 2 * ORTH_BK;
-  lds_char* const lds = (lds_char*)smem;
-  f4 acc[FM][FN];
-  if constexpr (TILE::PAIR) orth_pair_product<TILE, SPLIT>(P, Q, steps, lds, wave, acc);
-  else orth_product<TILE, SPLIT>(P, Q, steps, lds, wave, acc);
+}
 
+// What a product's sums become: B = aI + bA + cAA, or they are it.  Elements D[m ... m + 3][n].
+template <int MODE, bool SPLIT>
+__device__ __forceinline__ f4 orth_value(const OrthProduct& p, const OrthGroup& g, int k, int m, int n, f4 v) {
   constexpr float INV = 1.f / ORTH_SCALE;
-  const int m0 = tm * T + wm * FM * 16 + 4 * (lane >> 4), n0 = tn * T + wn * FN * 16 + (lane & 15);
-  if (MODE == LAST) {
-    const OrthMat m = p.mats[g.first + k];
-    const bool tall = m.rows > m.cols;
+  if (MODE == LAST) return v * (INV * INV);
+  v *= INV;
+  if (MODE == POLY) {
+    const half_t* const from = p.base + g.a + (long)k * 2 * g.R * g.R + orth_at(n, m, g.R, SPLIT);
+    const h4 ah = *(const h4*)from;
+    h4 al = {0, 0, 0, 0};
+    if (SPLIT) al = *(const h4*)(from + 32);
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = n0 + 16 * j, col = m0 + 16 * i + e;
-          if (row >= g.r || col >= g.c) continue;
-          const long at = tall ? (long)col * g.r + row : (long)row * g.c + col;
-          const float o = acc[i][j][e] * (INV * INV);
-          if (p.type == TYPE_F32) orth_store<float>(m, at, o, p.update);
-          else if (p.type == TYPE_BF16) orth_store<__hip_bfloat16>(m, at, o, p.update);
-          else orth_store<half_t>(m, at, o, p.update);
-        }
-    return;
+    for (int e = 0; e < 4; ++e) {
+      v[e] = fmaf(p.cc, v[e], p.cb * ((float)ah[e] + (float)al[e]));
+      if (m + e == n) v[e] += p.ca * ORTH_SCALE;
+    }
   }
-  // D[m][n] to row n: four values of a lane side by side
-  const long S = SYM ? AS : XS;
-  const int ld = SYM ? R : C;
-  half_t* const out = MODE == GRAM ? a : MODE == POLY ? b : p.base + g.x[1 - p.from] + k * 2 * XS;
+  return v;
+}
+
+// Where a product goes, its rows' length, and whether in two parts.
+template <int MODE, bool SPLIT>
+__device__ __forceinline__ half_t* orth_target(const OrthProduct& p, const OrthGroup& g, int k, int& ld, bool& low) {
+  constexpr bool SYM = MODE == GRAM || MODE == POLY;
+  ld = SYM ? g.R : g.C;
+  low = SYM ? SPLIT : p.low;
+  return p.base + (MODE == GRAM ? g.a : MODE == POLY ? g.b : g.x[1 - p.from]) + (long)k * 2 * g.R * ld;
+}
+
+// Writes the elements of a wave, FM x FN blocks from D[m0][n0] on: D[m][n] to row n, and for a symmetric
+// product also to row m (`mirror`).  A lane holds pieces of four along m of 16 rows n, which would reach
+// memory 32 bytes at a time (two, of the mirror image): they go through LDS, sixteen rows at a time, and
+// leave it as whole rows of the wave's part.  Without that a product of 16 matrices of 1024^2 spends 40 of
+// 113 us on writing.
+template <class TILE, bool SPLIT, int MODE>
+__device__ __forceinline__ void orth_write(const OrthProduct& p, const OrthGroup& g, const OrthMat& mat, int k, int m0,
+                                           int n0, bool mirror, f4 (&acc)[TILE::FM][TILE::FN], lds_char* lds, int lane) {
+  constexpr int FM = TILE::FM, FN = TILE::FN;
+  typedef __attribute__((address_space(3))) half_t lds_half;
+  typedef __attribute__((address_space(3))) h4 lds_h4;
+  typedef __attribute__((address_space(3))) f4 lds_f4;
+  typedef __attribute__((address_space(3))) float lds_float;
+  int ld = 0;
+  bool low = false;
+  half_t* const out = MODE == LAST ? nullptr : orth_target<MODE, SPLIT>(p, g, k, ld, low);
+  // 16 rows from `row0` on of W elements from column `col0` on, from LDS to memory
+  const auto rows_out = [&](auto width, int pitch, int row0, int col0) {
+    constexpr int W = decltype(width)::value;
+    asm volatile("" : "+v"(lane));     // (addresses are formed here, or all of a tile's would be kept in registers)
+    // (rolled up: the code of a whole tile has to stay in the instruction cache)
+    if (MODE == LAST) {
+#pragma unroll 1
+      for (int t = 0; t < W / 16; ++t) {
+        const int at = t * 64 + lane, row = at / (W / 4), c = at % (W / 4) * 4;
+        const f4 v = *(lds_f4*)(lds + row * pitch + c * 4);
+        if (p.type == TYPE_F32) orth_store<float>(mat, row0 + row, col0 + c, v, p.update);
+        else if (p.type == TYPE_BF16) orth_store<__hip_bfloat16>(mat, row0 + row, col0 + c, v, p.update);
+        else orth_store<half_t>(mat, row0 + row, col0 + c, v, p.update);
+      }
+    } else if (low) {
+#pragma unroll 2
+      for (int t = 0; t < W / 16; ++t) {
+        const int at = t * 64 + lane, row = at / (W / 4), c = at % (W / 4) * 16;
+        *(f4*)((char*)(out + orth_at(row0 + row, col0, ld, true)) + c) = *(lds_f4*)(lds + row * pitch + c);
+      }
+    } else {
+#pragma unroll 2
+      for (int t = 0; t < W / 32; ++t) {
+        const int at = t * 64 + lane, row = at / (W / 8), c = at % (W / 8) * 16;
+        *(f4*)((char*)(out + orth_at(row0 + row, col0, ld, false)) + c) = *(lds_f4*)(lds + row * pitch + c);
+      }
+    }
+  };
+  // (a result whose matrix is stored transposed has m down its rows)
+  const bool tall = MODE == LAST && mat.rows > mat.cols;
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+  for (int j = 0; j < FN; ++j) {
+    asm volatile("" : "+v"(lane));
+    const int nl = lane & 15, ml = 4 * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      acc[i][j] = orth_value<MODE, SPLIT>(p, g, k, m0 + 16 * i + ml, n0 + 16 * j + nl, acc[i][j]);
+      if (tall) continue;
+      lds_char* const row = lds + nl * TILE::M_PITCH;
+      const int c = 16 * i + ml;
+      if (MODE == LAST) {
+        *(lds_f4*)(row + c * 4) = acc[i][j];
+      } else {
+        h4 h, l;
+        split4(acc[i][j], h, l);
+        lds_h4* const to = (lds_h4*)(row + 2 * (int)orth_at(0, c, 0, low));
+        *to = h;
+        if (low) to[8] = l;
+      }
+    }
+    if (tall) continue;
+    wave_fence();
+    rows_out(std::integral_constant<int, FM * 16>(), TILE::M_PITCH, n0 + 16 * j, m0);
+    wave_fence();
+  }
+  if (!mirror && !tall) return;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    asm volatile("" : "+v"(lane));
+    const int nl = lane & 15, ml = 4 * (lane >> 4);
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      const int m = m0 + 16 * i, n = n0 + 16 * j;
-      f4 v = acc[i][j] * INV;
-      if (MODE == POLY) {
-        const h4 ah = *(const h4*)(a + (long)n * R + m);
-        h4 al = {0, 0, 0, 0};
-        if (SPLIT) al = *(const h4*)(a + AS + (long)n * R + m);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = fmaf(p.cc, v[e], p.cb * ((float)ah[e] + (float)al[e]));
-          if (m + e == n) v[e] += p.ca * ORTH_SCALE;
-        }
-      }
+      const int c = 16 * j + nl;
       h4 h, l;
-      split4(v, h, l);
-      half_t* const to = out + (long)n * ld + m;
-      *(h4*)to = h;
-      if (p.low) *(h4*)(to + S) = l;
-      if (SYM && tm != tn) {
+      asm volatile("" : "+v"(acc[i][j]));     // (or the parts of the whole tile would be kept from above)
+      split4(acc[i][j], h, l);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          half_t* const mirror = out + (long)(m + e) * ld + n;
-          *mirror = h[e];
-          if (p.low) mirror[S] = l[e];
+      for (int e = 0; e < 4; ++e) {
+        lds_char* const row = lds + (ml + e) * TILE::N_PITCH;
+        if (MODE == LAST) {
+          *(lds_float*)(row + c * 4) = acc[i][j][e];
+        } else {
+          lds_half* const to = (lds_half*)row + orth_at(0, c, 0, low);
+          *to = h[e];
+          if (low) to[32] = l[e];
         }
       }
     }
+    wave_fence();
+    rows_out(std::integral_constant<int, FN * 16>(), TILE::N_PITCH, m0 + 16 * i, n0);
+    wave_fence();
+  }
 }
 
 template <class TILE, bool SPLIT, int MODE>
-bool launch_tiles(OrthProduct& p, OrthBatch& b, hipStream_t stream) {
-  const int grid = orth_launch(b.groups, TILE::TM, MODE == GRAM || MODE == POLY);
-  p.n = (int)b.groups.size();
-  std::copy(b.groups.begin(), b.groups.end(), p.g);
-  constexpr int lds = TILE::LDS;
+__device__ __forceinline__ void orth_item(const OrthProduct& p, const OrthGroup& g, const OrthSlice& s, int t, int piece,
+                                          long partial, lds_char* lds) {
+  constexpr bool SYM = MODE == GRAM || MODE == POLY;
+  constexpr int T = TILE::TM, FM = TILE::FM, FN = TILE::FN, UNIT = SPLIT ? 2 : 1;    // stages of 64 steps
+  static_assert(TILE::TM == TILE::TN, "symmetric products");
+  int k, tm, tn;
+  orth_place<MODE>(g, T, t, k, tm, tn);
+  // (divisions leave them in vector registers)
+  k = __builtin_amdgcn_readfirstlane(k);
+  tm = __builtin_amdgcn_readfirstlane(tm);
+  tn = __builtin_amdgcn_readfirstlane(tn);
+  piece = __builtin_amdgcn_readfirstlane(piece);
+  const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = all % TILE::WAVES, team = all / TILE::WAVES;
+  const int wm = wave / TILE::WN, wn = wave % TILE::WN, R = g.R, C = g.C;
+  const long XS = (long)R * C, AS = (long)R * R;
+  const half_t* const x = p.base + g.x[p.from] + k * 2 * XS;
+  const half_t* const a = p.base + g.a + k * 2 * AS;
+  const half_t* const b = p.base + g.b + k * 2 * AS;
+  OrthOperand<TILE::TM, TILE::WAVES, FM, !SYM, SPLIT> P;   // (columns of X, or rows of X or A)
+  OrthOperand<TILE::TN, TILE::WAVES, FN, false, SPLIT> Q;
+  if (MODE == POLY) P.init(a, R, tm * T, wm, wave, lane);
+  else P.init(x, C, tm * T, wm, wave, lane);
+  if (MODE == GRAM) Q.init(x, C, tn * T, wn, wave, lane);
+  else Q.init(MODE == POLY ? a : b, R, tn * T, wn, wave, lane);
+  int steps = (MODE == GRAM ? C : R) / 64;
+  if (piece >= 0) {
+    const int from = piece * s.len;
+    P.base += from * UNIT * P.step;
+    Q.base += from * UNIT * Q.step;
+    steps = min(s.len, steps - from);
+  }
+  steps *= UNIT;
+  f4 acc[FM][FN];
+  if constexpr (TILE::PAIR) orth_pair_product<TILE, SPLIT>(P, Q, steps, lds, wave, acc);
+  else orth_product<TILE, SPLIT>(P, Q, steps, lds, wave, team, acc);
+  if (team > 0) return;
+  if (piece >= 0) {
+    f4* const to = (f4*)(p.partial + partial * T * T) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) to[(i * FN + j) * TILE::TEAM] = acc[i][j];
+    return;
+  }
+  OrthMat mat;
+  if (MODE == LAST) mat = p.mats[g.first + k];
+  orth_write<TILE, SPLIT, MODE>(p, g, mat, k, tm * T + wm * FM * 16, tn * T + wn * FN * 16, SYM && tm != tn, acc,
+                                lds + TILE::SUMS + wave * TILE::WRITE, lane);
+}
+
+template <class TILE, bool SPLIT, int MODE>
+__global__ __launch_bounds__(TILE::THREADS, TILE::LDS > 80 * 1024 ? 2 : 4) void orth_product_kernel(const OrthProduct p) {
+  extern __shared__ __align__(16) char smem[];
+  lds_char* const lds = (lds_char*)smem;
+  const int block = blockIdx.x;
+  int t, piece = -1, gi;
+  long partial = 0;
+  if (block < p.pieces0) {
+    gi = orth_find(p.tile0, block);
+    const int whole = p.s[gi].whole, local = block - p.tile0[gi], each = (whole + 7) / 8;
+    t = (local & 7) * each + (local >> 3);     // neighbours in the tile order share a die's cache
+    if (t >= whole) return;
+  } else {
+    gi = orth_find(p.piece0, block);
+    const int local = block - p.piece0[gi], cuts = p.s[gi].cuts;
+    t = p.s[gi].whole + local / cuts;
+    piece = local % cuts;
+    partial = block - p.pieces0;
+  }
+  const OrthGroup& g = p.g[gi];
+  const OrthSlice& s = p.s[gi];
+  if constexpr (TILE::TM == 128) {
+    if (s.tile == 64) {
+      orth_item<SmallTile, SPLIT, MODE>(p, g, s, t, piece, partial * 4, lds);
+      return;
+    }
+  }
+  orth_item<TILE, SPLIT, MODE>(p, g, s, t, piece, partial, lds);
+}
+
+// Adds up the pieces of cut tiles, in order; a workgroup takes two rows of fragments of a tile (32 rows of
+// each wave's part, a whole piece of the operands' layout).
+template <class TILE, bool SPLIT, int MODE>
+__device__ __forceinline__ void orth_fix_item(const OrthProduct& p, int gi, int local, int i, int scale,
+                                              lds_char* lds) {
+  constexpr int T = TILE::TM, FM = TILE::FM, FN = TILE::FN;
+  const OrthGroup& g = p.g[gi];
+  const OrthSlice& s = p.s[gi];
+  i *= 2;
+  if (i >= FM || threadIdx.x >= TILE::TEAM) return;
+  int k, tm, tn;
+  orth_place<MODE>(g, T, s.whole + local, k, tm, tn);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / TILE::WN, wn = wave % TILE::WN;
+  const long first = (long)(s.piece0 - p.pieces0 + local * s.cuts) * scale;
+  typedef OrthTile<32 * TILE::WM, TILE::TN, TILE::WM, TILE::WN, TILE::STAGES> Rows;
+  f4 sum[2][FN];
+#pragma unroll
+  for (int j = 0; j < 2 * FN; ++j) sum[j / FN][j % FN] = f4{0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < s.cuts; ++c) {
+    const f4* const from = (const f4*)(p.partial + (first + (long)c * scale) * T * T) + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < 2 * FN; ++j) sum[j / FN][j % FN] += from[(i * FN + j) * TILE::TEAM];
+  }
+  const int m = tm * T + wm * FM * 16 + 16 * i, n0 = tn * T + wn * FN * 16;
+  OrthMat mat;
+  if (MODE == LAST) mat = p.mats[g.first + k];
+  orth_write<Rows, SPLIT, MODE>(p, g, mat, k, m, n0, MODE != LAST && MODE != APPLY && tm != tn, sum,
+                                lds + wave * Rows::WRITE, lane);
+}
+
+template <class TILE, bool SPLIT, int MODE>
+__global__ __launch_bounds__(TILE::TEAM) void orth_fix_kernel(const OrthProduct p) {
+  constexpr int PITCH = 64 * (TILE::FN > 2 ? TILE::FN : 2) + 16;
+  __shared__ __align__(16) char smem[TILE::WAVES * 16 * PITCH];
+  lds_char* const lds = (lds_char*)smem;
+  const int cut = blockIdx.x / (TILE::FM / 2), i = blockIdx.x % (TILE::FM / 2), gi = orth_find(p.fix0, cut);
+  const int local = cut - p.fix0[gi];
+  if constexpr (TILE::TM == 128) {
+    if (p.s[gi].tile == 64) {
+      orth_fix_item<SmallTile, SPLIT, MODE>(p, gi, local, i, 4, lds);
+      return;
+    }
+  }
+  orth_fix_item<TILE, SPLIT, MODE>(p, gi, local, i, 1, lds);
+}
+
+template <class TILE, bool SPLIT, int MODE>
+bool launch_tiles(const OrthProduct& p, const OrthLaunch& l, hipStream_t stream) {
   const auto kernel = orth_product_kernel<TILE, SPLIT, MODE>;
-  if (!enable_large_lds((const void*)kernel, lds)) return false;
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(TILE::THREADS), lds, stream, p);
+  if (!enable_large_lds((const void*)kernel, TILE::LDS)) return false;
+  hipLaunchKernelGGL(kernel, dim3(l.blocks), dim3(TILE::THREADS), TILE::LDS, stream, p);
+  if (l.fixes > 0)
+    hipLaunchKernelGGL((orth_fix_kernel<TILE, SPLIT, MODE>), dim3(l.fixes * (TILE::FM / 2)), dim3(TILE::TEAM), 0, stream,
+                       p);
   return true;
 }
 
 template <class TILE, int MODE>
-bool launch_parts(OrthProduct& p, OrthBatch& b, bool split, hipStream_t stream) {
-  return split ? launch_tiles<TILE, true, MODE>(p, b, stream) : launch_tiles<TILE, false, MODE>(p, b, stream);
+bool launch_parts(const OrthProduct& p, const OrthLaunch& l, bool split, hipStream_t stream) {
+  return split ? launch_tiles<TILE, true, MODE>(p, l, stream) : launch_tiles<TILE, false, MODE>(p, l, stream);
 }
 
 template <int MODE>
-bool launch_product(OrthProduct& p, OrthBatch& b, bool split, hipStream_t stream) {
-  switch (orth_pick_tile(b, MODE == GRAM || MODE == POLY)) {
-    case ORTH_SMALL: return launch_parts<SmallTile, MODE>(p, b, split, stream);
-    case ORTH_DEEP: return launch_parts<DeepTile, MODE>(p, b, split, stream);
-    case ORTH_MID: return launch_parts<MidTile, MODE>(p, b, split, stream);
-    default: return launch_parts<LargeTile, MODE>(p, b, split, stream);
+bool launch_product(OrthProduct& p, const OrthBatch& b, const OrthLaunch& l, bool split, hipStream_t stream) {
+  // groups by their first whole tile, piece or cut tile: the same order for all three; those without one
+  // of a sort share its start with the group behind them, which is found
+  std::vector<int> order(b.groups.size());
+  for (size_t i = 0; i < order.size(); ++i) order[i] = (int)i;
+  std::stable_sort(order.begin(), order.end(), [&](int i, int j) {
+    const OrthSlice &u = l.slices[i], &v = l.slices[j];
+    if (u.tile0 != v.tile0) return u.tile0 < v.tile0;
+    return u.piece0 < v.piece0;
+  });
+  p.n = (int)order.size();
+  p.pieces0 = l.pieces0;
+  for (int i = 0; i < ORTH_GROUPS; ++i) {
+    const bool is = i < p.n;
+    if (is) {
+      p.g[i] = b.groups[order[i]];
+      p.s[i] = l.slices[order[i]];
+    }
+    p.tile0[i] = is ? p.s[i].tile0 : INT_MAX;
+    p.piece0[i] = is ? p.s[i].piece0 : INT_MAX;
+    p.fix0[i] = is ? p.s[i].fix0 : INT_MAX;
+  }
+  switch (l.kind) {
+    case ORTH_SMALL: return launch_parts<SmallTile, MODE>(p, l, split, stream);
+    case ORTH_DEEP: return launch_parts<DeepTile, MODE>(p, l, split, stream);
+    case ORTH_MID: return launch_parts<MidTile, MODE>(p, l, split, stream);
+    default: return launch_parts<LargeTile, MODE>(p, l, split, stream);
   }
 }
 
-bool launch_step(OrthProduct& p, OrthBatch& b, const float* coeffs, bool split, bool next_split, bool last,
-                 hipStream_t stream) {
+bool launch_step(OrthProduct& p, const OrthBatch& b, const OrthLaunch (&l)[3], const float* coeffs, bool split,
+                 bool next_split, bool last, hipStream_t stream) {
   p.ca = coeffs[0];
   p.cb = coeffs[1];
   p.cc = coeffs[2];
-  p.low = split;
-  if (!launch_product<GRAM>(p, b, split, stream) || !launch_product<POLY>(p, b, split, stream)) return false;
+  if (!launch_product<GRAM>(p, b, l[ORTH_GRAM], split, stream) ||
+      !launch_product<POLY>(p, b, l[ORTH_POLY], split, stream))
+    return false;
   p.low = next_split;
-  return last ? launch_product<LAST>(p, b, split, stream) : launch_product<APPLY>(p, b, split, stream);
+  return last ? launch_product<LAST>(p, b, l[ORTH_APPLY], split, stream)
+              : launch_product<APPLY>(p, b, l[ORTH_APPLY], split, stream);
 }
 
 template <class V, bool MUON>
@@ -372,7 +585,7 @@ void launch_passes(const OrthMat* mats, const OrthBatch& b, Momentum mom, double
 }
 
 struct Layout {
-  size_t table, sums, operands, bytes;
+  size_t table, sums, partials, operands, bytes;
 };
 Layout layout(const OrthPlan& plan) {
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
@@ -381,7 +594,8 @@ Layout layout(const OrthPlan& plan) {
   l.sums = up(plan.order.size() * sizeof(OrthMat));
   long sums = 0;
   for (const OrthBatch& b : plan.batches) sums = std::max(sums, (long)b.count * SUM_MAX);
-  l.operands = l.sums + up((size_t)sums * sizeof(double));
+  l.partials = l.sums + up((size_t)sums * sizeof(double));
+  l.operands = l.partials + (size_t)ORTH_PARTIAL_BYTES;
   l.bytes = l.operands + (size_t)plan.halves * sizeof(half_t);
   return l;
 }
@@ -447,6 +661,7 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
       m.keep = c.keep ? c.keep[i] : 0.f;
       // rows of whole 8-element groups at aligned addresses
       m.vec = m.cols % 8 == 0 && ((uintptr_t)m.in % (8 * size)) == 0 && ((uintptr_t)m.buf & 15) == 0;
+      m.wide = m.cols % 4 == 0 && (uintptr_t)m.out % (4 * size) == 0;
       sum0 += m.sums;
       pack0 += cdiv(g.R, PACK_R) * cdiv(g.C, PACK_C);
     }
@@ -472,14 +687,16 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
     else passes((half_t*)nullptr);
     OrthProduct p;
     memset(&p, 0, sizeof(p));
+    const OrthLaunch launches[3] = {orth_launch(b, ORTH_GRAM), orth_launch(b, ORTH_POLY), orth_launch(b, ORTH_APPLY)};
     p.base = base;
+    p.partial = (float*)(ws + l.partials);
     p.mats = mats;
     p.type = c.type;
     p.update = c.step != nullptr;
     for (int k = 0; k < c.steps; ++k) {
       const bool split = c.steps - k > c.late, next = c.steps - k - 1 > c.late, last = k + 1 == c.steps;
       p.from = k & 1;
-      if (!launch_step(p, b, c.coeffs + 3 * k, split, next, last, stream)) return KFAC_ERR_LAUNCH;
+      if (!launch_step(p, b, launches, c.coeffs + 3 * k, split, next, last, stream)) return KFAC_ERR_LAUNCH;
     }
   }
   return launch_status();

@@ -84,7 +84,7 @@ int main() {
         if (g.first != at) return 3;
         at += g.count;
         count += g.count;
-        if (g.R % g.tile || g.C % g.tile || g.R < g.r || g.C < g.c || g.r > g.c) return 4;
+        if (g.R % g.pad || g.C % g.pad || b.pad % g.pad || g.R < g.r || g.C < g.c || g.r > g.c) return 4;
         const long x = 2L * g.R * g.C * g.count, a = 2L * g.R * g.R * g.count;
         // the four operands lie behind one another and behind the group before
         if (g.x[0] != end || g.x[1] != end + x || g.a != end + 2 * x || g.b != end + 2 * x + a) return 5;
@@ -95,15 +95,39 @@ int main() {
         }
       }
       if (end > p.halves || count != b.count) return 7;
-      for (int sym = 0; sym < 2; ++sym) {
-        const int grid = orth_launch(b.groups, b.tile, sym);
-        int to = 0;
-        for (auto& g : b.groups) {
-          if (g.tile0 != to || g.tile0 % 8) return 8;
-          to += (g.tiles + 7) / 8 * 8;
+      for (int product = 0; product < 3; ++product)
+        for (int kind = -1; kind < ORTH_KINDS; ++kind) {
+          // the launch that is chosen, and those of all kinds that the padding allows
+          OrthLaunch l;
+          if (kind < 0) l = orth_launch(b, product);
+          else if (ORTH_KIND[kind].tile > b.pad) continue;
+          else orth_schedule(b, product, kind, l);
+          const int T = ORTH_KIND[l.kind].tile;
+          std::vector<int> owner(l.blocks, -1), fixed(l.fixes, -1);
+          for (size_t i = 0; i < b.groups.size(); ++i) {
+            const OrthGroup& g = b.groups[i];
+            const OrthSlice& s = l.slices[i];
+            if (s.tile > T || g.R % s.tile || g.C % s.tile) return 8;
+            const long t = g.R / s.tile;
+            if (s.tiles != g.count * (product == ORTH_APPLY ? t * (g.C / s.tile) : t * (t + 1) / 2)) return 9;
+            if (s.whole < 0 || s.whole > s.tiles || (s.whole < s.tiles && s.cuts < 1)) return 10;
+            if (s.tile0 % 8 || s.tile0 + (s.whole + 7) / 8 * 8 > l.pieces0) return 11;
+            for (int k = 0; k < (s.whole + 7) / 8 * 8; ++k)
+              if (owner[s.tile0 + k]++ != -1) return 12;
+            if (s.cuts == 0) continue;
+            // the pieces cover the reduction, none of them is empty
+            const int all = (product == ORTH_GRAM ? g.C : g.R) / 64;
+            if (s.len < 1 || s.len * s.cuts < all || s.len * (s.cuts - 1) >= all) return 13;
+            if (s.piece0 < l.pieces0) return 14;
+            for (int k = 0; k < (s.tiles - s.whole) * s.cuts; ++k)
+              if (owner[s.piece0 + k]++ != -1) return 15;
+            for (int k = 0; k < s.tiles - s.whole; ++k)
+              if (s.fix0 + k >= l.fixes || fixed[s.fix0 + k]++ != -1) return 16;
+          }
+          for (int o : fixed) if (o != 0) return 17;
+          for (int o : owner) if (o != 0) return 17;
+          if ((long)(l.blocks - l.pieces0) * T * T * 4 > ORTH_PARTIAL_BYTES) return 18;
         }
-        if (to != grid) return 9;
-      }
       seen += count;
     }
     printf("%ld %ld %ld\n", seen, (long)p.batches.size(), p.halves);
@@ -133,6 +157,11 @@ def test_plan_covers_every_matrix_once(plan):
     assert plan(many)[0] == 100 and plan(many)[1] > 1
     mixed = [(1000, 784), (10, 1000), (1000, 1000), (64, 147), (16384, 16384), (784, 1000)]
     assert plan(mixed)[0] == len(mixed)
+    # tiles that fill the chip unevenly, and long reductions of few tiles
+    for shapes in ([(4096, 9216), (4096, 4096), (1000, 4096)], [(10, 16384)], [(64, 16384), (300, 5000)],
+                   [(512, 4608)] * 3 + [(64, 576)] * 3 + [(2048, 512)] * 3, [(2048, 2048)] * 9 + [(600, 700)],
+                   [(16384, 16384)], [(1, 1)] * 40, [(513, 513)] * 31):
+        assert plan(shapes)[0] == len(shapes)
     # matrices that do not fit a batch together share the scratch one after another
     one, five = plan([(16384, 16384)]), plan([(16384, 16384)] * 5)
     assert five[0] == five[1] == 5 and five[2] == one[2]
