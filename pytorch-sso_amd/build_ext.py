@@ -15,7 +15,7 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'torchsso', 'libkfac_hip.so')
-HOST_SOURCE = os.path.join(CSRC, 'host_bindings.cpp')
+HOST_SOURCES = [os.path.join(CSRC, name) for name in ('host_bindings.cpp', 'host_norm.cpp')]
 HOST_OUT = os.path.join(HERE, 'torchsso', '_host.so')
 
 HIPCC_FLAGS = [
@@ -36,7 +36,7 @@ def host_command(hipcc):
     rocm = os.path.dirname(os.path.dirname(hipcc))
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     return ([hipcc, '-x', 'c++', '-O2', '-std=c++17', '-fPIC', '-shared', '-w', '-D__HIP_PLATFORM_AMD__',
-             '-D_GLIBCXX_USE_CXX11_ABI=%d' % abi, HOST_SOURCE, '-o', HOST_OUT,
+             '-D_GLIBCXX_USE_CXX11_ABI=%d' % abi] + HOST_SOURCES + ['-o', HOST_OUT,
              '-I' + sysconfig.get_paths()['include'], '-I' + os.path.join(root, 'include'),
              '-I' + os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
              '-I' + os.path.join(rocm, 'include'), '-L' + os.path.join(root, 'lib'), '-L' + os.path.join(rocm, 'lib'),
@@ -49,7 +49,7 @@ def build(verbose=True):
     cmd = host_command(hipcc)
     if verbose:
         print(' '.join(cmd), flush=True)
-    procs = [(HOST_SOURCE, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT))]
+    procs = [(' '.join(HOST_SOURCES), subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT))]
     for src in sources():
         obj = src[:-4] + '.o'
         cmd = [hipcc] + [f for f in HIPCC_FLAGS if f != '-shared'] + ['-c', src, '-o', obj]

@@ -17,6 +17,10 @@
 
 #include "../../include/kfac_hip.h"
 
+// (host_norm.cpp)
+PyObject* host_bind_norm(PyObject*, PyObject* const*, Py_ssize_t);
+PyObject* host_rms_norm(PyObject*, PyObject* const*, Py_ssize_t);
+
 namespace {
 
 // address of a tensor the engine can take, or nullptr
@@ -375,6 +379,8 @@ PyMethodDef methods[] = {
     {"rowsq_sum", KFAC_FAST(rowsq_sum), "rowsq_sum(function, x, channels, scale, shift): the sums, or None"},
     {"vectors", KFAC_FAST(vectors), "vectors(tensor, size, count): new vectors on its device"},
     {"order", KFAC_FAST(order), "order(device, waiting stream, stream waited for)"},
+    {"bind_norm", KFAC_FAST(host_bind_norm), "bind_norm(norm, workspace, backward): the library's entry points"},
+    {"rms_norm", KFAC_FAST(host_rms_norm), "rms_norm(x, residual, gain, eps, curvature, eight), or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,

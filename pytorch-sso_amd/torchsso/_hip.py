@@ -213,6 +213,8 @@ def load():
             fn.restype = res
             fn.argtypes = args
         _addresses['kfac_rowsq_sum'] = ctypes.cast(lib.kfac_rowsq_sum, ctypes.c_void_p).value
+        _host.bind_norm(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            'kfac_rms_norm', 'kfac_rms_norm_backward_workspace_bytes', 'kfac_rms_norm_backward')])
         _lib = lib
     return _lib
 

@@ -884,33 +884,41 @@ def _norm_dim(x):
     return x.shape[-1]
 
 
-def rms_norm(x, residual, gain, eps, eight_bit=False):
-    """(y, h, scale): h = x + residual (None without a residual), y = h / rms(h) * gain, in the type
-    of x or, with a float32 scale per row, in 8 bits (scale is None otherwise)."""
-    lib = _hip.load()
+def _check_rms_norm(x, residual, gain, curvature):
+    """Raises what is wrong with the arguments of a norm."""
     dim = _norm_dim(x)
-    kind = _element_type(x, 'input')
-    if residual is not None and residual.shape != x.shape:
-        raise _hip.KfacHipError('residual has shape %s, expected %s'
-                                % (tuple(residual.shape), tuple(x.shape)))
-    is_float, gain_ptr = _gain_args(gain, x, dim)
-    rows, ldx = _rows(x, dim)
-    x_ptr = _row_ptr(rows, x, 'input')
-    h = r_ptr = None
-    ldr = 0
+    _element_type(x, 'input')
+    _row_ptr(x, x, 'input')
     if residual is not None:
-        res, ldr = _rows(residual, dim)
-        r_ptr = _row_ptr(res, x, 'residual')
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if eight_bit else x.dtype, device=x.device)
-    scale = None
-    if eight_bit:
-        scale = torch.empty(x.shape[:-1] + (1,), dtype=torch.float32, device=x.device)
-    st = lib.kfac_rms_norm(kind, is_float, rows.shape[0], dim, x_ptr, ldx, r_ptr, ldr, gain_ptr, float(eps),
-                           y.data_ptr(), None if h is None else h.data_ptr(),
-                           None if scale is None else scale.data_ptr(), _hip.stream_ptr(x.device))
-    _hip.check(st, 'kfac_rms_norm')
-    return y, h, scale
+        if residual.shape != x.shape:
+            raise _hip.KfacHipError('residual has shape %s, expected %s'
+                                    % (tuple(residual.shape), tuple(x.shape)))
+        _row_ptr(residual, x, 'residual')
+    _gain_args(gain, x, dim)
+    if curvature is not None:
+        if tuple(curvature.shape) != (dim,):
+            raise _hip.KfacHipError('curvature has shape %s, expected (%d,)' % (tuple(curvature.shape), dim))
+        _hip.typed_ptr(curvature, torch.float32, x.device, 'curvature')
+    raise _hip.KfacHipError('rms_norm cannot take these arguments')
+
+
+def rms_norm_autograd(x, residual, gain, eps, curvature=None, eight_bit=False):
+    """y or (y, h) with h = x + residual and y = h / rms(h) * gain, with its backward pass (csrc/host_norm.cpp);
+    in 8 bits (y, scale) or (y, scale, h), without one."""
+    _hip.load()
+    out = _hip._host.rms_norm(x, residual, gain, eps, curvature, eight_bit)
+    if out is None:
+        _check_rms_norm(x, residual, gain, curvature)
+    return out
+
+
+@torch.no_grad()
+def rms_norm(x, residual, gain, eps, eight_bit=False):
+    """(y, h, scale) of rms_norm_autograd without a backward pass (None for what there is not)."""
+    out = rms_norm_autograd(x, residual, gain, eps, None, eight_bit)
+    if not isinstance(out, tuple):
+        return out, None, None
+    return (out[0], out[-1] if residual is not None else None, out[1] if eight_bit else None)
 
 
 def rms_norm_backward(dy, dh, h, gain, eps, samples, want_dx=True, want_dgain=True, curvature=None):

@@ -22,12 +22,42 @@ class DiagCovRMSNorm(DiagCurvature):
             raise TypeError('expected an RMSNorm module, got %s' % type(module).__name__)
         if isinstance(module, nn.RMSNorm) and len(module.normalized_shape) != 1:
             raise ValueError('RMSNorm over one dimension expected, got %s' % (tuple(module.normalized_shape),))
+        self._asked = []                # (tensor that a backward pass fills, its version before that)
         super(DiagCovRMSNorm, self).__init__(module, *args, **kwargs)
         if isinstance(module, RMSNorm):
-            module._curvature_done = self._receive
+            module._curvature = self
 
-    def _receive(self, curvature):
-        self._data = [curvature]
+    _ASKED_MOST = 4
+
+    def buffer(self, device):
+        """A tensor that the backward pass of one forward pass fills."""
+        t = torch.empty(self._module.dim, dtype=torch.float32, device=device)
+        self._asked = self._asked[1 - self._ASKED_MOST:] + [(t, t._version)]
+        return t
+
+    @property
+    def data(self):
+        """Of the latest forward pass that has had its backward pass (which changes its tensor's version)."""
+        for i in reversed(range(len(self._asked))):
+            t, version = self._asked[i]
+            if t._version != version:
+                self._data = [t]
+                self._asked = self._asked[i + 1:]
+                break
+        return self._data
+
+    @data.setter
+    def data(self, value):
+        self._asked = []
+        self._data = value
+
+    def adjust_data_scale(self, scale):
+        self.data                       # (takes what a backward pass has left)
+        super(DiagCovRMSNorm, self).adjust_data_scale(scale)
+
+    @property
+    def shape(self):
+        return self._get_shape()
 
     def forward_postprocess(self, module, input, output):
         assert self._module == module

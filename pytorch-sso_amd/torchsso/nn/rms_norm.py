@@ -9,58 +9,24 @@ in the same pass over memory as the gradients (curv/cov/rms_norm.py hands it to 
 """
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from torchsso import _ops
 
 
-class _RMSNorm(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, x, residual, gain, eps, curvature, done):
-        ctx.set_materialize_grads(False)
-        y, h, _ = _ops.rms_norm(x, residual, gain, eps)
-        ctx.save_for_backward(x if h is None else h, gain)
-        ctx.eps, ctx.curvature, ctx.done = eps, curvature, done
-        return y if h is None else (y, h)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, gain = ctx.saved_tensors
-        needs = ctx.needs_input_grad
-        curvature = ctx.curvature
-        want_dx = needs[0] or needs[1]
-        dgain = None
-        if dy is None:
-            dx = dh
-            if curvature is not None:
-                curvature.zero_()
-        elif not want_dx and not needs[2] and curvature is None:
-            dx = None
-        else:
-            dx, dgain = _ops.rms_norm_backward(dy, dh if want_dx else None, h, gain, ctx.eps,
-                                               h.shape[0] if h.dim() > 1 else 1, want_dx, needs[2], curvature)
-        if ctx.done is not None and curvature is not None:
-            ctx.done(curvature)
-        return dx if needs[0] else None, dx if needs[1] else None, dgain, None, None, None
-
-
-def _apply(x, residual, gain, eps, curvature, out_dtype, done=None):
+def _apply(x, residual, gain, eps, curvature, out_dtype):
     if not eps >= 0:
         raise ValueError('Invalid eps: {}'.format(eps))
     if curvature is not None and gain is None:
         raise ValueError('a curvature belongs to a gain')
     if out_dtype is None or out_dtype == x.dtype:
-        return _RMSNorm.apply(x, residual, gain, eps, curvature, done)
+        return _ops.rms_norm_autograd(x, residual, gain, eps, curvature)
     if out_dtype != torch.float8_e4m3fn:
         raise ValueError('Invalid out_dtype: {}'.format(out_dtype))
     if curvature is not None:
         raise ValueError('a result in 8 bits has no backward pass and no curvature')
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, gain)):
         raise ValueError('a result in 8 bits has no backward pass: call it under torch.no_grad()')
-    y, h, scale = _ops.rms_norm(x, residual, gain, eps, eight_bit=True)
-    return (y, scale) if h is None else (y, scale, h)
+    return _ops.rms_norm_autograd(x, residual, gain, eps, None, True)
 
 
 def rms_norm(x, gain=None, eps=1e-6, curvature=None, out_dtype=None):
@@ -89,13 +55,13 @@ class RMSNorm(nn.Module):
         self.dim = int(dim)
         self.eps = eps
         self.weight = nn.Parameter(torch.ones(self.dim, device=device, dtype=dtype))
-        self._curvature_done = None        # receives the curvature behind every backward pass
+        self._curvature = None             # a DiagCovRMSNorm: receives what the backward passes form
 
     def forward(self, x, residual=None):
         curvature = None
-        if self._curvature_done is not None and torch.is_grad_enabled():
-            curvature = torch.empty(self.dim, dtype=torch.float32, device=x.device)
-        return _apply(x, residual, self.weight, self.eps, curvature, None, self._curvature_done)
+        if self._curvature is not None and torch.is_grad_enabled():
+            curvature = self._curvature.buffer(x.device)
+        return _apply(x, residual, self.weight, self.eps, curvature, None)
 
     def extra_repr(self):
         return '{}, eps={}'.format(self.dim, self.eps)
