@@ -280,6 +280,7 @@ __global__ __launch_bounds__(block_threads(T)) void norm_backward_kernel(const B
     const V* const dy = (const V*)a.dy + row * a.lddy;
     const V* const h = (const V*)a.h + row * a.ldh;
     float g[N][E], v[N][E];
+    Pack<V, E> dh[N];
     float two[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -289,6 +290,7 @@ __global__ __launch_bounds__(block_threads(T)) void norm_backward_kernel(const B
       if (c >= a.dim) continue;
       load<V, E>(dy + c, g[n]);
       load<V, E>(h + c, v[n]);
+      if (a.dh) dh[n] = *(const Pack<V, E>*)((const V*)a.dh + row * a.lddh + c);
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -316,12 +318,9 @@ __global__ __launch_bounds__(block_threads(T)) void norm_backward_kernel(const B
         load_gain<V, E>(a.w, a.w_f32, c, w);
 #pragma unroll
         for (int e = 0; e < E; ++e) d[e] = r * (w[e] * g[n][e] - v[n][e] * k);
-        if (a.dh) {
-          float b[E];
-          load<V, E>((const V*)a.dh + row * a.lddh + c, b);
+        if (a.dh)
 #pragma unroll
-          for (int e = 0; e < E; ++e) d[e] += b[e];
-        }
+          for (int e = 0; e < E; ++e) d[e] += Element<V>::get(dh[n].v[e]);
         store<V, E>((V*)a.dx + row * a.dim + c, d);
       }
     }
@@ -406,74 +405,115 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(const BackArgs
   }
 }
 
-// The partial sums of the units, added up in an order that depends on their number alone: 64
-// columns a workgroup, 16 waves over the units.
-constexpr int REDUCE_WAVES = 16;
-__global__ __launch_bounds__(64 * REDUCE_WAVES) void norm_reduce_kernel(const float* partial, Deal d, int dim,
-                                                                        void* dw, int w_type, float* curvature) {
-  __shared__ float part[2][REDUCE_WAVES][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-  float sum = 0.f, sq = 0.f;
+// The partial sums of the units, added up in an order that depends on their number alone.  A workgroup
+// takes 32 columns, E of them to a thread, in G groups of threads over the units (1024 units of 4096
+// columns in 24 us with 16 groups of a column to a thread).
+constexpr int REDUCE_COLUMNS = 32, REDUCE_THREADS = 1024;
+template <int E>
+__global__ __launch_bounds__(REDUCE_THREADS) void norm_reduce_kernel(const float* partial, Deal d, int dim, void* dw,
+                                                                     int w_type, float* curvature) {
+  constexpr int LANES = REDUCE_COLUMNS / E, G = REDUCE_THREADS / LANES;
+  __shared__ float part[2][G][REDUCE_COLUMNS + 1];
+  const int group = threadIdx.x / LANES, column = threadIdx.x % LANES * E, c = blockIdx.x * REDUCE_COLUMNS + column;
+  float sum[E], sq[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum[e] = sq[e] = 0.f;
   const bool squares = curvature != nullptr;
-  const auto at = [&](int unit) { return c < dim ? partial[(long)unit * dim + c] : 0.f; };
-  // few samples in many parts: several waves a sample
-  const int share = d.parts > 0 && d.samples < REDUCE_WAVES ? REDUCE_WAVES / d.samples : 1;
+  // to = sum over `count` units from `first` on, `step` apart, several in flight
+  const auto add = [&](long first, long step, int count, float (&to)[E]) {
+    if (c >= dim) return;
+    const float* at = partial + first * dim + c;
+    constexpr int K = 8;
+    for (int i = 0; i < count; i += K) {
+      float v[K][E];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[k][e] = 0.f;
+        if (i + k < count) load<float, E>(at + (long)(i + k) * step * dim, v[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) to[e] += v[k][e];
+    }
+  };
+  // few samples in many parts: several groups a sample
+  const int share = d.parts > 0 && d.samples < G ? G / d.samples : 1;
   if (d.parts > 0) {
-    for (int n = wave / share; n < d.samples; n += REDUCE_WAVES / share) {
-      float s = 0.f;
-      for (int p = wave % share; p < d.parts; p += share) s += at(n * d.parts + p);
-      sum += s;
-      if (share == 1) sq = fmaf(s, s, sq);
+    for (int n = group / share; n < d.samples; n += G / share) {
+      float s[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[e] = 0.f;
+      const int p = group % share;
+      add((long)n * d.parts + p, share, p < d.parts ? (d.parts - p + share - 1) / share : 0, s);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        sum[e] += s[e];
+        if (share == 1) sq[e] = fmaf(s[e], s[e], sq[e]);
+      }
     }
   } else {
-    for (int u = wave; u < d.units; u += REDUCE_WAVES) {
-      sum += at(u);
-      if (squares) sq += at(u + d.units);
-    }
+    const int count = group < d.units ? (d.units - group + G - 1) / G : 0;
+    add(group, G, count, sum);
+    if (squares) add((long)group + d.units, G, count, sq);
   }
-  part[0][wave][lane] = sum;
-  part[1][wave][lane] = sq;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    part[0][group][column + e] = sum[e];
+    part[1][group][column + e] = sq[e];
+  }
   __syncthreads();
-  if (wave > 0 || c >= dim) return;
-  sum = sq = 0.f;
+  const int mine = threadIdx.x, to = blockIdx.x * REDUCE_COLUMNS + mine;
+  if (mine >= REDUCE_COLUMNS || to >= dim) return;
+  float total = 0.f, square = 0.f;
   if (share > 1) {
     for (int n = 0; n < d.samples; ++n) {
       float s = 0.f;
-      for (int i = 0; i < share; ++i) s += part[0][n * share + i][lane];
-      sum += s;
-      sq = fmaf(s, s, sq);
+      for (int i = 0; i < share; ++i) s += part[0][n * share + i][mine];
+      total += s;
+      square = fmaf(s, s, square);
     }
   } else {
-    for (int i = 0; i < REDUCE_WAVES; ++i) {
-      sum += part[0][i][lane];
-      sq += part[1][i][lane];
+    for (int i = 0; i < G; ++i) {
+      total += part[0][i][mine];
+      square += part[1][i][mine];
     }
   }
   if (dw) {
-    if (w_type == TYPE_F32) ((float*)dw)[c] = sum;
-    else if (w_type == TYPE_BF16) ((__hip_bfloat16*)dw)[c] = Element<__hip_bfloat16>::put(sum);
-    else ((_Float16*)dw)[c] = Element<_Float16>::put(sum);
+    if (w_type == TYPE_F32) ((float*)dw)[to] = total;
+    else if (w_type == TYPE_BF16) ((__hip_bfloat16*)dw)[to] = Element<__hip_bfloat16>::put(total);
+    else ((_Float16*)dw)[to] = Element<_Float16>::put(total);
   }
-  if (squares) curvature[c] = (float)d.samples * sq;
+  if (squares) curvature[to] = (float)d.samples * square;
 }
 
-// Threads a row and accesses a thread: a wave up to 4 accesses (16 of single elements), then 256
-// threads, then 1024; 0: longer than that.
+// Threads a row and accesses of `e` elements a thread; 0: longer than the registers of 1024 threads.
 struct Shape {
   int threads, accesses;
 };
-Shape shape_of(int dim, int e) {
-  const int n = (dim + e - 1) / e;
-  const int most = e == 1 ? 16 : 4;
+// forward: a wave up to four accesses (16 of single elements), then 256 threads, then 1024
+Shape norm_shape(int dim, int e) {
+  const int n = (dim + e - 1) / e, most = e == 1 ? 16 : 4;
   for (int t : {64, 256, 1024})
     for (int k : {most / 4, most / 2, most})
       if (n <= t * k) return Shape{t, k};
   return Shape{0, 0};
 }
+// backward, which holds three rows and the sums: at most two accesses a thread (16384 rows of 4096 in
+// bfloat16: two on 256 threads 132 us, 4.1 TB/s, one on 512 142; asking for the next row before the sums of
+// one are formed changes nothing)
+constexpr Shape BACK_SHAPES[] = {{64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}};
+Shape backward_shape(int dim, int e) {
+  const int n = (dim + e - 1) / e, scale = e == 1 ? 8 : 1;
+  for (const Shape& s : BACK_SHAPES)
+    if (n <= s.threads * s.accesses * scale) return Shape{s.threads, s.accesses * scale};
+  return Shape{0, 0};
+}
 
 Deal deal_rows(long rows, int samples, bool squares, int threads) {
   Deal d;
-  const long target = threads == 64 ? 4096 : threads == 256 ? 1024 : 512;
+  const long target = threads == 64 ? 4096 : threads == 0 || threads == 1024 ? 512 : 1024;
   d.samples = samples;
   d.tokens = rows / samples;
   const long per = std::max(1L, (rows + target - 1) / target);       // rows of a unit
@@ -493,7 +533,7 @@ Deal deal_rows(long rows, int samples, bool squares, int threads) {
 
 template <class V, int E>
 bool launch_norm(const NormArgs& a, hipStream_t stream) {
-  const Shape s = shape_of(a.dim, E);
+  const Shape s = norm_shape(a.dim, E);
 #define NORM_CASE(T, N)                                                                                   \
   if (s.threads == T && s.accesses == N) {                                                                \
     const long per = block_threads(T) / T;                                                                \
@@ -512,7 +552,7 @@ bool launch_norm(const NormArgs& a, hipStream_t stream) {
 
 template <class V, int E>
 bool launch_backward(const BackArgs& a, float* current, hipStream_t stream) {
-  const Shape s = shape_of(a.dim, E);
+  const Shape s = backward_shape(a.dim, E);
 #define BACK_CASE(T, N)                                                                                   \
   if (s.threads == T && s.accesses == N) {                                                                \
     const int per = block_threads(T) / T;                                                                 \
@@ -521,10 +561,8 @@ bool launch_backward(const BackArgs& a, float* current, hipStream_t stream) {
     else hipLaunchKernelGGL((norm_backward_kernel<V, E, T, N, false>), grid, block, 0, stream, a);        \
     return true;                                                                                          \
   }
-  constexpr int M = E == 1 ? 16 : 4;
-  BACK_CASE(64, M / 4) BACK_CASE(64, M / 2) BACK_CASE(64, M)
-  BACK_CASE(256, M / 4) BACK_CASE(256, M / 2) BACK_CASE(256, M)
-  BACK_CASE(1024, M / 4) BACK_CASE(1024, M / 2) BACK_CASE(1024, M)
+  constexpr int M = E == 1 ? 8 : 1;
+  BACK_CASE(64, M) BACK_CASE(64, 2 * M) BACK_CASE(256, M) BACK_CASE(256, 2 * M) BACK_CASE(512, 2 * M) BACK_CASE(1024, 2 * M)
 #undef BACK_CASE
   hipLaunchKernelGGL((norm_backward_long_kernel<V>), dim3(a.deal.units), dim3(1024), 0, stream, a, current);
   return true;
@@ -555,7 +593,7 @@ int run_norm(int type, const NormArgs& a, hipStream_t stream) {
 }
 
 // the deal must not depend on alignment (the caller asks for scratch by sizes alone)
-int deal_threads(int type, int dim) { return shape_of(dim, type == TYPE_F32 ? 4 : 8).threads; }
+int deal_threads(int type, int dim) { return backward_shape(dim, type == TYPE_F32 ? 4 : 8).threads; }
 
 size_t backward_floats(const Deal& d, int dim) { return (size_t)d.units * dim * (d.whole ? 3 : 1); }
 
@@ -605,8 +643,9 @@ int kfac_rms_norm_backward(int type, int gain_is_float, int64_t rows, int dim, i
     vec ? launch_backward<__hip_bfloat16, 8>(a, current, s) : launch_backward<__hip_bfloat16, 1>(a, current, s);
   else vec ? launch_backward<_Float16, 8>(a, current, s) : launch_backward<_Float16, 1>(a, current, s);
   if (sums)
-    hipLaunchKernelGGL(norm_reduce_kernel, dim3(cdiv(dim, 64)), dim3(64 * REDUCE_WAVES), 0, s, a.partial, a.deal, dim,
-                       dgain, gain_is_float ? TYPE_F32 : type, curvature);
+    hipLaunchKernelGGL((dim % 4 == 0 && ((uintptr_t)a.partial & 15) == 0 ? norm_reduce_kernel<4> : norm_reduce_kernel<1>),
+                       dim3(cdiv(dim, REDUCE_COLUMNS)), dim3(REDUCE_THREADS), 0, s, a.partial, a.deal, dim, dgain,
+                       gain_is_float ? TYPE_F32 : type, curvature);
   return launch_status();
 }
 
