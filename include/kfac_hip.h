@@ -507,7 +507,7 @@ int kfac_unpack_batched(int count, float* const* arrays, const int64_t* numel,
  * rows[i] x cols[i], contiguous row-major, of the element type `type` (0 float32, 1 bfloat16,
  * 2 float16), inputs and results alike; a matrix with more rows than columns is iterated on
  * transposed; a matrix without elements is skipped.  in[i] == out[i] is allowed.  coefficients:
- * HOST array of `steps` triples (a, b, c) under which |X| in the spectral norm stays below 7: a product's
+ * HOST array of `steps` triples (a, b, c), at most 64, under which |X| in the spectral norm stays below 7: a product's
  * operands are kept as fp16 numbers in two parts (22 bits; absolute error 2^-38) times 2^13.
  * late_steps: in as many steps at the end they are kept in one part (11 bits).  The update that a
  * layer takes in the place of the preconditioning of optim/secondorder.py:195-209 of the reference

@@ -50,10 +50,21 @@ constexpr long ORTH_UNITS = 256;           // compute units
 // tiles on and below the diagonal
 inline long orth_triangle(long t) { return t * (t + 1) / 2; }
 
-inline OrthPlan orth_plan(int count, const int* rows, const int* cols) {
+// Matrices that a workgroup iterates on by itself, in LDS, with sides padded to multiples of 32.  64 x 64 takes
+// 27 us and 16 x 20 15, where the seventeen launches of the others take about 90 even with next to nothing to
+// do.  Larger ones (64 x 256 50 us) are left to those launches, in which they cost nothing beside others.
+constexpr int ORTH_TINY_SIDE = 64, ORTH_TINY_SIZE = 4096;
+constexpr int ORTH_MAX_STEPS = 64;               // of an iteration (their coefficients travel as kernel arguments)
+inline bool orth_tiny(int rows, int cols) {
+  const int R = orth_pad(std::min(rows, cols), 32), C = orth_pad(std::max(rows, cols), 32);
+  return R <= ORTH_TINY_SIDE && R * C <= ORTH_TINY_SIZE;
+}
+
+// without_tiny: those are left out
+inline OrthPlan orth_plan(int count, const int* rows, const int* cols, bool without_tiny = false) {
   OrthPlan p;
   for (int i = 0; i < count; ++i)
-    if (rows[i] > 0 && cols[i] > 0) p.order.push_back(i);
+    if (rows[i] > 0 && cols[i] > 0 && !(without_tiny && orth_tiny(rows[i], cols[i]))) p.order.push_back(i);
   const auto lo = [&](int i) { return std::min(rows[i], cols[i]); };
   const auto hi = [&](int i) { return std::max(rows[i], cols[i]); };
   long large = 0;

@@ -584,13 +584,225 @@ void launch_passes(const OrthMat* mats, const OrthBatch& b, Momentum mom, double
                      (const double*)sums, eps, base, groups, (int)low);
 }
 
+// ---------------------------------------------------------------------------------------
+// small matrices
+// ---------------------------------------------------------------------------------------
+
+template <int N>
+struct TinyArgs {
+  OrthMat m[N];
+  float coeffs[3 * ORTH_MAX_STEPS];
+  int steps, update;
+  Momentum mom;
+  float eps;
+};
+static_assert(sizeof(TinyArgs<32>) <= 4096, "kernel arguments");
+
+constexpr int TINY_THREADS = 512, TINY_WAVES = 8;
+// halves between rows in LDS of n elements: 16 bytes more, so that rows begin in different banks
+__host__ __device__ constexpr int tiny_pitch(int n) { return n + 8; }
+constexpr int tiny_lds(int R, int C) { return 4 * R * tiny_pitch(C) + 8 * R * tiny_pitch(R); }
+// of 64 x 256, which needs most: rows cost more than columns
+constexpr int TINY_LDS = tiny_lds(ORTH_TINY_SIDE, ORTH_TINY_SIZE / ORTH_TINY_SIDE);
+static_assert(TINY_LDS >= tiny_lds(32, ORTH_TINY_SIZE / 32) && TINY_LDS <= 150 * 1024, "LDS of a small matrix");
+
+// The fragments of 32 reduction steps: of rows row0 ... row0 + 15 with k along them, or of columns.
+__device__ __forceinline__ h8 tiny_rows(lds_char* at, int pitch, int row0, int k0, int lane) {
+  return *(__attribute__((address_space(3))) h8*)(at + 2 * ((row0 + (lane & 15)) * pitch + k0 + 8 * (lane >> 4)));
+}
+__device__ __forceinline__ h8 tiny_columns(lds_char* at, int pitch, int col0, int k0, int lane) {
+  lds_char* const p = at + 2 * ((k0 + 8 * (lane >> 4) + ((lane & 15) >> 2)) * pitch + col0 + 4 * (lane & 3));
+  const h4s u = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) h4s*)p);
+  const h4s v = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) h4s*)(p + 8 * pitch));
+  return __builtin_bit_cast(h8, (h8s)__builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// A workgroup does all of one matrix: X, A and B in LDS in two parts, one launch for a list.  What bounds it
+// are latencies: of the instructions, which no workgroup before this one has fetched, and of a chain of short
+// phases.  So loops are rolled up, and where a product has fewer blocks than there are waves, these share its
+// reduction.
+template <class V, bool MUON, int N>
+__global__ __launch_bounds__(TINY_THREADS) void orth_tiny_kernel(const TinyArgs<N> a) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ double sums[TINY_WAVES];
+  __shared__ f4 shares[TINY_WAVES][64];
+  typedef __attribute__((address_space(3))) half_t lds_half;
+  typedef __attribute__((address_space(3))) h4 lds_h4;
+  typedef __attribute__((address_space(3))) h8 lds_h8;
+  const OrthMat& m = a.m[blockIdx.x];
+  const bool tall = m.rows > m.cols;
+  const int cols = m.cols, numel = m.rows * cols;
+  const int r = tall ? cols : m.rows, c = tall ? m.rows : cols;
+  const int R = (r + 31) / 32 * 32, C = (c + 31) / 32 * 32, px = tiny_pitch(C), pa = tiny_pitch(R);
+  lds_char* const x = (lds_char*)smem;               // two planes of R rows each
+  lds_char* const A = x + 4 * R * px;
+  lds_char* const B = A + 4 * R * pa;
+  const int xs = 2 * R * px, as = 2 * R * pa;        // bytes to the low plane
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const V* const in = (const V*)m.in;
+  for (int i = threadIdx.x; i < (4 * R * px + 8 * R * pa) / 16; i += TINY_THREADS)
+    ((lds_h8*)x)[i] = h8{0, 0, 0, 0, 0, 0, 0, 0};
+  // the direction, and with it the sum of squares, then the operand: a thread meets the same elements again
+  // and reads the momentum that it wrote
+  constexpr int K = 4;
+  double s = 0.;
+  float scale = 0.f;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int i0 = threadIdx.x; i0 < numel; i0 += K * TINY_THREADS) {
+      float u[K], b[K];
+#pragma unroll
+      for (int e = 0; e < K; ++e) {
+        const int i = i0 + e * TINY_THREADS;
+        u[e] = b[e] = 0.f;
+        if (i < numel) {
+          u[e] = Element<V>::get(in[i]);
+          if (MUON) b[e] = m.buf[i];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < K; ++e) {
+        const int i = i0 + e * TINY_THREADS;
+        if (i >= numel) break;
+        if (MUON) {
+          if (pass == 0) m.buf[i] = b[e] = fmaf(a.mom.mu, b[e], u[e]);
+          u[e] = a.mom.nesterov ? fmaf(a.mom.mu, b[e], u[e]) : b[e];
+        }
+        if (pass == 0) {
+          s = fma((double)u[e], (double)u[e], s);
+        } else {
+          const int p = i / cols, q = i - p * cols;
+          lds_half* const to = (lds_half*)x + (tall ? q * px + p : p * px + q);
+          const float v = u[e] * scale;
+          const half_t h = (half_t)v;
+          *to = h;
+          to[xs / 2] = (half_t)(v - (float)h);
+        }
+      }
+    }
+    if (pass == 0) {
+      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+      if (lane == 0) sums[wave] = s;
+    }
+    __syncthreads();
+    if (pass == 0) {
+      s = 0.;
+      for (int w = 0; w < TINY_WAVES; ++w) s += sums[w];
+      scale = (float)((double)ORTH_SCALE / (sqrt(s) + (double)a.eps));
+    }
+  }
+  constexpr float INV = 1.f / ORTH_SCALE;
+  const int nb = (r + 15) / 16, blocks = nb * (nb + 1) / 2, nl = lane & 15, ml = 4 * (lane >> 4);
+  const int share = blocks <= TINY_WAVES / 2 ? TINY_WAVES / blocks : 1;      // waves to a block
+  for (int step = 0; step < a.steps; ++step) {
+    const float ca = a.coeffs[3 * step], cb = a.coeffs[3 * step + 1], cc = a.coeffs[3 * step + 2];
+    // A = X X^T, then B = aI + bA + cAA: the blocks on and below the diagonal
+#pragma unroll 1
+    for (int poly = 0; poly < 2; ++poly) {
+      lds_char* const src = poly ? A : x;
+      lds_char* const dst = poly ? B : A;
+      const int pitch = poly ? pa : px, second = poly ? as : xs, K = poly ? R : C;
+      for (int b0 = 0; b0 < blocks; b0 += TINY_WAVES / share) {
+        const int b = b0 + wave / share;
+        int i = 0;
+        while ((i + 1) * (i + 2) / 2 <= b) ++i;
+        const int j = b - i * (i + 1) / 2;
+        f4 d0 = {0.f, 0.f, 0.f, 0.f}, d1 = d0, d2 = d0;
+        if (b < blocks && wave < blocks * share) {
+          for (int k = 32 * (wave % share); k < K; k += 32 * share) {
+            const h8 ph = tiny_rows(src, pitch, 16 * i, k, lane), pl = tiny_rows(src + second, pitch, 16 * i, k, lane);
+            const h8 qh = tiny_rows(src, pitch, 16 * j, k, lane), ql = tiny_rows(src + second, pitch, 16 * j, k, lane);
+            d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, d0, 0, 0, 0);
+            d1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, d1, 0, 0, 0);
+            d2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, d2, 0, 0, 0);
+          }
+        }
+        f4 d = (d0 + d1) + d2;
+        if (share > 1) {
+          shares[wave][lane] = d;
+          __syncthreads();
+          if (wave % share == 0)
+            for (int w = 1; w < share; ++w) d += shares[wave + w][lane];
+        }
+        if (b >= blocks || wave >= blocks * share || wave % share != 0) continue;
+        d *= INV;
+        const int mm = 16 * i + ml, n = 16 * j + nl;
+        if (poly) {
+          const h4 ah = *(lds_h4*)(A + 2 * (n * pa + mm)), al = *(lds_h4*)(A + as + 2 * (n * pa + mm));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            d[e] = fmaf(cc, d[e], cb * ((float)ah[e] + (float)al[e]));
+            if (mm + e == n) d[e] += ca * ORTH_SCALE;
+          }
+        }
+        h4 h, l;
+        split4(d, h, l);
+        *(lds_h4*)(dst + 2 * (n * pa + mm)) = h;
+        *(lds_h4*)(dst + as + 2 * (n * pa + mm)) = l;
+        if (i != j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            lds_half* const to = (lds_half*)dst + (mm + e) * pa + n;
+            *to = h[e];
+            to[as / 2] = l[e];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    // X = B X in place: a wave reads 16 columns whole and writes them
+    for (int col = 16 * wave; col < C; col += 16 * TINY_WAVES) {
+      constexpr int NB = ORTH_TINY_SIDE / 16;
+      f4 d[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) d[n] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < R; k += 32) {
+        const h8 ph = tiny_columns(x, px, col, k, lane), pl = tiny_columns(x + xs, px, col, k, lane);
+        h8 qh[NB], ql[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          if (n >= nb) continue;
+          qh[n] = tiny_rows(B, pa, 16 * n, k, lane);
+          ql[n] = tiny_rows(B + as, pa, 16 * n, k, lane);
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+          if (n < nb) d[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh[n], d[n], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+          if (n < nb) d[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql[n], d[n], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+          if (n < nb) d[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh[n], d[n], 0, 0, 0);
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        if (n >= nb) continue;
+        h4 h, l;
+        split4(d[n] * INV, h, l);
+        lds_char* const to = x + 2 * ((16 * n + nl) * px + col + ml);
+        *(lds_h4*)to = h;
+        *(lds_h4*)(to + xs) = l;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll 2
+  for (int i = threadIdx.x; i < numel; i += TINY_THREADS) {
+    const int p = i / cols, q = i - p * cols;
+    const lds_half* const from = (const lds_half*)x + (tall ? q * px + p : p * px + q);
+    const float o = ((float)from[0] + (float)from[xs / 2]) * INV;
+    V* const to = (V*)m.out + i;
+    *to = Element<V>::put(a.update ? m.keep * Element<V>::get(*to) - m.step * o : o);
+  }
+}
+
 struct Layout {
   size_t table, sums, partials, operands, bytes;
 };
 Layout layout(const OrthPlan& plan) {
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  Layout l;
-  l.table = 0;
+  Layout l{0, 0, 0, 0, 256};
+  if (plan.order.empty()) return l;        // small matrices alone
   l.sums = up(plan.order.size() * sizeof(OrthMat));
   long sums = 0;
   for (const OrthBatch& b : plan.batches) sums = std::max(sums, (long)b.count * SUM_MAX);
@@ -622,17 +834,69 @@ struct Call {
   int late;                          // steps at the end with single products
 };
 
+template <class V, bool MUON, int N>
+bool launch_tiny(const Call& c, const std::vector<int>& which, size_t first, hipStream_t stream) {
+  TinyArgs<N> a;
+  memset(&a, 0, sizeof(a));
+  const int n = (int)std::min(which.size() - first, (size_t)N);
+  int lds = 0;
+  for (int k = 0; k < n; ++k) {
+    const int i = which[first + k];
+    OrthMat& m = a.m[k];
+    m.in = c.in[i];
+    m.out = c.out[i];
+    m.buf = c.buf ? c.buf[i] : nullptr;
+    m.rows = c.rows[i];
+    m.cols = c.cols[i];
+    m.step = c.step ? c.step[i] : 0.f;
+    m.keep = c.keep ? c.keep[i] : 0.f;
+    lds = std::max(lds, tiny_lds(orth_pad(std::min(m.rows, m.cols), 32), orth_pad(std::max(m.rows, m.cols), 32)));
+  }
+  std::copy(c.coeffs, c.coeffs + 3 * c.steps, a.coeffs);
+  a.steps = c.steps;
+  a.update = c.step != nullptr;
+  a.mom = c.mom;
+  a.eps = c.eps;
+  const auto kernel = orth_tiny_kernel<V, MUON, N>;
+  if (!enable_large_lds((const void*)kernel, TINY_LDS)) return false;
+  hipLaunchKernelGGL(kernel, dim3(n), dim3(TINY_THREADS), lds, stream, a);
+  return true;
+}
+
+// (short lists have short arguments: they cost host time)
+template <class V, bool MUON>
+bool launch_tiny_list(const Call& c, const std::vector<int>& which, hipStream_t stream) {
+  for (size_t first = 0; first < which.size(); first += 32)
+    if (!(which.size() <= 4 ? launch_tiny<V, MUON, 4>(c, which, first, stream)
+                            : launch_tiny<V, MUON, 32>(c, which, first, stream)))
+      return false;
+  return true;
+}
+template <class V>
+bool launch_tiny_type(const Call& c, const std::vector<int>& which, hipStream_t stream) {
+  return c.buf ? launch_tiny_list<V, true>(c, which, stream) : launch_tiny_list<V, false>(c, which, stream);
+}
+
 int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (!sizes_ok(c.count, c.rows, c.cols)) return KFAC_ERR_ARG;
   if (c.count == 0) return KFAC_OK;
-  if (!c.in || !c.out || !c.coeffs || c.steps < 1 || c.late < 0 || c.type < TYPE_F32 || c.type > TYPE_F16)
+  if (!c.in || !c.out || !c.coeffs || c.steps < 1 || c.steps > ORTH_MAX_STEPS || c.late < 0 || c.type < TYPE_F32 || c.type > TYPE_F16)
     return KFAC_ERR_ARG;
-  OrthPlan plan = orth_plan(c.count, c.rows, c.cols);
-  if (plan.order.empty()) return KFAC_OK;
-  for (int i : plan.order)
+  std::vector<int> tiny;
+  for (int i = 0; i < c.count; ++i) {
+    if (c.rows[i] == 0 || c.cols[i] == 0) continue;
     if (!c.in[i] || !c.out[i] || (c.buf && !c.buf[i])) return KFAC_ERR_ARG;
+    if (orth_tiny(c.rows[i], c.cols[i])) tiny.push_back(i);
+  }
+  OrthPlan plan = orth_plan(c.count, c.rows, c.cols, true);
+  if (plan.order.empty() && tiny.empty()) return KFAC_OK;
   const Layout l = layout(plan);
   if (!workspace || workspace_bytes < l.bytes) return KFAC_ERR_WORKSPACE;
+  if (!tiny.empty() && !(c.type == TYPE_F32    ? launch_tiny_type<float>(c, tiny, stream)
+                         : c.type == TYPE_BF16 ? launch_tiny_type<__hip_bfloat16>(c, tiny, stream)
+                                               : launch_tiny_type<half_t>(c, tiny, stream)))
+    return KFAC_ERR_LAUNCH;
+  if (plan.order.empty()) return launch_status();
   std::vector<OrthMat> table(plan.order.size());
   std::vector<int> sum_blocks, pack_blocks;
   const size_t size = type_size(c.type);
@@ -710,7 +974,7 @@ extern "C" {
 size_t kfac_orthogonalize_workspace_bytes(int count, const int* rows, const int* cols) {
   try {
     if (!kfac::sizes_ok(count, rows, cols) || count == 0) return 0;
-    return kfac::layout(kfac::orth_plan(count, rows, cols)).bytes;
+    return kfac::layout(kfac::orth_plan(count, rows, cols, true)).bytes;
   } catch (const std::exception&) {
     return 0;
   }

@@ -29,6 +29,7 @@ def cholesky(m, upper=True):
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 # what a kernel's operand may hold (they are fp16 numbers times 2^13)
 _OPERAND_BOUND = 7.9
+_MOST_STEPS = 64
 
 
 def _largest(coeffs, x):
@@ -50,7 +51,7 @@ def _largest(coeffs, x):
 
 @functools.lru_cache(maxsize=64)
 def _flat_schedule(steps, coefficients):
-    if isinstance(steps, bool) or int(steps) != steps or steps < 1:
+    if isinstance(steps, bool) or int(steps) != steps or not 1 <= steps <= _MOST_STEPS:
         raise ValueError('Invalid steps: {}'.format(steps))
     triples = coefficients if isinstance(coefficients[0], tuple) else (coefficients,) * int(steps)
     if len(triples) != steps or any(len(t) != 3 for t in triples):
