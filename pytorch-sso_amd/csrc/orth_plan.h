@@ -124,10 +124,18 @@ inline OrthPlan orth_plan(int count, const int* rows, const int* cols, bool with
 enum { ORTH_LARGE, ORTH_MID, ORTH_DEEP, ORTH_SMALL, ORTH_KINDS };
 struct OrthKind {
   int tile, slots;       // workgroups at a time
-  float unit;            // us for 64 reduction steps of a tile, in two parts, with all slots taken
+  float unit, ends, poly_ends;   // us for 64 reduction steps of a tile, in two parts, and to start and end it
+                                 // (of B, which reads A and is written twice), with all slots taken
 };
-constexpr OrthKind ORTH_KIND[ORTH_KINDS] = {{256, 256, 4.4f}, {128, 512, 2.9f}, {64, 256, 0.6f}, {64, 512, 0.9f}};
-constexpr float ORTH_ENDS = 1.5f;          // what starting and ending a tile takes, in units
+// From 16 matrices of 1024 x 2752, 8 of 2048^2 and of 512 x 2048, a ResNet-50's, 784-1000-1000-10 and AlexNet's
+// layers, each in all kinds (what the padding allows), us with the second launch for pieces:
+//   A  200 218 - - - 570 / 169 208 30 64 21 640 / 232 333 31 69 14 1031 / 207 291 25 60 16 974
+//   B  98 228 - - - 351 / 82 219 19 36 23 382 / 114 349 17 36 14 668 / 98 291 12 27 17 633
+//   BX 249 313 - - - 948 / 293 369 28 86 27 1118 / 543 721 52 158 21 2079 / 445 598 39 112 17 1918
+constexpr OrthKind ORTH_KIND[ORTH_KINDS] = {{256, 256, 4.3f, 11.f, 20.f},
+                                            {128, 512, 2.7f, 6.5f, 6.5f},
+                                            {64, 256, 0.63f, 4.5f, 4.5f},
+                                            {64, 512, 1.f, 3.f, 3.f}};
 
 enum { ORTH_GRAM, ORTH_POLY, ORTH_APPLY };
 
@@ -189,6 +197,7 @@ inline float orth_schedule(const OrthBatch& b, int product, int kind, OrthLaunch
   out.slices.assign(n, OrthSlice{});
   std::vector<float> length(n);                   // of a tile, in this kind's units
   std::vector<int> order(n);
+  const float ends = (product == ORTH_POLY ? K.poly_ends : K.ends) / K.unit;
   double work = 0.;
   float longest = 0.f;
   for (int i = 0; i < n; ++i) {
@@ -196,7 +205,7 @@ inline float orth_schedule(const OrthBatch& b, int product, int kind, OrthLaunch
     OrthSlice& s = out.slices[i];
     s.tile = std::min(K.tile, g.pad);
     s.tiles = s.whole = (int)orth_tiles(g, s.tile, product);
-    length[i] = orth_length(g, product) * (s.tile < K.tile ? 0.6f : 1.f) + ORTH_ENDS;
+    length[i] = orth_length(g, product) * (s.tile < K.tile ? 0.6f : 1.f) + ends;
     work += (double)length[i] * s.tiles;
     longest = std::max(longest, length[i]);
     order[i] = i;
@@ -235,7 +244,7 @@ inline float orth_schedule(const OrthBatch& b, int product, int kind, OrthLaunch
         s.cuts = c;
         s.len = (all + c - 1) / c;
         const long m = (long)(s.tiles - s.whole) * c;
-        clock.take((length[i] - ORTH_ENDS) * s.len / all + ORTH_ENDS, m);
+        clock.take((length[i] - ends) * s.len / all + ends, m);
         pieces += m;
       }
       const long bytes = pieces * K.tile * K.tile * 4;
