@@ -30,11 +30,12 @@ struct OrthMat {
   int sum0, sums;        // its partial sums, and the workgroups that make them
   int pack0;             // first workgroup of the second pass (within the batch)
   float step, keep;      // parameter = keep * parameter - step * result
-  int vec;               // in and buf can be read 8 elements at a time
+  int aligned;           // in and buf can be read 8 elements at a time from their start
+  int vec;               // ... and from the start of every row
   int wide;              // out can be written 4 elements at a time
 };
 
-constexpr int SUM_ELEMS = 16384;                 // a workgroup of the first pass
+constexpr int SUM_ELEMS = 4096;                  // a workgroup of the first pass
 constexpr int SUM_MAX = 1024;                    // ... at most as many for a matrix
 constexpr int PACK_R = 64, PACK_C = 128;         // a workgroup of the second pass
 
@@ -69,37 +70,50 @@ __global__ __launch_bounds__(256) void orth_sum_kernel(const OrthMat* mats, int 
   const V* const in = (const V*)m.in;
   double s = 0.;
   constexpr int N = 8;
-  if (m.vec) {
-    for (long i = ((long)local * 256 + threadIdx.x) * N; i < m.numel; i += (long)m.sums * 256 * N) {
-      const Pack<V, N> g = *(const Pack<V, N>*)(in + i);
-      float b[N];
-      if (MUON) {
-        Pack<float, 4>* const at = (Pack<float, 4>*)(m.buf + i);
-        Pack<float, 4> b0 = at[0], b1 = at[1];
+  const long whole = m.aligned ? m.numel / N * N : 0;
+  for (long i = ((long)local * 256 + threadIdx.x) * N; i < whole; i += (long)m.sums * 256 * N) {
+    const Pack<V, N> g = *(const Pack<V, N>*)(in + i);
+    float b[N];
+    if (MUON) {
+      Pack<float, 4>* const at = (Pack<float, 4>*)(m.buf + i);
+      Pack<float, 4> b0 = at[0], b1 = at[1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          b[e] = b0.v[e] = fmaf(mom.mu, b0.v[e], Element<V>::get(g.v[e]));
-          b[e + 4] = b1.v[e] = fmaf(mom.mu, b1.v[e], Element<V>::get(g.v[e + 4]));
-        }
-        at[0] = b0;
-        at[1] = b1;
+      for (int e = 0; e < 4; ++e) {
+        b[e] = b0.v[e] = fmaf(mom.mu, b0.v[e], Element<V>::get(g.v[e]));
+        b[e + 4] = b1.v[e] = fmaf(mom.mu, b1.v[e], Element<V>::get(g.v[e + 4]));
       }
+      at[0] = b0;
+      at[1] = b1;
+    }
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        float u = Element<V>::get(g.v[e]);
-        if (MUON) u = mom.nesterov ? fmaf(mom.mu, b[e], u) : b[e];
-        s = fma((double)u, (double)u, s);
+    for (int e = 0; e < N; ++e) {
+      float u = Element<V>::get(g.v[e]);
+      if (MUON) u = mom.nesterov ? fmaf(mom.mu, b[e], u) : b[e];
+      s = fma((double)u, (double)u, s);
+    }
+  }
+  // the rest, or all where the addresses do not allow that
+  const long step = (long)m.sums * 256;
+  for (long i0 = whole + (long)local * 256 + threadIdx.x; i0 < m.numel; i0 += N * step) {
+    float u[N], b[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const long i = i0 + e * step;
+      u[e] = b[e] = 0.f;
+      if (i < m.numel) {
+        u[e] = Element<V>::get(in[i]);
+        if (MUON) b[e] = m.buf[i];
       }
     }
-  } else {
-    for (long i = (long)local * 256 + threadIdx.x; i < m.numel; i += (long)m.sums * 256) {
-      float u = Element<V>::get(in[i]);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const long i = i0 + e * step;
+      if (i >= m.numel) break;
       if (MUON) {
-        const float b = fmaf(mom.mu, m.buf[i], u);
-        m.buf[i] = b;
-        u = mom.nesterov ? fmaf(mom.mu, b, u) : b;
+        m.buf[i] = b[e] = fmaf(mom.mu, b[e], u[e]);
+        u[e] = mom.nesterov ? fmaf(mom.mu, b[e], u[e]) : b[e];
       }
-      s = fma((double)u, (double)u, s);
+      s = fma((double)u[e], (double)u[e], s);
     }
   }
   s = block_sum(s, tmp);
@@ -134,15 +148,28 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
   const V* const in = (const V*)m.in;
   const auto value = [&](long i) {
     float u = Element<V>::get(in[i]);
-    if (MUON) u = mom.nesterov ? fmaf(mom.mu, m.buf[i], u) : m.buf[i];
+    if (MUON) {
+      const float b = m.buf[i];
+      u = mom.nesterov ? fmaf(mom.mu, b, u) : b;
+    }
     return u * scale;
   };
   const bool tall = m.rows > m.cols;
   if (tall) {
     // in: rows of g.r values, as many as g.c
-    for (int i = threadIdx.x; i < PACK_R * PACK_C; i += 256) {
-      const int r = i % PACK_R, c = i / PACK_R;
-      tile[r][c] = r0 + r < g.r && c0 + c < g.c ? value((long)(c0 + c) * g.r + r0 + r) : 0.f;
+    for (int i0 = threadIdx.x; i0 < PACK_R * PACK_C; i0 += 8 * 256) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // (a load under a condition would wait for the one before it)
+        const int i = i0 + e * 256, r = min(r0 + i % PACK_R, g.r - 1), c = min(c0 + i / PACK_R, g.c - 1);
+        v[e] = value((long)c * g.r + r);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = i0 + e * 256, r = i % PACK_R, c = i / PACK_R;
+        tile[r][c] = r0 + r < g.r && c0 + c < g.c ? v[e] : 0.f;
+      }
     }
     __syncthreads();
   }
@@ -173,7 +200,9 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = c0 + c + e < g.c ? value(at + e) : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = value((long)(r0 + r) * g.c + min(c0 + c + e, g.c - 1));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c0 + c + e < g.c ? v[e] : 0.f;
     }
     h8 h, l;
 #pragma unroll
@@ -923,8 +952,8 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
       m.pack0 = pack0;
       m.step = c.step ? c.step[i] : 0.f;
       m.keep = c.keep ? c.keep[i] : 0.f;
-      // rows of whole 8-element groups at aligned addresses
-      m.vec = m.cols % 8 == 0 && ((uintptr_t)m.in % (8 * size)) == 0 && ((uintptr_t)m.buf & 15) == 0;
+      m.aligned = (uintptr_t)m.in % (8 * size) == 0 && ((uintptr_t)m.buf & 15) == 0;
+      m.vec = m.aligned && m.cols % 8 == 0;
       m.wide = m.cols % 4 == 0 && (uintptr_t)m.out % (4 * size) == 0;
       sum0 += m.sums;
       pack0 += cdiv(g.R, PACK_R) * cdiv(g.C, PACK_C);
