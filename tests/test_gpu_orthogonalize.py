@@ -249,3 +249,76 @@ def test_refusals_on_the_device():
         torchsso.optim.muon([g], [torch.zeros(4, 16, device='cuda')], [torch.zeros_like(g)], lr=0.1)
     with pytest.raises(ValueError):
         torchsso.optim.muon([g.t()[:, :4]], [g[:, :4]], [torch.zeros(8, 4, device='cuda')], lr=0.1)
+
+
+# ---------------------------------------------------------------------------------------
+# large tiles, reductions in pieces, several batches
+# ---------------------------------------------------------------------------------------
+
+def reference_on_device(g):
+    """`reference` of one matrix in 64 bits on the device (for sides that the host takes minutes for)."""
+    a, b, c = COEFFS
+    x = g.double()
+    tall = x.shape[0] > x.shape[1]
+    x = x.t().contiguous() if tall else x
+    x = x / (x.square().sum().sqrt() + 1e-7)
+    for _ in range(5):
+        m = x @ x.t().contiguous()
+        y = m @ x
+        x = a * x + b * y + c * (m @ y)
+    return x.t() if tall else x
+
+
+def off_on_device(got, want):
+    return ((got.double() - want).norm() / want.norm()).item()
+
+
+LISTS = {
+    # 256-wide tiles that fill the chip once and a little: the last round in pieces
+    'square': [(4096, 4096)],
+    'wide_and_tall': [(2048, 2310), (2310, 2048), (2047, 2304), (2100, 2050)],
+    # long reductions of few tiles, small matrices beside large ones
+    'long': [(512, 9000), (9001, 130), (64, 576), (20, 30)],
+    'mixed': [(1300, 2900), (2048, 2048), (2048, 2048), (3000, 700), (600, 600), (100, 2000), (48, 50)],
+    # many shapes of convolutions
+    'convolutions': [(64, 147), (64, 576), (256, 64), (128, 1152), (512, 128), (256, 2304), (1024, 256), (512, 4608),
+                     (2048, 512), (1000, 2048)],
+}
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('name', sorted(LISTS))
+def test_lists_of_all_sizes(name, dtype):
+    mats = [random(s, dtype, i) for i, s in enumerate(LISTS[name])]
+    for m, o in zip(mats, torchsso.utils.orthogonalize(mats)):
+        assert off_on_device(o, reference_on_device(m)) <= TOL[dtype]
+
+
+def test_more_than_a_batch():
+    """A list whose operands do not fit the scratch at once is worked on in parts."""
+    mats = [random((2048, 3500), torch.bfloat16, i) for i in range(16)]
+    outs = torchsso.utils.orthogonalize(mats)
+    for i in (0, 8, 15):
+        assert off_on_device(outs[i], reference_on_device(mats[i])) <= TOL[torch.bfloat16]
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_muon_of_large_matrices(dtype):
+    shapes = [(2048, 2304), (2304, 2048), (2047, 2100), (2100, 2046), (300, 5000)]
+    ps = [random(s, dtype, i) for i, s in enumerate(shapes)]
+    gs = [random(s, dtype, 10 + i) for i, s in enumerate(shapes)]
+    bufs = [random(s, torch.float32, 20 + i) for i, s in enumerate(shapes)]
+    want = []
+    for p, g, b in zip(ps, gs, bufs):
+        m = 0.9 * b.double() + g.double()
+        scale = max(1., p.shape[0] / p.shape[1]) ** 0.5
+        want.append((p.double() * 0.9 - scale * reference_on_device(g.double() + 0.9 * m), m))
+    torchsso.optim.muon(ps, gs, bufs, lr=1., momentum=0.9, weight_decay=0.1)
+    for p, b, (wp, wb) in zip(ps, bufs, want):
+        assert off_on_device(b, wb) <= 2 ** -23
+        assert off_on_device(p, wp) <= MUON_TOL[dtype] + off_on_device(wp.to(dtype), wp)
+
+
+def test_the_largest_side():
+    g = random((16384, 1030), torch.float32)
+    assert off_on_device(torchsso.utils.orthogonalize(g), reference_on_device(g)) <= TOL[torch.float32]
