@@ -176,15 +176,14 @@ template <class TILE, bool SPLIT, class OP_P, class OP_Q>
 __device__ __forceinline__ void orth_product(OP_P& P, OP_Q& Q, int steps, lds_char* lds, int wave, int team,
                                              f4 (&acc)[TILE::FM][TILE::FN]) {
   constexpr int S = TILE::STAGES, LOADS = OP_P::LOADS + OP_Q::LOADS, WK = TILE::WK;
+  static_assert(WK > 1, "teams");
   orth_clear<TILE>(acc);
   lds_char* const mine = lds + team * S * TILE::STAGE;
   const unsigned at = (unsigned)(uintptr_t)mine;
-  if (WK > 1) {
-    P.base += team * P.step;
-    Q.base += team * Q.step;
-    P.step *= WK;
-    Q.step *= WK;
-  }
+  P.base += team * P.step;
+  Q.base += team * Q.step;
+  P.step *= WK;
+  Q.step *= WK;
   const int own = (steps + WK - 1 - team) / WK, all = (steps + WK - 1) / WK;
   const auto load = [&](int stage) {
     P.load(at + stage * TILE::STAGE, wave);
@@ -200,7 +199,7 @@ __device__ __forceinline__ void orth_product(OP_P& P, OP_Q& Q, int steps, lds_ch
       load(into);
       ++ahead;
     }
-    if (WK == 1 || s < own) {
+    if (s < own) {
       lds_char* const stage = mine + cur * TILE::STAGE;
       h8 p[2][TILE::FM], q[2][TILE::FN];
       orth_read(P, stage, p);
@@ -210,21 +209,19 @@ __device__ __forceinline__ void orth_product(OP_P& P, OP_Q& Q, int steps, lds_ch
     into = cur;
     cur = cur + 1 == S ? 0 : cur + 1;
   }
-  if constexpr (WK > 1) {
-    typedef __attribute__((address_space(3))) f4 lds_f4;
-    constexpr int PER = TILE::FM * TILE::FN, TEAM = TILE::TEAM;
-    stage_barrier<0>();
-    lds_f4* const sums = (lds_f4*)lds + (threadIdx.x & (TEAM - 1));
-    if (team > 0)
+  typedef __attribute__((address_space(3))) f4 lds_f4;
+  constexpr int PER = TILE::FM * TILE::FN, TEAM = TILE::TEAM;
+  stage_barrier<0>();
+  lds_f4* const sums = (lds_f4*)lds + (threadIdx.x & (TEAM - 1));
+  if (team > 0)
 #pragma unroll
-      for (int i = 0; i < PER; ++i) sums[((team - 1) * PER + i) * TEAM] = acc[i / TILE::FN][i % TILE::FN];
-    stage_barrier<0>();
-    if (team == 0)
+    for (int i = 0; i < PER; ++i) sums[((team - 1) * PER + i) * TEAM] = acc[i / TILE::FN][i % TILE::FN];
+  stage_barrier<0>();
+  if (team == 0)
 #pragma unroll
-      for (int w = 0; w < WK - 1; ++w)
+    for (int w = 0; w < WK - 1; ++w)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i / TILE::FN][i % TILE::FN] += sums[(w * PER + i) * TEAM];
-  }
+      for (int i = 0; i < PER; ++i) acc[i / TILE::FN][i % TILE::FN] += sums[(w * PER + i) * TEAM];
 }
 
 // The same for a workgroup of eight waves that has the compute unit to itself, two waves on every

@@ -157,10 +157,6 @@ inline long orth_tiles(const OrthGroup& g, int tile, int product) {
 }
 inline int orth_length(const OrthGroup& g, int product) { return (product == ORTH_GRAM ? g.C : g.R) / 64; }
 
-struct OrthItems {
-  float length;
-  long n;
-};
 // When the last of the items is done, each taken by the slot that is free first, in order.
 struct OrthClock {
   std::vector<std::pair<float, long>> free;     // (time, slots), earliest first

@@ -122,7 +122,6 @@ __global__ __launch_bounds__(256) void orth_sum_kernel(const OrthMat* mats, int 
 
 struct OrthGroups {
   OrthGroup g[ORTH_GROUPS];
-  int n;
 };
 
 // Second pass: X, normalised, scaled and in halves, zeros in the padding.
@@ -226,7 +225,7 @@ struct OrthProduct {
   int from;              // which X is read (the other one is written)
   int low;               // APPLY: the next step reads X in two parts
   int type, update;      // LAST: type of the result; parameters are updated with it
-  int n, pieces0;
+  int pieces0;
   int tile0[ORTH_GROUPS], piece0[ORTH_GROUPS], fix0[ORTH_GROUPS];     // (beyond any workgroup: no group)
   OrthGroup g[ORTH_GROUPS];
   OrthSlice s[ORTH_GROUPS];
@@ -569,10 +568,9 @@ bool launch_product(OrthProduct& p, const OrthBatch& b, const OrthLaunch& l, boo
     if (u.tile0 != v.tile0) return u.tile0 < v.tile0;
     return u.piece0 < v.piece0;
   });
-  p.n = (int)order.size();
   p.pieces0 = l.pieces0;
   for (int i = 0; i < ORTH_GROUPS; ++i) {
-    const bool is = i < p.n;
+    const bool is = i < (int)order.size();
     if (is) {
       p.g[i] = b.groups[order[i]];
       p.s[i] = l.slices[order[i]];
@@ -607,7 +605,6 @@ void launch_passes(const OrthMat* mats, const OrthBatch& b, Momentum mom, double
                    int pack_blocks, float eps, half_t* base, bool low, hipStream_t stream) {
   hipLaunchKernelGGL((orth_sum_kernel<V, MUON>), dim3(sum_blocks), dim3(256), 0, stream, mats, b.count, mom, sums);
   OrthGroups groups;
-  groups.n = (int)b.groups.size();
   std::copy(b.groups.begin(), b.groups.end(), groups.g);
   hipLaunchKernelGGL((orth_pack_kernel<V, MUON>), dim3(pack_blocks), dim3(256), 0, stream, mats, b.count, mom,
                      (const double*)sums, eps, base, groups, (int)low);
@@ -631,7 +628,7 @@ constexpr int TINY_THREADS = 512, TINY_WAVES = 8;
 // halves between rows in LDS of n elements: 16 bytes more, so that rows begin in different banks
 __host__ __device__ constexpr int tiny_pitch(int n) { return n + 8; }
 constexpr int tiny_lds(int R, int C) { return 4 * R * tiny_pitch(C) + 8 * R * tiny_pitch(R); }
-// of 64 x 256, which needs most: rows cost more than columns
+// of 64 x 64, which needs most: rows cost more than columns
 constexpr int TINY_LDS = tiny_lds(ORTH_TINY_SIDE, ORTH_TINY_SIZE / ORTH_TINY_SIDE);
 static_assert(TINY_LDS >= tiny_lds(32, ORTH_TINY_SIZE / 32) && TINY_LDS <= 150 * 1024, "LDS of a small matrix");
 
@@ -645,6 +642,7 @@ __device__ __forceinline__ h8 tiny_columns(lds_char* at, int pitch, int col0, in
   const h4s v = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) h4s*)(p + 8 * pitch));
   return __builtin_bit_cast(h8, (h8s)__builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
 }
+
 // A workgroup does all of one matrix: X, A and B in LDS in two parts, one launch for a list.  What bounds it
 // are latencies: of the instructions, which no workgroup before this one has fetched, and of a chain of short
 // phases.  So loops are rolled up, and where a product has fewer blocks than there are waves, these share its
