@@ -153,21 +153,49 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
     }
     return u * scale;
   };
+  // 8 of them that lie side by side
+  const auto run = [&](long at, float (&v)[8]) {
+    const Pack<V, 8> p = *(const Pack<V, 8>*)(in + at);
+    float b[8];
+    if (MUON) {
+      *(Pack<float, 4>*)b = *(const Pack<float, 4>*)(m.buf + at);
+      *(Pack<float, 4>*)(b + 4) = *(const Pack<float, 4>*)(m.buf + at + 4);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float u = Element<V>::get(p.v[e]);
+      if (MUON) u = mom.nesterov ? fmaf(mom.mu, b[e], u) : b[e];
+      v[e] = u * scale;
+    }
+  };
   const bool tall = m.rows > m.cols;
   if (tall) {
     // in: rows of g.r values, as many as g.c
-    for (int i0 = threadIdx.x; i0 < PACK_R * PACK_C; i0 += 8 * 256) {
-      float v[8];
+    if (m.vec) {
+      // (a run of 8 is inside the matrix or outside; a wave's 64 runs are stored to different banks)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        // (a load under a condition would wait for the one before it)
-        const int i = i0 + e * 256, r = min(r0 + i % PACK_R, g.r - 1), c = min(c0 + i / PACK_R, g.c - 1);
-        v[e] = value((long)c * g.r + r);
+      for (int t = 0; t < PACK_R * PACK_C / 8 / 256; ++t) {
+        const int i = threadIdx.x + t * 256, r = i % (PACK_R / 8) * 8, c = i / (PACK_R / 8);
+        const bool inside = r0 + r < g.r && c0 + c < g.c;
+        float v[8];
+        run((long)min(c0 + c, g.c - 1) * g.r + min(r0 + r, g.r - 8), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tile[r + e][c] = inside ? v[e] : 0.f;
       }
+    } else {
+      for (int i0 = threadIdx.x; i0 < PACK_R * PACK_C; i0 += 8 * 256) {
+        float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = i0 + e * 256, r = i % PACK_R, c = i / PACK_R;
-        tile[r][c] = r0 + r < g.r && c0 + c < g.c ? v[e] : 0.f;
+        for (int e = 0; e < 8; ++e) {
+          // (a load under a condition would wait for the one before it)
+          const int i = i0 + e * 256, r = min(r0 + i % PACK_R, g.r - 1), c = min(c0 + i / PACK_R, g.c - 1);
+          v[e] = value((long)c * g.r + r);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int i = i0 + e * 256, r = i % PACK_R, c = i / PACK_R;
+          tile[r][c] = r0 + r < g.r && c0 + c < g.c ? v[e] : 0.f;
+        }
       }
     }
     __syncthreads();
@@ -185,18 +213,7 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = 0.f;
     } else if (m.vec && c0 + c + 8 <= g.c) {
-      const Pack<V, 8> p = *(const Pack<V, 8>*)(in + at);
-      float b[8];
-      if (MUON) {
-        *(Pack<float, 4>*)b = *(const Pack<float, 4>*)(m.buf + at);
-        *(Pack<float, 4>*)(b + 4) = *(const Pack<float, 4>*)(m.buf + at + 4);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float u = Element<V>::get(p.v[e]);
-        if (MUON) u = mom.nesterov ? fmaf(mom.mu, b[e], u) : b[e];
-        v[e] = u * scale;
-      }
+      run(at, v);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = value((long)(r0 + r) * g.c + min(c0 + c + e, g.c - 1));
