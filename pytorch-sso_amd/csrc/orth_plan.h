@@ -128,7 +128,7 @@ struct OrthKind {
                                  // (of B, which reads A and is written twice), with all slots taken
 };
 // From 16 matrices of 1024 x 2752, 8 of 2048^2 and of 512 x 2048, a ResNet-50's, 784-1000-1000-10 and AlexNet's
-// layers, each in all kinds (what the padding allows), us with the second launch for pieces:
+// layers, each in all kinds that the padding allows (large / mid / deep / small), us with the second launch for pieces:
 //   A  200 218 - - - 570 / 169 208 30 64 21 640 / 232 333 31 69 14 1031 / 207 291 25 60 16 974
 //   B  98 228 - - - 351 / 82 219 19 36 23 382 / 114 349 17 36 14 668 / 98 291 12 27 17 633
 //   BX 249 313 - - - 948 / 293 369 28 86 27 1118 / 543 721 52 158 21 2079 / 445 598 39 112 17 1918

@@ -56,7 +56,9 @@ __device__ __forceinline__ double block_sum(double v, double* tmp) {
 }
 
 // First pass: momentum, and the sum of squares in 64 bits (the squares of float32 numbers neither
-// overflow nor vanish there).
+// overflow nor vanish there).  Bound by memory: 58.6 million float32 elements in 54 us, 4.3 TB/s; 177
+// million bfloat16 ones with their momentum, in three launches, 293 us, 6.0 TB/s of the 10 bytes each (part
+// of which the caches hold).
 template <class V, bool MUON>
 __global__ __launch_bounds__(256) void orth_sum_kernel(const OrthMat* mats, int n, Momentum mom, double* sums) {
   __shared__ double tmp[4];
@@ -124,7 +126,9 @@ struct OrthGroups {
   OrthGroup g[ORTH_GROUPS];
 };
 
-// Second pass: X, normalised, scaled and in halves, zeros in the padding.
+// Second pass: X, normalised, scaled and in halves, zeros in the padding.  Bound by memory: the matrices
+// above 94 us, 5.0 TB/s, and 389 us, 4.6 TB/s, of 8 and 10 bytes an element.  A matrix stored transposed goes
+// through LDS, read in runs of 8 where its rows allow that (element by element the second figure is 527 us).
 template <class V, bool MUON>
 __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int n, Momentum mom, const double* sums,
                                                         float eps, half_t* base, OrthGroups groups, int low) {
@@ -482,6 +486,12 @@ __device__ __forceinline__ void orth_item(const OrthProduct& p, const OrthGroup&
                                 lds + TILE::SUMS + wave * TILE::WRITE, lane);
 }
 
+// One launch: the tiles of all groups, or pieces of them.  256-wide tiles run at 1390 TFLOP/s of fp16 products
+// (BX of AlexNet's layers, three products a number: 463 of float32 quality; the matrix cores busy 81 % of the
+// cycles at the 1.6 GHz that the power leaves), 1200 where a launch is one round of tiles and its tail; 128-wide
+// ones, two workgroups to a unit, at 1140 (A of 16 matrices of 1024 x 2752), both near what the library's own
+// fp16 product of 8192^3 reaches, 1250.  64-wide ones load 51 GB/s a unit, 13 TB/s in all, which bounds them: 635
+// (A of a ResNet-50's matrices), but they fill the chip where there are few tiles.
 template <class TILE, bool SPLIT, int MODE>
 __global__ __launch_bounds__(TILE::THREADS, TILE::LDS > 80 * 1024 ? 2 : 4) void orth_product_kernel(const OrthProduct p) {
   extern __shared__ __align__(16) char smem[];
@@ -513,7 +523,9 @@ __global__ __launch_bounds__(TILE::THREADS, TILE::LDS > 80 * 1024 ? 2 : 4) void 
 }
 
 // Adds up the pieces of cut tiles, in order; a workgroup takes two rows of fragments of a tile (32 rows of
-// each wave's part, a whole piece of the operands' layout).
+// each wave's part, a whole piece of the operands' layout).  7 to 16 us.  The last piece to end adding up
+// the others instead, in the products' launch, needs fences between the dies' caches that cost more: 17 -> 78 us
+// for A of 517 x 301, 1263 x 517 and 37 x 1263.
 template <class TILE, bool SPLIT, int MODE>
 __device__ __forceinline__ void orth_fix_item(const OrthProduct& p, int gi, int local, int i, int scale,
                                               lds_char* lds) {

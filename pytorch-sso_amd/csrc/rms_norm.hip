@@ -115,7 +115,8 @@ __device__ __forceinline__ void unit_reduce(float (&v)[K], float* tmp, int& turn
 
 constexpr int block_threads(int T) { return T < 256 ? 256 : T; }
 
-// T threads a row, N accesses of E elements each
+// T threads a row, N accesses of E elements each.  8193 rows of 5120 in bfloat16 with their residual, 8 bits
+// out: 58 us, 5.1 TB/s, a copy's rate; 16384 rows of 4096 with their residual 92 us, 5.8 TB/s.
 template <class V, int E, int T, int N>
 __global__ __launch_bounds__(block_threads(T)) void norm_kernel(const NormArgs a) {
   __shared__ float tmp[T > 64 ? 2 * T / 64 : 1];
@@ -406,8 +407,8 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(const BackArgs
 }
 
 // The partial sums of the units, added up in an order that depends on their number alone.  A workgroup
-// takes 32 columns, E of them to a thread, in G groups of threads over the units (1024 units of 4096
-// columns in 24 us with 16 groups of a column to a thread).
+// takes 32 columns, E of them to a thread, in G groups of threads over the units (1024 units of 4096 columns in
+// 7 to 8 us; in 24 with 16 groups of a column to a thread).
 constexpr int REDUCE_COLUMNS = 32, REDUCE_THREADS = 1024;
 template <int E>
 __global__ __launch_bounds__(REDUCE_THREADS) void norm_reduce_kernel(const float* partial, Deal d, int dim, void* dw,
@@ -501,7 +502,7 @@ Shape norm_shape(int dim, int e) {
   return Shape{0, 0};
 }
 // backward, which holds three rows and the sums: at most two accesses a thread (16384 rows of 4096 in
-// bfloat16: two on 256 threads 132 us, 4.1 TB/s, one on 512 142; asking for the next row before the sums of
+// bfloat16: two on 256 threads 123 to 132 us, 4.1 to 4.4 TB/s, one on 512 142; asking for the next row before the sums of
 // one are formed changes nothing)
 constexpr Shape BACK_SHAPES[] = {{64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}};
 Shape backward_shape(int dim, int e) {
