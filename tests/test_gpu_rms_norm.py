@@ -329,3 +329,16 @@ def test_refusals():
         torchsso.DiagCovRMSNorm(torch.nn.LayerNorm(5))
     with pytest.raises(ValueError):
         torchsso.DiagCovRMSNorm(torch.nn.RMSNorm((5, 6)))
+
+
+def test_more_elements_than_32_bits_count():
+    rows, dim = (1 << 18) + 3, 8192
+    x = torch.empty(rows, dim, device='cuda', dtype=torch.bfloat16).normal_().requires_grad_()
+    gain = torch.linspace(0.5, 2., dim, device='cuda')
+    y = torchsso.nn.rms_norm(x, gain)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    for part in (slice(0, 2), slice(rows // 2, rows // 2 + 2), slice(rows - 2, rows)):
+        xs = x.detach()[part].clone().requires_grad_()
+        ys = torchsso.nn.rms_norm(xs, gain)
+        assert torch.equal(y[part], ys)
+        assert torch.equal(dx[part], torch.autograd.grad(ys, xs, xs.detach())[0])
