@@ -52,6 +52,33 @@ __device__ __forceinline__ void store(V* p, const float (&v)[N]) {
   for (int e = 0; e < N; ++e) a.v[e] = Element<V>::put(v[e]);
   *(Pack<V, N>*)p = a;
 }
+
+// 16 bytes of a stream.  ONCE: of more bytes in all than the last cache holds, which are not to displace one
+// another there: 16384 rows of 4096 in bfloat16 forward and backward 219 us without that, 206 with it, 8193
+// rows of 5120 to 8 bits 64 and 56.  Where the caches hold them for the kernels in front and behind it costs
+// (4096 rows of 4096 between two other operations on them: forward 48 us without and 51 with it, backward 55
+// and 66).
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+constexpr long LAST_CACHE = 256L << 20;
+template <bool ONCE, class V, int N>
+__device__ __forceinline__ Pack<V, N> stream_load(const V* p) {
+  if constexpr (ONCE) return __builtin_bit_cast(Pack<V, N>, __builtin_nontemporal_load((const u4*)p));
+  else return *(const Pack<V, N>*)p;
+}
+template <bool ONCE, class V, int N>
+__device__ __forceinline__ void stream_load(const V* p, float (&v)[N]) {
+  const Pack<V, N> a = stream_load<ONCE, V, N>(p);
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = Element<V>::get(a.v[e]);
+}
+template <bool ONCE, class V, int N>
+__device__ __forceinline__ void stream_store(V* p, const float (&v)[N]) {
+  Pack<V, N> a;
+#pragma unroll
+  for (int e = 0; e < N; ++e) a.v[e] = Element<V>::put(v[e]);
+  if constexpr (ONCE) __builtin_nontemporal_store(__builtin_bit_cast(u4, a), (u4*)p);
+  else *(Pack<V, N>*)p = a;
+}
 template <class V, int N>
 __device__ __forceinline__ void load_gain(const void* w, int w_f32, int c, float (&v)[N]) {
   if (w == nullptr) {
@@ -116,8 +143,8 @@ __device__ __forceinline__ void unit_reduce(float (&v)[K], float* tmp, int& turn
 constexpr int block_threads(int T) { return T < 256 ? 256 : T; }
 
 // T threads a row, N accesses of E elements each.  8193 rows of 5120 in bfloat16 with their residual, 8 bits
-// out: 58 us, 5.1 TB/s, a copy's rate; 16384 rows of 4096 with their residual 92 us, 5.8 TB/s.
-template <class V, int E, int T, int N>
+// out: 56 us, 5.2 TB/s, a copy's rate; 16384 rows of 4096 with their residual 91 us, 5.9 TB/s.
+template <class V, int E, int T, int N, bool ONCE>
 __global__ __launch_bounds__(block_threads(T)) void norm_kernel(const NormArgs a) {
   __shared__ float tmp[T > 64 ? 2 * T / 64 : 1];
   const int t = threadIdx.x % T;
@@ -135,10 +162,10 @@ __global__ __launch_bounds__(block_threads(T)) void norm_kernel(const NormArgs a
 #pragma unroll
     for (int e = 0; e < E; ++e) h[n][e] = 0.f;
     if (c >= a.dim) continue;
-    load<V, E>(x + c, h[n]);
+    stream_load<ONCE, V, E>(x + c, h[n]);
     if (res) {
       float b[E];
-      load<V, E>(res + c, b);
+      stream_load<ONCE, V, E>(res + c, b);
 #pragma unroll
       for (int e = 0; e < E; ++e) h[n][e] = Element<V>::get(Element<V>::put(h[n][e] + b[e]));
     }
@@ -147,7 +174,7 @@ __global__ __launch_bounds__(block_threads(T)) void norm_kernel(const NormArgs a
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int c = (n * T + t) * E;
-      if (c < a.dim) store<V, E>(hout + c, h[n]);
+      if (c < a.dim) stream_store<ONCE, V, E>(hout + c, h[n]);
     }
   }
 #pragma unroll
@@ -168,7 +195,7 @@ __global__ __launch_bounds__(block_threads(T)) void norm_kernel(const NormArgs a
       h[n][e] = h[n][e] * r * w[e];
       top[0] = fmaxf(top[0], fabsf(h[n][e]));
     }
-    if (!a.scale) store<V, E>((V*)a.y + row * a.dim + c, h[n]);
+    if (!a.scale) stream_store<ONCE, V, E>((V*)a.y + row * a.dim + c, h[n]);
   }
   if (!a.scale) return;
   unit_reduce<Max, T, 1>(top, tmp, turn);
@@ -256,7 +283,7 @@ __device__ __forceinline__ void unit_rows(const Deal& d, long all, int unit, lon
   }
 }
 
-template <class V, int E, int T, int N, bool WHOLE>
+template <class V, int E, int T, int N, bool WHOLE, bool ONCE>
 __global__ __launch_bounds__(block_threads(T)) void norm_backward_kernel(const BackArgs a) {
   __shared__ float tmp[T > 64 ? 4 * T / 64 : 1];
   const int t = threadIdx.x % T;
@@ -289,9 +316,9 @@ __global__ __launch_bounds__(block_threads(T)) void norm_backward_kernel(const B
 #pragma unroll
       for (int e = 0; e < E; ++e) g[n][e] = v[n][e] = 0.f;
       if (c >= a.dim) continue;
-      load<V, E>(dy + c, g[n]);
-      load<V, E>(h + c, v[n]);
-      if (a.dh) dh[n] = *(const Pack<V, E>*)((const V*)a.dh + row * a.lddh + c);
+      stream_load<ONCE, V, E>(dy + c, g[n]);
+      stream_load<ONCE, V, E>(h + c, v[n]);
+      if (a.dh) dh[n] = stream_load<ONCE, V, E>((const V*)a.dh + row * a.lddh + c);
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -322,7 +349,7 @@ __global__ __launch_bounds__(block_threads(T)) void norm_backward_kernel(const B
         if (a.dh)
 #pragma unroll
           for (int e = 0; e < E; ++e) d[e] += Element<V>::get(dh[n].v[e]);
-        store<V, E>((V*)a.dx + row * a.dim + c, d);
+        stream_store<ONCE, V, E>((V*)a.dx + row * a.dim + c, d);
       }
     }
     if (WHOLE && ++token == a.deal.tokens) {
@@ -502,7 +529,7 @@ Shape norm_shape(int dim, int e) {
   return Shape{0, 0};
 }
 // backward, which holds three rows and the sums: at most two accesses a thread (16384 rows of 4096 in
-// bfloat16: two on 256 threads 123 to 132 us, 4.1 to 4.4 TB/s, one on 512 142; asking for the next row before the sums of
+// bfloat16: two on 256 threads 112 us, 4.8 TB/s; with cached streams 132, one on 512 142; asking for the next row before the sums of
 // one are formed changes nothing)
 constexpr Shape BACK_SHAPES[] = {{64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}};
 Shape backward_shape(int dim, int e) {
@@ -532,13 +559,16 @@ Deal deal_rows(long rows, int samples, bool squares, int threads) {
   return d;
 }
 
-template <class V, int E>
+template <class V, int E, bool ONCE = false>
 bool launch_norm(const NormArgs& a, hipStream_t stream) {
+  const long bytes = a.rows * a.dim * (long)((a.residual ? 3 : a.h ? 2 : 1) * sizeof(V) + (a.scale ? 1 : sizeof(V)));
+  if constexpr (E > 1 && !ONCE)
+    if (bytes > LAST_CACHE) return launch_norm<V, E, true>(a, stream);
   const Shape s = norm_shape(a.dim, E);
 #define NORM_CASE(T, N)                                                                                   \
   if (s.threads == T && s.accesses == N) {                                                                \
     const long per = block_threads(T) / T;                                                                \
-    hipLaunchKernelGGL((norm_kernel<V, E, T, N>), dim3((unsigned)((a.rows + per - 1) / per)),             \
+    hipLaunchKernelGGL((norm_kernel<V, E, T, N, ONCE>), dim3((unsigned)((a.rows + per - 1) / per)),       \
                        dim3(block_threads(T)), 0, stream, a);                                             \
     return true;                                                                                          \
   }
@@ -551,15 +581,20 @@ bool launch_norm(const NormArgs& a, hipStream_t stream) {
   return true;
 }
 
-template <class V, int E>
+template <class V, int E, bool ONCE = false>
 bool launch_backward(const BackArgs& a, float* current, hipStream_t stream) {
+  const long bytes = a.rows * a.dim * (long)((2 + (a.dh != nullptr) + (a.dx != nullptr)) * sizeof(V));
+  if constexpr (E > 1 && !ONCE)
+    if (bytes > LAST_CACHE) return launch_backward<V, E, true>(a, current, stream);
   const Shape s = backward_shape(a.dim, E);
 #define BACK_CASE(T, N)                                                                                   \
   if (s.threads == T && s.accesses == N) {                                                                \
     const int per = block_threads(T) / T;                                                                 \
     const dim3 grid(cdiv(a.deal.units, per)), block(block_threads(T));                                    \
-    if (a.deal.whole) hipLaunchKernelGGL((norm_backward_kernel<V, E, T, N, true>), grid, block, 0, stream, a);   \
-    else hipLaunchKernelGGL((norm_backward_kernel<V, E, T, N, false>), grid, block, 0, stream, a);        \
+    if (a.deal.whole)                                                                                     \
+      hipLaunchKernelGGL((norm_backward_kernel<V, E, T, N, true, ONCE>), grid, block, 0, stream, a);      \
+    else                                                                                                  \
+      hipLaunchKernelGGL((norm_backward_kernel<V, E, T, N, false, ONCE>), grid, block, 0, stream, a);     \
     return true;                                                                                          \
   }
   constexpr int M = E == 1 ? 8 : 1;

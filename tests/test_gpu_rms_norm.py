@@ -342,3 +342,25 @@ def test_more_elements_than_32_bits_count():
         ys = torchsso.nn.rms_norm(xs, gain)
         assert torch.equal(y[part], ys)
         assert torch.equal(dx[part], torch.autograd.grad(ys, xs, xs.detach())[0])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize('dim', [96, 1000, 5120])
+def test_streams_beyond_the_caches_give_what_a_few_rows_give(dtype, dim):
+    rows = (1 << 28) // (dim * 4) + 7           # (every tensor of them: 128 MiB or more)
+    gen = torch.Generator(device='cuda').manual_seed(dim)
+    x, res, dy, dh = (torch.empty(rows, dim, device='cuda', dtype=dtype).normal_(generator=gen) for _ in range(4))
+    gain = torch.linspace(0.5, 2., dim, device='cuda')
+
+    def passes(x, res, dy, dh):
+        x, res = x.clone().requires_grad_(), res.clone().requires_grad_()
+        y, h = torchsso.nn.add_rms_norm(x, res, gain)
+        with torch.no_grad():
+            eight = torchsso.nn.add_rms_norm(x, res, gain, out_dtype=torch.float8_e4m3fn)
+        return (y, h) + torch.autograd.grad((y, h), (x, res), (dy, dh)) + (eight[0].view(torch.uint8), eight[1], eight[2])
+
+    whole = passes(x, res, dy, dh)
+    for part in (slice(0, 3), slice(rows // 2, rows // 2 + 3), slice(rows - 3, rows)):
+        few = passes(x[part], res[part], dy[part], dh[part])
+        for a, b in zip(whole, few):
+            assert torch.equal(a[part], b)
