@@ -4,6 +4,8 @@ Each wrapper checks shapes on the host before anything is launched, brings the
 scratch the entry point asks for, and enqueues on torch's current stream.
 """
 import ctypes
+import functools
+import math
 
 import torch
 
@@ -796,11 +798,37 @@ def _matrix_dims(mats, what):
     return _hip.ints([m.shape[0] for m in mats]), _hip.ints([m.shape[1] for m in mats])
 
 
-# In as many steps at the end of an orthogonalisation operands are kept in 11 bits instead of 22.
-# What a step rounds away grows by the slope of the iteration at zero (3.4) with every step behind
-# it, where a direction of the gradient is weak; of the last two at most 12 * 2^-12 is left where
-# a bfloat16 result rounds by 2^-9, and no step is late where the result holds more bits.
-LATE_STEPS = {torch.float32: 0, torch.float16: 0, torch.bfloat16: 2}
+@functools.lru_cache(maxsize=64)
+def late_steps(dtype, coefficients):
+    """In how many steps at the end of an orthogonalisation operands are kept in 11 bits instead of 22.
+
+    None of them where the result holds 11 bits or more.  Rounding X to 11 bits loses an eighth of what
+    rounding the result to bfloat16's 8 loses; in that unit a late step, f(t) = a t + b t^3 + c t^5 on
+    singular values t, turns an error e of X into at most
+        e' = max |t / f(t)| * sqrt(L^2 (e^2 + 1) + P^2),   L = max |f'|,  P = max |f(t) / t|:
+    X is rounded, and so is the diagonal of B; the factor in front is that of a matrix whose norm lies
+    in one direction while the errors lie in weak ones.  (What A rounds away is spread over all of it, and
+    that direction meets but a small part.)  As many steps are late as keep the result, at worst, within
+    1.5 times the error that its own rounding makes: e' <= 8 sqrt(1.5^2 - 1) = 8.9.  Of five steps of the
+    default coefficients that is one (8.1; a second one would make it 50): rank one with noise of 10^-3
+    is then 1.86e-3 from 64 bits, where the rounding alone makes 1.63e-3."""
+    if dtype != torch.bfloat16:
+        return 0
+    steps, bound = [], 1.               # (slope, largest and smallest factor) of each
+    for a, b, c in zip(*[iter(coefficients)] * 3):
+        ts = [bound * i / 256 for i in range(257)]
+        factors = [abs(a + b * t ** 2 + c * t ** 4) for t in ts]
+        steps.append((max(abs(a + 3 * b * t ** 2 + 5 * c * t ** 4) for t in ts), max(factors), min(factors)))
+        bound = max(t * f for t, f in zip(ts, factors))
+    late = 0
+    while late < len(steps):
+        error = 0.
+        for slope, most, least in steps[len(steps) - late - 1:]:
+            error = math.inf if least == 0. else math.sqrt(slope ** 2 * (error ** 2 + 1) + most ** 2) / least
+        if error > 8.9:
+            break
+        late += 1
+    return late
 
 
 def orthogonalize_batched(mats, outs, coefficients, eps):
@@ -819,7 +847,7 @@ def orthogonalize_batched(mats, outs, coefficients, eps):
     ws, ws_bytes = _hip.workspace(first.device, lib.kfac_orthogonalize_workspace_bytes(len(mats), rows, cols))
     st = lib.kfac_orthogonalize_batched(
         len(mats), rows, cols, kind, ins, results, len(coefficients) // 3, _hip.floats(coefficients),
-        float(eps), LATE_STEPS[first.dtype], _ws_ptr(ws), ws_bytes, _hip.stream_ptr(first.device))
+        float(eps), late_steps(first.dtype, tuple(coefficients)), _ws_ptr(ws), ws_bytes, _hip.stream_ptr(first.device))
     _hip.check(st, 'kfac_orthogonalize_batched')
 
 
@@ -845,7 +873,7 @@ def muon_update_batched(params, grads, buffers, step_sizes, keeps, momentum, nes
     st = lib.kfac_muon_update_batched(
         len(params), rows, cols, kind, ps, gs, bs, _hip.floats(step_sizes), _hip.floats(keeps),
         float(momentum), int(bool(nesterov)), len(coefficients) // 3, _hip.floats(coefficients),
-        float(eps), LATE_STEPS[first.dtype], _ws_ptr(ws), ws_bytes, _hip.stream_ptr(first.device))
+        float(eps), late_steps(first.dtype, tuple(coefficients)), _ws_ptr(ws), ws_bytes, _hip.stream_ptr(first.device))
     _hip.check(st, 'kfac_muon_update_batched')
 
 

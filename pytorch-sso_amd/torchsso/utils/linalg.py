@@ -88,8 +88,9 @@ def orthogonalize(mats, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     list of such tensors, in float32, bfloat16 or float16 (one type a list).  Returns new
     tensors of the same shapes and type.  `coefficients`: (a, b, c), or one triple per step.
 
-    Products run on the fp16 matrix cores in two parts a number (as good as float32); of a bfloat16
-    matrix the last two steps in one part, whose rounding is below that of the result."""
+    Products run on the fp16 matrix cores in two parts a number (as good as float32).  Of a bfloat16
+    matrix the last steps run in one part, as many as leave at most 1.5 times the error that rounding the
+    result makes (of the default steps one)."""
     schedule = newton_schulz_schedule(steps, coefficients)
     if not eps > 0:
         raise ValueError('Invalid eps: {}'.format(eps))
