@@ -297,6 +297,10 @@ class _Workspace(threading.local):
         if device.type != 'cuda':
             raise KfacHipError('scratch requested on %s: the K-FAC kernels run on a HIP device '
                                'only (no CPU path exists in this package)' % device)
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            buf = self._recorded(device, nbytes, stream)
+            if buf is not None:
+                return buf, nbytes
         key = (device.type, device.index, stream_ptr(device, stream))
         buf = self.bufs.get(key)
         if buf is None or buf.numel() < nbytes:
@@ -309,6 +313,19 @@ class _Workspace(threading.local):
             buf = torch.empty(size, dtype=torch.uint8, device=device)
             self.bufs[key] = buf
         return buf, buf.numel()
+
+    @staticmethod
+    def _recorded(device, nbytes, stream):
+        """Scratch of a call that is being recorded: memory of the graph, which writes to it at every
+        replay.  (A cached buffer would be dropped for a larger one some time, or be in use by other
+        work of its stream meanwhile.)  None where `stream` is not part of the recording."""
+        if stream is None:
+            return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        # (taken under that stream: what is freed here may be handed out again to work behind it there)
+        with torch.cuda.stream(stream):
+            if torch.cuda.is_current_stream_capturing():
+                return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return None
 
 
 _workspace = _Workspace()
