@@ -15,6 +15,7 @@
 
 #include "common.h"
 #include "element_types.h"
+#include "norm_rows.h"
 
 namespace kfac {
 namespace {
@@ -559,6 +560,19 @@ Deal deal_rows(long rows, int samples, bool squares, int threads) {
   return d;
 }
 
+// `n` rows of `a` from `first` on
+template <class V>
+NormArgs norm_rows(NormArgs a, long first, long n) {
+  const auto ahead = [](const void* p, long elements, size_t size) { return p ? (const char*)p + elements * (long)size : nullptr; };
+  a.x = ahead(a.x, first * a.ldx, sizeof(V));
+  a.residual = ahead(a.residual, first * a.ldr, sizeof(V));
+  a.y = (void*)ahead(a.y, first * a.dim, a.scale ? 1 : sizeof(V));
+  a.h = (void*)ahead(a.h, first * a.dim, sizeof(V));
+  a.scale = (float*)ahead(a.scale, first, sizeof(float));
+  a.rows = n;
+  return a;
+}
+
 template <class V, int E, bool ONCE = false>
 bool launch_norm(const NormArgs& a, hipStream_t stream) {
   const long bytes = a.rows * a.dim * (long)((a.residual ? 3 : a.h ? 2 : 1) * sizeof(V) + (a.scale ? 1 : sizeof(V)));
@@ -567,9 +581,10 @@ bool launch_norm(const NormArgs& a, hipStream_t stream) {
   const Shape s = norm_shape(a.dim, E);
 #define NORM_CASE(T, N)                                                                                   \
   if (s.threads == T && s.accesses == N) {                                                                \
-    const long per = block_threads(T) / T;                                                                \
-    hipLaunchKernelGGL((norm_kernel<V, E, T, N, ONCE>), dim3((unsigned)((a.rows + per - 1) / per)),       \
-                       dim3(block_threads(T)), 0, stream, a);                                             \
+    for_row_ranges(a.rows, block_threads(T), block_threads(T) / T, [&](long first, long n, unsigned blocks) { \
+      hipLaunchKernelGGL((norm_kernel<V, E, T, N, ONCE>), dim3(blocks), dim3(block_threads(T)), 0, stream, \
+                         norm_rows<V>(a, first, n));                                                      \
+    });                                                                                                   \
     return true;                                                                                          \
   }
   constexpr int M = E == 1 ? 16 : 4;
@@ -577,7 +592,9 @@ bool launch_norm(const NormArgs& a, hipStream_t stream) {
   NORM_CASE(256, M / 4) NORM_CASE(256, M / 2) NORM_CASE(256, M)
   NORM_CASE(1024, M / 4) NORM_CASE(1024, M / 2) NORM_CASE(1024, M)
 #undef NORM_CASE
-  hipLaunchKernelGGL((norm_long_kernel<V>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
+  for_row_ranges(a.rows, 1024, 1, [&](long first, long n, unsigned blocks) {
+    hipLaunchKernelGGL((norm_long_kernel<V>), dim3(blocks), dim3(1024), 0, stream, norm_rows<V>(a, first, n));
+  });
   return true;
 }
 
