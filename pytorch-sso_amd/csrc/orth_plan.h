@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 #include <vector>
 
 namespace kfac {
@@ -55,6 +56,41 @@ inline long orth_triangle(long t) { return t * (t + 1) / 2; }
 // do.  Larger ones (64 x 256 50 us) are left to those launches, in which they cost nothing beside others.
 constexpr int ORTH_TINY_SIDE = 64, ORTH_TINY_SIZE = 4096;
 constexpr int ORTH_MAX_STEPS = 64;               // of an iteration (their coefficients travel as kernel arguments)
+// A schedule whose operands fit fp16 numbers times 2^13, up to 7.99: with |X| = t in the spectral norm at most
+// `bound` in front of a step, A has t^2, B |a + b t^2 + c t^4| and the next X |a t + b t^3 + c t^5|.  (Two per
+// cent for what the products round.)
+constexpr double ORTH_OPERAND_BOUND = 7.9;
+inline bool orth_schedule_ok(int steps, const float* coeffs) {
+  double bound = 1.;
+  if (steps < 1 || steps > ORTH_MAX_STEPS) return false;
+  for (int k = 0; k < steps; ++k) {
+    const double a = coeffs[3 * k], b = coeffs[3 * k + 1], c = coeffs[3 * k + 2], end = bound * bound;
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+    double value = 0., factor = 0.;
+    // at s = t^2: the ends, and where the derivatives of the two vanish
+    const auto look = [&](double s) {
+      if (!(s >= 0. && s <= end)) return;
+      const double f = std::fabs(a + (b + c * s) * s);
+      factor = std::max(factor, f);
+      value = std::max(value, f * std::sqrt(s));
+    };
+    look(0.);
+    look(end);
+    if (c == 0.) {
+      if (b != 0.) look(-a / (3. * b));
+    } else {
+      look(-b / (2. * c));
+      const double d = 9. * b * b - 20. * a * c;
+      if (d >= 0.)
+        for (double root : {std::sqrt(d), -std::sqrt(d)}) look((-3. * b + root) / (10. * c));
+    }
+    bound = value;
+    // (the caller's coefficients may have been rounded to float32)
+    if (!(1.02 * std::max(bound, std::max(bound * bound, factor)) <= ORTH_OPERAND_BOUND * (1. + 1e-5))) return false;
+  }
+  return true;
+}
+
 inline bool orth_tiny(int rows, int cols) {
   const int R = orth_pad(std::min(rows, cols), 32), C = orth_pad(std::max(rows, cols), 32);
   return R <= ORTH_TINY_SIDE && R * C <= ORTH_TINY_SIZE;

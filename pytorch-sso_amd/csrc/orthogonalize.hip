@@ -936,7 +936,8 @@ bool launch_tiny_type(const Call& c, const std::vector<int>& which, hipStream_t 
 int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (!sizes_ok(c.count, c.rows, c.cols)) return KFAC_ERR_ARG;
   if (c.count == 0) return KFAC_OK;
-  if (!c.in || !c.out || !c.coeffs || c.steps < 1 || c.steps > ORTH_MAX_STEPS || c.late < 0 || c.type < TYPE_F32 || c.type > TYPE_F16)
+  if (!c.in || !c.out || !c.coeffs || !orth_schedule_ok(c.steps, c.coeffs) || c.late < 0 || c.type < TYPE_F32 ||
+      c.type > TYPE_F16)
     return KFAC_ERR_ARG;
   std::vector<int> tiny;
   for (int i = 0; i < c.count; ++i) {
