@@ -501,7 +501,7 @@ int kfac_unpack_batched(int count, float* const* arrays, const int64_t* numel,
 /* ---- Orthogonalised updates ---------------------------------------------- */
 
 /* Newton-Schulz orthogonalisation of a list of matrices (HOST arrays of length `count`):
- *   X = in[i] / (|in[i]| + eps)                       (Frobenius norm)
+ *   X = in[i] / (|in[i]| + eps)                       (Frobenius norm; eps > 0)
  *   `steps` times:  A = X X^T,  X = (a I + b A + c A A) X
  *   out[i] = X
  * rows[i] x cols[i], contiguous row-major, of the element type `type` (0 float32, 1 bfloat16,

@@ -55,6 +55,17 @@ __device__ __forceinline__ double block_sum(double v, double* tmp) {
   return s;
 }
 
+// What normalises and scales an element, in two factors: of numbers close to the ends of float32's range the
+// product of the two lies outside it (a matrix of zeros would be 0 * inf).
+struct OrthNorm {
+  float first, second;
+};
+__device__ __forceinline__ OrthNorm orth_norm(double squares, float eps) {
+  const double v = (double)ORTH_SCALE / (sqrt(squares) + (double)eps);
+  const double first = v > 0x1p100 ? 0x1p100 : v < 0x1p-100 ? 0x1p-60 : 1.;
+  return OrthNorm{(float)first, (float)(v / first)};
+}
+
 // First pass: momentum, and the sum of squares in 64 bits (the squares of float32 numbers neither
 // overflow nor vanish there).  Bound by memory: 58.6 million float32 elements in 54 us, 4.3 TB/s; 177
 // million bfloat16 ones with their momentum, in three launches, 293 us, 6.0 TB/s of the 10 bytes each (part
@@ -144,7 +155,7 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
   double s = 0.;
   for (int i = threadIdx.x; i < m.sums; i += 256) s += sums[m.sum0 + i];
   s = block_sum(s, tmp);
-  const float scale = (float)((double)ORTH_SCALE / (sqrt(s) + (double)eps));
+  const OrthNorm norm = orth_norm(s, eps);
   const int across = (g.C + PACK_C - 1) / PACK_C, local = blockIdx.x - m.pack0;
   const int r0 = local / across * PACK_R, c0 = local % across * PACK_C;
   const int R = g.R, C = g.C;
@@ -155,7 +166,7 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
       const float b = m.buf[i];
       u = mom.nesterov ? fmaf(mom.mu, b, u) : b;
     }
-    return u * scale;
+    return u * norm.first * norm.second;
   };
   // 8 of them that lie side by side
   const auto run = [&](long at, float (&v)[8]) {
@@ -169,7 +180,7 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
     for (int e = 0; e < 8; ++e) {
       float u = Element<V>::get(p.v[e]);
       if (MUON) u = mom.nesterov ? fmaf(mom.mu, b[e], u) : b[e];
-      v[e] = u * scale;
+      v[e] = u * norm.first * norm.second;
     }
   };
   const bool tall = m.rows > m.cols;
@@ -701,7 +712,7 @@ __global__ __launch_bounds__(TINY_THREADS) void orth_tiny_kernel(const TinyArgs<
   // and reads the momentum that it wrote
   constexpr int K = 4;
   double s = 0.;
-  float scale = 0.f;
+  OrthNorm norm{0.f, 0.f};
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     for (int i0 = threadIdx.x; i0 < numel; i0 += K * TINY_THREADS) {
@@ -728,7 +739,7 @@ __global__ __launch_bounds__(TINY_THREADS) void orth_tiny_kernel(const TinyArgs<
         } else {
           const int p = i / cols, q = i - p * cols;
           lds_half* const to = (lds_half*)x + (tall ? q * px + p : p * px + q);
-          const float v = u[e] * scale;
+          const float v = u[e] * norm.first * norm.second;
           const half_t h = (half_t)v;
           *to = h;
           to[xs / 2] = (half_t)(v - (float)h);
@@ -743,7 +754,7 @@ __global__ __launch_bounds__(TINY_THREADS) void orth_tiny_kernel(const TinyArgs<
     if (pass == 0) {
       s = 0.;
       for (int w = 0; w < TINY_WAVES; ++w) s += sums[w];
-      scale = (float)((double)ORTH_SCALE / (sqrt(s) + (double)a.eps));
+      norm = orth_norm(s, a.eps);
     }
   }
   constexpr float INV = 1.f / ORTH_SCALE;
@@ -937,7 +948,7 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
   if (!sizes_ok(c.count, c.rows, c.cols)) return KFAC_ERR_ARG;
   if (c.count == 0) return KFAC_OK;
   if (!c.in || !c.out || !c.coeffs || !orth_schedule_ok(c.steps, c.coeffs) || c.late < 0 || c.type < TYPE_F32 ||
-      c.type > TYPE_F16)
+      c.type > TYPE_F16 || !(c.eps > 0.f && c.eps < INFINITY))
     return KFAC_ERR_ARG;
   std::vector<int> tiny;
   for (int i = 0; i < c.count; ++i) {

@@ -15,7 +15,7 @@ import torch
 from torch.optim import Optimizer
 
 from torchsso import _ops
-from torchsso.utils.linalg import NEWTON_SCHULZ, newton_schulz_schedule
+from torchsso.utils.linalg import NEWTON_SCHULZ, check_orthogonalize_eps, newton_schulz_schedule
 
 
 def _check(lr, momentum, weight_decay, eps):
@@ -25,8 +25,7 @@ def _check(lr, momentum, weight_decay, eps):
         raise ValueError('Invalid momentum: {}'.format(momentum))
     if not weight_decay >= 0:
         raise ValueError('Invalid weight_decay value: {}'.format(weight_decay))
-    if not eps > 0:
-        raise ValueError('Invalid eps: {}'.format(eps))
+    check_orthogonalize_eps(eps)
 
 
 def _matrix(t):

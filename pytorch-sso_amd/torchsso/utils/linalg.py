@@ -80,6 +80,12 @@ def newton_schulz_schedule(steps, coefficients):
     return _flat_schedule(steps, key)
 
 
+def check_orthogonalize_eps(eps):
+    # (the kernels take it in float32, where it must not become zero or infinite)
+    if not 2. ** -149 <= eps < 2. ** 128:
+        raise ValueError('Invalid eps: {}'.format(eps))
+
+
 def orthogonalize(mats, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """Newton-Schulz iterates towards the orthogonal factor U V^T of each matrix G = U S V^T:
     X = G / (|G| + eps), then `steps` times X = a X + (b A + c A A) X with A = X X^T.
@@ -92,8 +98,7 @@ def orthogonalize(mats, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     matrix the last steps run in one part, as many as leave at most 1.5 times the error that rounding the
     result makes (of the default steps one)."""
     schedule = newton_schulz_schedule(steps, coefficients)
-    if not eps > 0:
-        raise ValueError('Invalid eps: {}'.format(eps))
+    check_orthogonalize_eps(eps)
     single = isinstance(mats, torch.Tensor)
     sources = [m.detach().contiguous() for m in ([mats] if single else mats)]
     results = [torch.empty_like(m) for m in sources]
