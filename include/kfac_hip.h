@@ -508,7 +508,8 @@ int kfac_unpack_batched(int count, float* const* arrays, const int64_t* numel,
  * 2 float16), inputs and results alike; a matrix with more rows than columns is iterated on
  * transposed; a matrix without elements is skipped.  in[i] == out[i] is allowed.  coefficients:
  * HOST array of `steps` triples (a, b, c), at most 64.  A product's operands X, A and B = a I + b A + c A A
- * are kept as fp16 numbers in two parts (22 bits; absolute error 2^-38) times 2^13, so that each has to stay
+ * are kept as fp16 numbers in two parts (22 bits; absolute error 2^-38) times 2^13 (and times a power of two that lifts
+ * a norm |X| below 1/2, for as long as the steps leave it there), so that each has to stay
  * below 8: over all t up to |X| in the spectral norm (1 at the start), |a + b t^2 + c t^4|, the next |X| =
  * |a t + b t^3 + c t^5| and its square have to be at most 7.9 / 1.02 (|X| below 2.8), or KFAC_ERR_ARG.
  * late_steps: in as many steps at the end they are kept in one part (11 bits).  The update that a

@@ -58,9 +58,9 @@ constexpr int ORTH_TINY_SIDE = 64, ORTH_TINY_SIZE = 4096;
 constexpr int ORTH_MAX_STEPS = 64;               // of an iteration (their coefficients travel as kernel arguments)
 // A schedule whose operands fit fp16 numbers times 2^13, up to 7.99: with |X| = t in the spectral norm at most
 // `bound` in front of a step, A has t^2, B |a + b t^2 + c t^4| and the next X |a t + b t^3 + c t^5|.  (Two per
-// cent for what the products round.)
+// cent for what the products round.)  growth: so many bits at most X gains in each step.
 constexpr double ORTH_OPERAND_BOUND = 7.9;
-inline bool orth_schedule_ok(int steps, const float* coeffs) {
+inline bool orth_schedule_ok(int steps, const float* coeffs, int* growth = nullptr) {
   double bound = 1.;
   if (steps < 1 || steps > ORTH_MAX_STEPS) return false;
   for (int k = 0; k < steps; ++k) {
@@ -87,6 +87,7 @@ inline bool orth_schedule_ok(int steps, const float* coeffs) {
     bound = value;
     // (the caller's coefficients may have been rounded to float32)
     if (!(1.02 * std::max(bound, std::max(bound * bound, factor)) <= ORTH_OPERAND_BOUND * (1. + 1e-5))) return false;
+    if (growth) growth[k] = std::max(0, (int)std::ceil(std::log2(std::max(1.02 * factor, 0.5))));
   }
   return true;
 }

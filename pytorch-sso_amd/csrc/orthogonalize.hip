@@ -2,6 +2,10 @@
 //
 //   X = G / (|G| + eps);   every step:  A = X X^T,  B = a I + b A + c A A,  X = B X
 //
+// A matrix whose norm is small beside eps would leave the lower end of what its operands hold (2^-38): it is
+// iterated on as X 2^lift, with b 2^-2lift and c 2^-4lift, and in every step that X may gain g bits the lift
+// falls by g, until it is 0.
+//
 // G: the matrix itself, or the direction that momentum makes of a gradient.  A pass over the inputs
 // renews the momentum and sums the squares, a second one normalises and writes the operands; then
 // three launches a step, each over the tiles of all matrices.  The last one writes the result in
@@ -59,11 +63,14 @@ __device__ __forceinline__ double block_sum(double v, double* tmp) {
 // product of the two lies outside it (a matrix of zeros would be 0 * inf).
 struct OrthNorm {
   float first, second;
+  int lift;              // |X| 2^lift is at least 1/2, or lift 0
 };
 __device__ __forceinline__ OrthNorm orth_norm(double squares, float eps) {
-  const double v = (double)ORTH_SCALE / (sqrt(squares) + (double)eps);
+  const double norm = sqrt(squares), all = norm + (double)eps, share = norm / all;
+  const int lift = share > 0. && share < 0.5 ? -ilogb(share) - 1 : 0;
+  const double v = ldexp((double)ORTH_SCALE / all, lift);
   const double first = v > 0x1p100 ? 0x1p100 : v < 0x1p-100 ? 0x1p-60 : 1.;
-  return OrthNorm{(float)first, (float)(v / first)};
+  return OrthNorm{(float)first, (float)(v / first), lift};
 }
 
 // First pass: momentum, and the sum of squares in 64 bits (the squares of float32 numbers neither
@@ -142,7 +149,8 @@ struct OrthGroups {
 // through LDS, read in runs of 8 where its rows allow that (element by element the second figure is 527 us).
 template <class V, bool MUON>
 __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int n, Momentum mom, const double* sums,
-                                                        float eps, half_t* base, OrthGroups groups, int low) {
+                                                        float eps, half_t* base, int* lifts, OrthGroups groups,
+                                                        int low) {
   __shared__ double tmp[4];
   __shared__ float tile[PACK_R][PACK_C + 1];
   int j = 0, end = n;
@@ -157,6 +165,7 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(const OrthMat* mats, int
   s = block_sum(s, tmp);
   const OrthNorm norm = orth_norm(s, eps);
   const int across = (g.C + PACK_C - 1) / PACK_C, local = blockIdx.x - m.pack0;
+  if (local == 0 && threadIdx.x == 0) lifts[j] = norm.lift;
   const int r0 = local / across * PACK_R, c0 = local % across * PACK_C;
   const int R = g.R, C = g.C;
   const V* const in = (const V*)m.in;
@@ -253,7 +262,9 @@ struct OrthProduct {
   half_t* base;
   float* partial;        // sums of the pieces, a tile each
   const OrthMat* mats;
+  const int* lifts;
   float ca, cb, cc;      // of this step
+  int fallen, growth;    // the lifts have fallen by so much before this step, and fall by this behind it
   int from;              // which X is read (the other one is written)
   int low;               // APPLY: the next step reads X in two parts
   int type, update;      // LAST: type of the result; parameters are updated with it
@@ -316,11 +327,23 @@ __device__ __forceinline__ void orth_place(const OrthGroup& g, int tile, int t, 
   }
 }
 
+// The coefficients of matrices that are lifted, and the factor of BX: to the next step's lift, or to none.
+struct OrthFactors {
+  float b, c, x;
+};
+template <int MODE>
+__device__ __forceinline__ OrthFactors orth_factors(const OrthProduct& p, int lift) {
+  constexpr float INV = 1.f / ORTH_SCALE;
+  const int now = max(0, lift - p.fallen), next = MODE == LAST ? 0 : max(0, now - p.growth);
+  return OrthFactors{ldexpf(p.cb, -2 * now), ldexpf(p.cc, -4 * now), ldexpf(MODE == LAST ? INV * INV : INV, next - now)};
+}
+
 // What a product's sums become: B = aI + bA + cAA, or they are it.  Elements D[m ... m + 3][n].
 template <int MODE, bool SPLIT>
-__device__ __forceinline__ f4 orth_value(const OrthProduct& p, const OrthGroup& g, int k, int m, int n, f4 v) {
+__device__ __forceinline__ f4 orth_value(const OrthProduct& p, const OrthFactors& f, const OrthGroup& g, int k, int m, int n,
+                                         f4 v) {
   constexpr float INV = 1.f / ORTH_SCALE;
-  if (MODE == LAST) return v * (INV * INV);
+  if (MODE == APPLY || MODE == LAST) return v * f.x;
   v *= INV;
   if (MODE == POLY) {
     const half_t* const from = p.base + g.a + (long)k * 2 * g.R * g.R + orth_at(n, m, g.R, SPLIT);
@@ -329,7 +352,7 @@ __device__ __forceinline__ f4 orth_value(const OrthProduct& p, const OrthGroup& 
     if (SPLIT) al = *(const h4*)(from + 32);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      v[e] = fmaf(p.cc, v[e], p.cb * ((float)ah[e] + (float)al[e]));
+      v[e] = fmaf(f.c, v[e], f.b * ((float)ah[e] + (float)al[e]));
       if (m + e == n) v[e] += p.ca * ORTH_SCALE;
     }
   }
@@ -351,8 +374,8 @@ __device__ __forceinline__ half_t* orth_target(const OrthProduct& p, const OrthG
 // leave it as whole rows of the wave's part.  Without that a product of 16 matrices of 1024^2 spends 40 of
 // 113 us on writing.
 template <class TILE, bool SPLIT, int MODE>
-__device__ __forceinline__ void orth_write(const OrthProduct& p, const OrthGroup& g, const OrthMat& mat, int k, int m0,
-                                           int n0, bool mirror, f4 (&acc)[TILE::FM][TILE::FN], lds_char* lds, int lane) {
+__device__ __forceinline__ void orth_write(const OrthProduct& p, const OrthFactors& factors, const OrthGroup& g,
+                                           const OrthMat& mat, int k, int m0, int n0, bool mirror, f4 (&acc)[TILE::FM][TILE::FN], lds_char* lds, int lane) {
   constexpr int FM = TILE::FM, FN = TILE::FN;
   typedef __attribute__((address_space(3))) half_t lds_half;
   typedef __attribute__((address_space(3))) h4 lds_h4;
@@ -397,7 +420,7 @@ __device__ __forceinline__ void orth_write(const OrthProduct& p, const OrthGroup
     const int nl = lane & 15, ml = 4 * (lane >> 4);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      acc[i][j] = orth_value<MODE, SPLIT>(p, g, k, m0 + 16 * i + ml, n0 + 16 * j + nl, acc[i][j]);
+      acc[i][j] = orth_value<MODE, SPLIT>(p, factors, g, k, m0 + 16 * i + ml, n0 + 16 * j + nl, acc[i][j]);
       if (tall) continue;
       lds_char* const row = lds + nl * TILE::M_PITCH;
       const int c = 16 * i + ml;
@@ -479,6 +502,7 @@ __device__ __forceinline__ void orth_item(const OrthProduct& p, const OrthGroup&
     steps = min(s.len, steps - from);
   }
   steps *= UNIT;
+  const int lift = MODE == GRAM ? 0 : p.lifts[g.first + k];
   f4 acc[FM][FN];
   if constexpr (TILE::PAIR) orth_pair_product<TILE, SPLIT>(P, Q, steps, lds, wave, acc);
   else orth_product<TILE, SPLIT>(P, Q, steps, lds, wave, team, acc);
@@ -493,7 +517,8 @@ __device__ __forceinline__ void orth_item(const OrthProduct& p, const OrthGroup&
   }
   OrthMat mat;
   if (MODE == LAST) mat = p.mats[g.first + k];
-  orth_write<TILE, SPLIT, MODE>(p, g, mat, k, tm * T + wm * FM * 16, tn * T + wn * FN * 16, SYM && tm != tn, acc,
+  const OrthFactors factors = orth_factors<MODE>(p, lift);
+  orth_write<TILE, SPLIT, MODE>(p, factors, g, mat, k, tm * T + wm * FM * 16, tn * T + wn * FN * 16, SYM && tm != tn, acc,
                                 lds + TILE::SUMS + wave * TILE::WRITE, lane);
 }
 
@@ -561,7 +586,8 @@ __device__ __forceinline__ void orth_fix_item(const OrthProduct& p, int gi, int 
   const int m = tm * T + wm * FM * 16 + 16 * i, n0 = tn * T + wn * FN * 16;
   OrthMat mat;
   if (MODE == LAST) mat = p.mats[g.first + k];
-  orth_write<Rows, SPLIT, MODE>(p, g, mat, k, m, n0, MODE != LAST && MODE != APPLY && tm != tn, sum,
+  const OrthFactors factors = orth_factors<MODE>(p, MODE == GRAM ? 0 : p.lifts[g.first + k]);
+  orth_write<Rows, SPLIT, MODE>(p, factors, g, mat, k, m, n0, MODE != LAST && MODE != APPLY && tm != tn, sum,
                                 lds + wave * Rows::WRITE, lane);
 }
 
@@ -642,12 +668,12 @@ bool launch_step(OrthProduct& p, const OrthBatch& b, const OrthLaunch (&l)[3], c
 
 template <class V, bool MUON>
 void launch_passes(const OrthMat* mats, const OrthBatch& b, Momentum mom, double* sums, int sum_blocks,
-                   int pack_blocks, float eps, half_t* base, bool low, hipStream_t stream) {
+                   int pack_blocks, float eps, half_t* base, int* lifts, bool low, hipStream_t stream) {
   hipLaunchKernelGGL((orth_sum_kernel<V, MUON>), dim3(sum_blocks), dim3(256), 0, stream, mats, b.count, mom, sums);
   OrthGroups groups;
   std::copy(b.groups.begin(), b.groups.end(), groups.g);
   hipLaunchKernelGGL((orth_pack_kernel<V, MUON>), dim3(pack_blocks), dim3(256), 0, stream, mats, b.count, mom,
-                     (const double*)sums, eps, base, groups, (int)low);
+                     (const double*)sums, eps, base, lifts, groups, (int)low);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -658,6 +684,7 @@ template <int N>
 struct TinyArgs {
   OrthMat m[N];
   float coeffs[3 * ORTH_MAX_STEPS];
+  unsigned char growth[ORTH_MAX_STEPS];
   int steps, update;
   Momentum mom;
   float eps;
@@ -712,7 +739,7 @@ __global__ __launch_bounds__(TINY_THREADS) void orth_tiny_kernel(const TinyArgs<
   // and reads the momentum that it wrote
   constexpr int K = 4;
   double s = 0.;
-  OrthNorm norm{0.f, 0.f};
+  OrthNorm norm{0.f, 0.f, 0};
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     for (int i0 = threadIdx.x; i0 < numel; i0 += K * TINY_THREADS) {
@@ -760,8 +787,13 @@ __global__ __launch_bounds__(TINY_THREADS) void orth_tiny_kernel(const TinyArgs<
   constexpr float INV = 1.f / ORTH_SCALE;
   const int nb = (r + 15) / 16, blocks = nb * (nb + 1) / 2, nl = lane & 15, ml = 4 * (lane >> 4);
   const int share = blocks <= TINY_WAVES / 2 ? TINY_WAVES / blocks : 1;      // waves to a block
+  int lift = norm.lift;
   for (int step = 0; step < a.steps; ++step) {
-    const float ca = a.coeffs[3 * step], cb = a.coeffs[3 * step + 1], cc = a.coeffs[3 * step + 2];
+    const float ca = a.coeffs[3 * step], cb = ldexpf(a.coeffs[3 * step + 1], -2 * lift),
+                cc = ldexpf(a.coeffs[3 * step + 2], -4 * lift);
+    const int next = max(0, lift - (int)a.growth[step]);
+    const float to_next = ldexpf(INV, next - lift);
+    lift = next;
     // A = X X^T, then B = aI + bA + cAA: the blocks on and below the diagonal
 #pragma unroll 1
     for (int poly = 0; poly < 2; ++poly) {
@@ -845,7 +877,7 @@ __global__ __launch_bounds__(TINY_THREADS) void orth_tiny_kernel(const TinyArgs<
       for (int n = 0; n < NB; ++n) {
         if (n >= nb) continue;
         h4 h, l;
-        split4(d[n] * INV, h, l);
+        split4(d[n] * to_next, h, l);
         lds_char* const to = x + 2 * ((16 * n + nl) * px + col + ml);
         *(lds_h4*)to = h;
         *(lds_h4*)(to + xs) = l;
@@ -853,27 +885,32 @@ __global__ __launch_bounds__(TINY_THREADS) void orth_tiny_kernel(const TinyArgs<
     }
     __syncthreads();
   }
+  const float to_result = ldexpf(INV, -lift);
 #pragma unroll 2
   for (int i = threadIdx.x; i < numel; i += TINY_THREADS) {
     const int p = i / cols, q = i - p * cols;
     const lds_half* const from = (const lds_half*)x + (tall ? q * px + p : p * px + q);
-    const float o = ((float)from[0] + (float)from[xs / 2]) * INV;
+    const float o = ((float)from[0] + (float)from[xs / 2]) * to_result;
     V* const to = (V*)m.out + i;
     *to = Element<V>::put(a.update ? m.keep * Element<V>::get(*to) - m.step * o : o);
   }
 }
 
 struct Layout {
-  size_t table, sums, partials, operands, bytes;
+  size_t table, sums, lifts, partials, operands, bytes;
 };
 Layout layout(const OrthPlan& plan) {
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  Layout l{0, 0, 0, 0, 256};
+  Layout l{0, 0, 0, 0, 0, 256};
   if (plan.order.empty()) return l;        // small matrices alone
   l.sums = up(plan.order.size() * sizeof(OrthMat));
-  long sums = 0;
-  for (const OrthBatch& b : plan.batches) sums = std::max(sums, (long)b.count * SUM_MAX);
-  l.partials = l.sums + up((size_t)sums * sizeof(double));
+  long sums = 0, count = 0;
+  for (const OrthBatch& b : plan.batches) {
+    sums = std::max(sums, (long)b.count * SUM_MAX);
+    count = std::max(count, (long)b.count);
+  }
+  l.lifts = l.sums + up((size_t)sums * sizeof(double));
+  l.partials = l.lifts + up((size_t)count * sizeof(int));
   l.operands = l.partials + (size_t)ORTH_PARTIAL_BYTES;
   l.bytes = l.operands + (size_t)plan.halves * sizeof(half_t);
   return l;
@@ -899,6 +936,7 @@ struct Call {
   const float* coeffs;
   float eps;
   int late;                          // steps at the end with single products
+  int growth[ORTH_MAX_STEPS];        // bits that X may gain in a step
 };
 
 template <class V, bool MUON, int N>
@@ -920,6 +958,7 @@ bool launch_tiny(const Call& c, const std::vector<int>& which, size_t first, hip
     lds = std::max(lds, tiny_lds(orth_pad(std::min(m.rows, m.cols), 32), orth_pad(std::max(m.rows, m.cols), 32)));
   }
   std::copy(c.coeffs, c.coeffs + 3 * c.steps, a.coeffs);
+  std::copy(c.growth, c.growth + c.steps, a.growth);
   a.steps = c.steps;
   a.update = c.step != nullptr;
   a.mom = c.mom;
@@ -944,10 +983,10 @@ bool launch_tiny_type(const Call& c, const std::vector<int>& which, hipStream_t 
   return c.buf ? launch_tiny_list<V, true>(c, which, stream) : launch_tiny_list<V, false>(c, which, stream);
 }
 
-int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+int run(Call& c, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (!sizes_ok(c.count, c.rows, c.cols)) return KFAC_ERR_ARG;
   if (c.count == 0) return KFAC_OK;
-  if (!c.in || !c.out || !c.coeffs || !orth_schedule_ok(c.steps, c.coeffs) || c.late < 0 || c.type < TYPE_F32 ||
+  if (!c.in || !c.out || !c.coeffs || !orth_schedule_ok(c.steps, c.coeffs, c.growth) || c.late < 0 || c.type < TYPE_F32 ||
       c.type > TYPE_F16 || !(c.eps > 0.f && c.eps < INFINITY))
     return KFAC_ERR_ARG;
   std::vector<int> tiny;
@@ -1003,6 +1042,7 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
   char* const ws = (char*)workspace;
   upload_table(table.data(), table.size() * sizeof(OrthMat), ws + l.table, stream);
   double* const sums = (double*)(ws + l.sums);
+  int* const lifts = (int*)(ws + l.lifts);
   half_t* const base = (half_t*)(ws + l.operands);
   for (size_t bi = 0; bi < plan.batches.size(); ++bi) {
     OrthBatch& b = plan.batches[bi];
@@ -1011,8 +1051,8 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
     const bool low = c.steps > c.late;
     const auto passes = [&](auto* v) {
       using V = std::remove_pointer_t<decltype(v)>;
-      if (c.buf) launch_passes<V, true>(mats, b, c.mom, sums, sum_blocks[bi], pack_blocks[bi], c.eps, base, low, stream);
-      else launch_passes<V, false>(mats, b, c.mom, sums, sum_blocks[bi], pack_blocks[bi], c.eps, base, low, stream);
+      if (c.buf) launch_passes<V, true>(mats, b, c.mom, sums, sum_blocks[bi], pack_blocks[bi], c.eps, base, lifts, low, stream);
+      else launch_passes<V, false>(mats, b, c.mom, sums, sum_blocks[bi], pack_blocks[bi], c.eps, base, lifts, low, stream);
     };
     if (c.type == TYPE_F32) passes((float*)nullptr);
     else if (c.type == TYPE_BF16) passes((__hip_bfloat16*)nullptr);
@@ -1023,12 +1063,15 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stre
     p.base = base;
     p.partial = (float*)(ws + l.partials);
     p.mats = mats;
+    p.lifts = lifts;
     p.type = c.type;
     p.update = c.step != nullptr;
     for (int k = 0; k < c.steps; ++k) {
       const bool split = c.steps - k > c.late, next = c.steps - k - 1 > c.late, last = k + 1 == c.steps;
       p.from = k & 1;
+      p.growth = c.growth[k];
       if (!launch_step(p, b, launches, c.coeffs + 3 * k, split, next, last, stream)) return KFAC_ERR_LAUNCH;
+      p.fallen += p.growth;
     }
   }
   return launch_status();
@@ -1053,7 +1096,7 @@ int kfac_orthogonalize_batched(int count, const int* rows, const int* cols, int 
                                void* workspace, size_t workspace_bytes, void* stream) {
   try {
     kfac::Call c{count, rows, cols, type, in, out, nullptr, nullptr, nullptr, {0.f, 0},
-                 steps, coefficients, eps, late_steps};
+                 steps, coefficients, eps, late_steps, {}};
     return kfac::run(c, workspace, workspace_bytes, (hipStream_t)stream);
   } catch (const std::exception&) {
     return KFAC_ERR_TOO_LARGE;
@@ -1067,7 +1110,7 @@ int kfac_muon_update_batched(int count, const int* rows, const int* cols, int ty
   try {
     if (count > 0 && (!buffers || !step || !keep)) return KFAC_ERR_ARG;
     kfac::Call c{count, rows, cols, type, grads, params, buffers, step, keep, {momentum, nesterov},
-                 steps, coefficients, eps, late_steps};
+                 steps, coefficients, eps, late_steps, {}};
     return kfac::run(c, workspace, workspace_bytes, (hipStream_t)stream);
   } catch (const std::exception&) {
     return KFAC_ERR_TOO_LARGE;

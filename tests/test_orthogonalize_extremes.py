@@ -59,3 +59,58 @@ def test_the_smallest_and_the_largest_numbers(shape, scale, eps):
     assert torch.isfinite(g).all()
     out = torchsso.utils.orthogonalize(g, eps=eps).cpu().double()
     assert (out - want).norm() <= 4.7e-5 * want.norm()
+
+
+def off(got, want):
+    return ((got.detach().cpu().double() - want).norm() / want.norm()).item()
+
+
+# (tolerances: 4.7e-5 as above; of a float16 result 2^-11, of a bfloat16 one 1.5 times 2^-8, the largest rounding of an element)
+SMALL = {torch.float32: 4.7e-5, torch.float16: 2. ** -11 + 4.7e-5, torch.bfloat16: 1.5 * 2. ** -8}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype,scale,eps', [(torch.float32, s, e) for s, e in (
+    (1e-8, 1e-7), (1e-10, 1e-7), (1e-13, 1e-7), (1e-16, 1e-7), (1e-20, 1e-7), (1e-30, 1e-7), (1e-36, 1e-2), (1., 1e12),
+    (1e-3, 1e20))] + [(torch.bfloat16, 1e-20, 1e-7), (torch.bfloat16, 1e-12, 1e-7), (torch.float16, 1., 1e3), (torch.float16, 1e-1, 1e3)])
+@pytest.mark.parametrize('shape', SHAPES)
+def test_norms_that_are_small_beside_eps(shape, dtype, scale, eps):
+    """The iterate is then small throughout, and as exact as any other."""
+    g = (torch.randn(shape, generator=torch.Generator().manual_seed(0)) * scale).to(dtype).cuda()
+    want = reference(g, eps)
+    assert off(torchsso.utils.orthogonalize(g, eps=eps), want) <= SMALL[dtype]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('scale', [1e-4, 1e-12, 1e-24])
+@pytest.mark.parametrize('schedule', [((7.7, -14., 7.),), ((0.5, 0., 0.),) * 3, ((1.5, -0.5, 0.),) * 8,
+                                      ((3.4, -4.7, 2.0), (2.0, -1.5, 0.5), (1.875, -1.25, 0.375))])
+def test_other_coefficients_on_small_norms(schedule, scale):
+    for shape in SHAPES:
+        g = (torch.randn(shape, generator=torch.Generator().manual_seed(1)) * scale).cuda()
+        x = g.cpu().double()
+        x = x / (x.norm() + 1e-7)
+        for a, b, c in schedule:
+            m = x @ x.t()
+            x = a * x + (b * m + c * m @ m) @ x
+        assert off(torchsso.utils.orthogonalize(g, len(schedule), schedule), x) <= 4.7e-5
+
+
+@pytest.mark.gpu
+def test_small_and_ordinary_matrices_in_one_list():
+    """Every matrix has a scale of its own, in launches that reduce in pieces too."""
+    shapes = [(300, 900), (900, 300), (64, 3000), (300, 900), (16, 20), (16, 20), (1100, 1300)]
+    scales = [1., 1e-12, 1e-20, 1e-7, 1e-15, 1., 1e-18]
+    mats = [(torch.randn(s, generator=torch.Generator().manual_seed(i)) * k).cuda()
+            for i, (s, k) in enumerate(zip(shapes, scales))]
+    for m, o in zip(mats, torchsso.utils.orthogonalize(mats)):
+        assert off(o, reference(m, 1e-7)) <= 4.7e-5
+
+
+@pytest.mark.gpu
+def test_muon_of_small_gradients():
+    shape = (70, 200)
+    g = torch.randn(shape, generator=torch.Generator().manual_seed(0)) * 1e-18
+    p, buf = torch.zeros(shape, device='cuda'), torch.zeros(shape, device='cuda')
+    torchsso.optim.muon([p], [g.cuda()], [buf], lr=1., momentum=0.5, nesterov=False)
+    assert off(p, -reference(g, 1e-7)) <= 4.7e-5
