@@ -504,7 +504,7 @@ int kfac_unpack_batched(int count, float* const* arrays, const int64_t* numel,
  *   X = in[i] / (|in[i]| + eps)                       (Frobenius norm; eps > 0)
  *   `steps` times:  A = X X^T,  X = (a I + b A + c A A) X
  *   out[i] = X
- * rows[i] x cols[i], contiguous row-major, of the element type `type` (0 float32, 1 bfloat16,
+ * rows[i] x cols[i], at most 16384 each, contiguous row-major, of the element type `type` (0 float32, 1 bfloat16,
  * 2 float16), inputs and results alike; a matrix with more rows than columns is iterated on
  * transposed; a matrix without elements is skipped.  in[i] == out[i] is allowed.  coefficients:
  * HOST array of `steps` triples (a, b, c), at most 64.  A product's operands X, A and B = a I + b A + c A A

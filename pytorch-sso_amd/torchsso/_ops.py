@@ -791,10 +791,16 @@ def _addresses(tensors, like, what, dtype=None):
         *[_hip.typed_ptr(t, dtype, like.device, '%s %d' % (what, i)) for i, t in enumerate(tensors)])
 
 
+ORTH_MAX_SIDE = 16384        # rows and columns of a matrix that the kernels orthogonalise
+
+
 def _matrix_dims(mats, what):
     for i, m in enumerate(mats):
         if m.dim() != 2:
             raise _hip.KfacHipError('%s %d is not a matrix: %s' % (what, i, tuple(m.shape)))
+        if max(m.shape) > ORTH_MAX_SIDE:
+            raise _hip.KfacHipError('%s %d is %d x %d: orthogonalisation takes sides of up to %d'
+                                    % (what, i, m.shape[0], m.shape[1], ORTH_MAX_SIDE))
     return _hip.ints([m.shape[0] for m in mats]), _hip.ints([m.shape[1] for m in mats])
 
 

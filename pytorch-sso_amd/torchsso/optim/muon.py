@@ -38,8 +38,8 @@ def muon(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_decay=
          coefficients=NEWTON_SCHULZ, eps=1e-7):
     """One update of a list of parameters, in place, with all matrices in the same launches.
 
-    params, grads: tensors of two dimensions or more (of more, all but the first are columns) of
-    one type, float32, bfloat16 or float16, the parameters contiguous; buffers: contiguous float32
+    params, grads: tensors of two dimensions or more (of more, all but the first are columns), with
+    at most 16384 rows and columns, of one type, float32, bfloat16 or float16, the parameters contiguous; buffers: contiguous float32
     tensors of the same shapes, zero before the first update."""
     _check(lr, momentum, weight_decay, eps)
     schedule = newton_schulz_schedule(steps, coefficients)
@@ -67,7 +67,7 @@ def muon(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_decay=
 
 class Muon(Optimizer):
     r"""Optimizer for the matrices of a model (see `muon`): the weights of Linear and Conv2d layers,
-    in float32, bfloat16 or float16.  Gains, biases and embeddings take another optimizer.
+    in float32, bfloat16 or float16, with at most 16384 rows and columns.  Gains, biases and embeddings take another optimizer.
 
     Args:
         params: parameters of two dimensions or more, or param groups
@@ -87,6 +87,9 @@ class Muon(Optimizer):
                 if p.dim() < 2:
                     raise ValueError('Muon updates matrices, got a parameter of shape {}'
                                      .format(tuple(p.shape)))
+                if max(p.shape[0], math.prod(p.shape[1:])) > _ops.ORTH_MAX_SIDE:
+                    raise ValueError('Muon updates matrices with sides of up to {}, got a parameter of shape {}'
+                                     .format(_ops.ORTH_MAX_SIDE, tuple(p.shape)))
 
     def load_state_dict(self, state_dict):
         super(Muon, self).load_state_dict(state_dict)

@@ -91,7 +91,8 @@ def orthogonalize(mats, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     X = G / (|G| + eps), then `steps` times X = a X + (b A + c A A) X with A = X X^T.
 
     `mats`: a tensor of two dimensions, or of more for a stack of matrices (its last two), or a
-    list of such tensors, in float32, bfloat16 or float16 (one type a list).  Returns new
+    list of such tensors, in float32, bfloat16 or float16 (one type a list), with sides of up to
+    16384.  Returns new
     tensors of the same shapes and type.  `coefficients`: (a, b, c), or one triple per step.
 
     Products run on the fp16 matrix cores in two parts a number (as good as float32).  Of a bfloat16
