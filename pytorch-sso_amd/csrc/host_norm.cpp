@@ -191,6 +191,8 @@ PyObject* host_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!norm_entry || args[0] == Py_None || !tensor_of(args[0], x) || !tensor_of(args[1], residual) ||
         !tensor_of(args[2], gain) || !tensor_of(args[4], curvature) || !takes(x, residual, gain, curvature))
       Py_RETURN_NONE;
+    for (const Tensor& t : {x, residual, gain})
+      TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "rms_norm has no forward-mode derivative");
     const auto needs = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
     if (!eight && at::GradMode::is_enabled() && (needs(x) || needs(residual) || needs(gain))) {
       const auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };

@@ -1,0 +1,31 @@
+"""What autograd asks of torchsso.nn.rms_norm beside its gradients."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import torchsso
+
+pytestmark = pytest.mark.gpu
+
+EIGHT = torch.float8_e4m3fn
+
+
+@pytest.mark.parametrize('requires_grad', [False, True])
+@pytest.mark.parametrize('which', [0, 1, 2])
+def test_forward_mode_is_refused(which, requires_grad):
+    """(There is no such derivative; a result without a tangent would stand for one of zero.)"""
+    x, residual, gain = torch.randn(4, 50, device='cuda'), torch.randn(4, 50, device='cuda'), torch.ones(50, device='cuda')
+    with forward_ad.dual_level():
+        args = [x, residual, gain]
+        args[which] = forward_ad.make_dual(args[which].requires_grad_(requires_grad), torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError):
+            torchsso.nn.add_rms_norm(*args)
+        if which != 1:
+            with pytest.raises(RuntimeError):
+                torchsso.nn.rms_norm(args[0], args[2])
+        if not requires_grad:
+            with pytest.raises(RuntimeError):
+                torchsso.nn.add_rms_norm(*args, out_dtype=EIGHT)
+        # without a tangent, inside such a level, it works
+        y = torchsso.nn.rms_norm(torch.ones(4, 50, device='cuda'))
+        assert forward_ad.unpack_dual(y).tangent is None
