@@ -9,6 +9,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros_like.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -64,6 +65,7 @@ struct Normed {
   Tensor y, h, scale;
 };
 Normed norm(const Tensor& x, const Tensor& residual, const Tensor& gain, double eps, bool eight) {
+  const c10::DeviceGuard guard(x.device());      // (the handle of a null stream means that of the current device)
   const int64_t dim = x.size(-1);
   const Tensor rows = rows_of(x, dim), res = residual.defined() ? rows_of(residual, dim) : Tensor();
   Normed n;

@@ -6,6 +6,7 @@ for device memory (tensors, the caching allocator for scratch) and for the
 current stream handle.
 """
 import atexit
+import contextlib
 import ctypes
 import os
 import threading
@@ -268,6 +269,13 @@ def stream_ptr(device=None, stream=None):
     if index is None:
         return torch.cuda.current_stream(device).cuda_stream
     return torch._C._cuda_getCurrentRawStream(index)     # (no Stream object around the handle)
+
+
+def on_device(device):
+    """Context in which `device` is current (the handle of a null stream means that of the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def order_streams(index, waiting, waited):

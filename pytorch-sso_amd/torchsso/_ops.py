@@ -850,10 +850,12 @@ def orthogonalize_batched(mats, outs, coefficients, eps):
         if m.shape != o.shape:
             raise _hip.KfacHipError('result %d has shape %s, expected %s' % (i, tuple(o.shape), tuple(m.shape)))
     ins, results = _addresses(mats, first, 'matrix'), _addresses(outs, first, 'result')
-    ws, ws_bytes = _hip.workspace(first.device, lib.kfac_orthogonalize_workspace_bytes(len(mats), rows, cols))
-    st = lib.kfac_orthogonalize_batched(
-        len(mats), rows, cols, kind, ins, results, len(coefficients) // 3, _hip.floats(coefficients),
-        float(eps), late_steps(first.dtype, tuple(coefficients)), _ws_ptr(ws), ws_bytes, _hip.stream_ptr(first.device))
+    with _hip.on_device(first.device):
+        ws, ws_bytes = _hip.workspace(first.device, lib.kfac_orthogonalize_workspace_bytes(len(mats), rows, cols))
+        st = lib.kfac_orthogonalize_batched(
+            len(mats), rows, cols, kind, ins, results, len(coefficients) // 3, _hip.floats(coefficients),
+            float(eps), late_steps(first.dtype, tuple(coefficients)), _ws_ptr(ws), ws_bytes,
+            _hip.stream_ptr(first.device))
     _hip.check(st, 'kfac_orthogonalize_batched')
 
 
@@ -875,11 +877,13 @@ def muon_update_batched(params, grads, buffers, step_sizes, keeps, momentum, nes
     written = [t.data_ptr() for t in list(params) + list(buffers) if t.numel() > 0]
     if len(set(written)) != len(written):
         raise _hip.KfacHipError('a parameter or momentum buffer is in the list twice')
-    ws, ws_bytes = _hip.workspace(first.device, lib.kfac_orthogonalize_workspace_bytes(len(params), rows, cols))
-    st = lib.kfac_muon_update_batched(
-        len(params), rows, cols, kind, ps, gs, bs, _hip.floats(step_sizes), _hip.floats(keeps),
-        float(momentum), int(bool(nesterov)), len(coefficients) // 3, _hip.floats(coefficients),
-        float(eps), late_steps(first.dtype, tuple(coefficients)), _ws_ptr(ws), ws_bytes, _hip.stream_ptr(first.device))
+    with _hip.on_device(first.device):
+        ws, ws_bytes = _hip.workspace(first.device, lib.kfac_orthogonalize_workspace_bytes(len(params), rows, cols))
+        st = lib.kfac_muon_update_batched(
+            len(params), rows, cols, kind, ps, gs, bs, _hip.floats(step_sizes), _hip.floats(keeps),
+            float(momentum), int(bool(nesterov)), len(coefficients) // 3, _hip.floats(coefficients),
+            float(eps), late_steps(first.dtype, tuple(coefficients)), _ws_ptr(ws), ws_bytes,
+            _hip.stream_ptr(first.device))
     _hip.check(st, 'kfac_muon_update_batched')
 
 
@@ -988,12 +992,13 @@ def rms_norm_backward(dy, dh, h, gain, eps, samples, want_dx=True, want_dgain=Tr
         dh, lddh = _rows(dh, dim)
         args[2:] = [_row_ptr(dh, h, 'stream gradient'), lddh]
     ws, ws_bytes = None, 0
-    if dgain is not None or curvature is not None:
-        ws, ws_bytes = _hip.workspace(h.device, lib.kfac_rms_norm_backward_workspace_bytes(
-            kind, rows, dim, samples, int(curvature is not None)))
-    st = lib.kfac_rms_norm_backward(
-        kind, is_float, rows, dim, samples, *args, _row_ptr(stream_rows, h, 'stream'), ldh, gain_ptr, float(eps),
-        None if dx is None else dx.data_ptr(), None if dgain is None else dgain.data_ptr(), c_ptr,
-        _ws_ptr(ws), ws_bytes, _hip.stream_ptr(h.device))
+    with _hip.on_device(h.device):
+        if dgain is not None or curvature is not None:
+            ws, ws_bytes = _hip.workspace(h.device, lib.kfac_rms_norm_backward_workspace_bytes(
+                kind, rows, dim, samples, int(curvature is not None)))
+        st = lib.kfac_rms_norm_backward(
+            kind, is_float, rows, dim, samples, *args, _row_ptr(stream_rows, h, 'stream'), ldh, gain_ptr, float(eps),
+            None if dx is None else dx.data_ptr(), None if dgain is None else dgain.data_ptr(), c_ptr,
+            _ws_ptr(ws), ws_bytes, _hip.stream_ptr(h.device))
     _hip.check(st, 'kfac_rms_norm_backward')
     return dx, dgain
