@@ -11,6 +11,7 @@
 #include <ATen/ops/zeros_like.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -205,8 +206,8 @@ PyObject* host_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (n.scale.defined()) out.push_back(n.scale);
     if (n.h.defined()) out.push_back(n.h);
     return tuple_of(out);
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    torch::translate_exception_to_python(std::current_exception());      // (each as torch's own calls raise it)
     return nullptr;
   }
 }

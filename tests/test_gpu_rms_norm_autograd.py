@@ -29,3 +29,17 @@ def test_forward_mode_is_refused(which, requires_grad):
         # without a tangent, inside such a level, it works
         y = torchsso.nn.rms_norm(torch.ones(4, 50, device='cuda'))
         assert forward_ad.unpack_dual(y).tangent is None
+
+
+@pytest.mark.parametrize('requires_grad', [False, True])
+def test_running_out_of_memory_is_raised_as_torch_does(requires_grad):
+    x = torch.ones(1, 1 << 17, device='cuda', dtype=torch.bfloat16, requires_grad=requires_grad)
+    # (16 GiB asked of an allocator that may hand out 2 % of the memory: nothing is allocated)
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.02)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            torchsso.nn.rms_norm(x.expand(1 << 16, 1 << 17))
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.)
+    assert torchsso.nn.rms_norm(x).shape == x.shape
