@@ -144,6 +144,13 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
   }
 };
 
+// Other threads go on meanwhile: an allocation may free cached blocks, a launch wait for room in the stream's
+// queue.
+struct WithoutInterpreter {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~WithoutInterpreter() { PyEval_RestoreThread(state); }
+};
+
 bool tensor_of(PyObject* o, Tensor& t) {
   if (o == Py_None) return true;
   if (!THPVariable_Check(o)) return false;
@@ -197,14 +204,19 @@ PyObject* host_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     for (const Tensor& t : {x, residual, gain})
       TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "rms_norm has no forward-mode derivative");
     const auto needs = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
-    if (!eight && at::GradMode::is_enabled() && (needs(x) || needs(residual) || needs(gain))) {
-      const auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-      return tuple_of(RmsNorm::apply(x, maybe(residual), maybe(gain), eps, maybe(curvature)));
+    variable_list out;
+    {
+      const WithoutInterpreter released;
+      if (!eight && at::GradMode::is_enabled() && (needs(x) || needs(residual) || needs(gain))) {
+        const auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+        out = RmsNorm::apply(x, maybe(residual), maybe(gain), eps, maybe(curvature));
+      } else {
+        const Normed n = norm(x, residual, gain, eps, eight);
+        out = {n.y};
+        if (n.scale.defined()) out.push_back(n.scale);
+        if (n.h.defined()) out.push_back(n.h);
+      }
     }
-    const Normed n = norm(x, residual, gain, eps, eight);
-    variable_list out{n.y};
-    if (n.scale.defined()) out.push_back(n.scale);
-    if (n.h.defined()) out.push_back(n.h);
     return tuple_of(out);
   } catch (...) {
     torch::translate_exception_to_python(std::current_exception());      // (each as torch's own calls raise it)

@@ -1,9 +1,12 @@
 """What autograd asks of torchsso.nn.rms_norm beside its gradients."""
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import torchsso
+from torchsso import _hip
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +46,21 @@ def test_running_out_of_memory_is_raised_as_torch_does(requires_grad):
     finally:
         torch.cuda.set_per_process_memory_fraction(1.)
     assert torchsso.nn.rms_norm(x).shape == x.shape
+
+
+@pytest.mark.parametrize('how', ['gradient', 'none', 'eight bits'])
+def test_other_threads_run_during_a_norm(how):
+    """The interpreter is released around the engine's entry point: in its place stands a function that returns
+    whether this thread holds the interpreter, which the norm takes for a status (0: success)."""
+    lib = _hip.load()
+    address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+    entries = [address(f) for f in (lib.kfac_rms_norm, lib.kfac_rms_norm_backward_workspace_bytes, lib.kfac_rms_norm_backward)]
+    x = torch.ones(4, 50, device='cuda', requires_grad=how == 'gradient')
+    more = dict(out_dtype=EIGHT) if how == 'eight bits' else {}
+    torchsso.nn.rms_norm(x, **more)
+    _hip._host.bind_norm(address(ctypes.pythonapi.PyGILState_Check), *entries[1:])
+    try:
+        torchsso.nn.rms_norm(x, **more)
+    finally:
+        _hip._host.bind_norm(*entries)
+    assert torch.equal(torchsso.nn.rms_norm(torch.ones(4, 50, device='cuda')), torchsso.nn.rms_norm(x.detach()))
