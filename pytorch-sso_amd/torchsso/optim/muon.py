@@ -46,7 +46,7 @@ def muon(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_decay=
     if not len(params) == len(grads) == len(buffers):
         raise ValueError('%d parameters, %d gradients, %d buffers'
                          % (len(params), len(grads), len(buffers)))
-    ps, gs, bs, sizes, keeps = [], [], [], [], []
+    ps, gs, bs, sizes, keeps, written = [], [], [], [], [], []
     for p, g, b in zip(params, grads, buffers):
         if p.dim() < 2:
             raise ValueError('Muon updates matrices, got a parameter of shape {}'.format(tuple(p.shape)))
@@ -56,6 +56,7 @@ def muon(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_decay=
             continue
         if not p.is_contiguous() or not b.is_contiguous():
             raise ValueError('parameters and momentum buffers have to be contiguous')
+        written.extend((p, b))
         p = _matrix(p)
         ps.append(p)
         gs.append(_matrix(g.contiguous()))
@@ -63,6 +64,8 @@ def muon(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_decay=
         sizes.append(lr * math.sqrt(max(1., p.shape[0] / p.shape[1])))
         keeps.append(1. - lr * weight_decay)
     _ops.muon_update_batched(ps, gs, bs, sizes, keeps, momentum, nesterov, schedule, eps)
+    # (a graph from before the update that goes through these weights is refused by its backward pass)
+    torch.autograd.graph.increment_version(written)
 
 
 class Muon(Optimizer):
@@ -118,7 +121,7 @@ class Muon(Optimizer):
                 if 'momentum_buffer' not in state:
                     state['momentum_buffer'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 ps, gs, bs = by_type.setdefault((p.dtype, p.device), ([], [], []))
-                ps.append(p.data)
+                ps.append(p)
                 gs.append(p.grad)
                 bs.append(state['momentum_buffer'])
             options = {k: group[k] for k in ('lr', 'momentum', 'nesterov', 'weight_decay', 'steps',
