@@ -536,10 +536,11 @@ int kfac_muon_update_batched(int count, const int* rows, const int* cols, int ty
 /* ---- Root-mean-square norm ------------------------------------------------- */
 
 /* h = x + residual, rounded to its type;  y = h / sqrt(mean(h^2) + eps) * gain  for `rows` rows of
- * `dim` elements of `type` (0 float32, 1 bfloat16, 2 float16), rows of x and residual ldx and ldr
- * elements apart, those of y and h contiguous.  residual may be NULL (h is x then, and may be NULL);
- * gain is of `type`, or float32 with gain_is_float, or NULL for ones.  scale != NULL: y is in 8 bits
- * (float8 e4m3fn), scale[row] = max |y| / 448 (1 for a row of zeros) and y holds y / scale.
+ * `dim` elements (fewer than 2^31 rows of at most 2^24) of `type` (0 float32, 1 bfloat16, 2 float16),
+ * rows of x and residual ldx and ldr elements apart, those of y and h contiguous.  residual may be
+ * NULL (h is x then, and may be NULL); gain is of `type`, or float32 with gain_is_float, or NULL for
+ * ones.  scale != NULL: y is in 8 bits (float8 e4m3fn), scale[row] = max |y| / 448 (1 for a row of
+ * zeros) and y holds y / scale.
  * The normalisation in front of the layers of a decoder, as the reference has BatchNorm in front of
  * its (curv/cov/batchnorm.py:10-49). */
 int kfac_rms_norm(int type, int gain_is_float, int64_t rows, int dim, const void* x, int64_t ldx,

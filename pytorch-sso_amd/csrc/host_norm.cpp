@@ -44,8 +44,11 @@ bool gain_ok(const Tensor& gain, const Tensor& x) {
                              gain.size(0) == x.size(-1) && gain.is_contiguous() &&
                              (gain.scalar_type() == at::kFloat || gain.scalar_type() == x.scalar_type()));
 }
+// (the entry points take 32 bits of a row's length)
+constexpr int64_t MAX_DIM = 1 << 24;
 bool takes(const Tensor& x, const Tensor& residual, const Tensor& gain, const Tensor& curvature) {
-  if (!on_device(x) || type_code(x.scalar_type()) < 0 || x.dim() < 1 || x.size(-1) < 1) return false;
+  if (!on_device(x) || type_code(x.scalar_type()) < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > MAX_DIM)
+    return false;
   if (residual.defined() && (!on_device(residual) || residual.device() != x.device() ||
                              residual.scalar_type() != x.scalar_type() || residual.sizes() != x.sizes()))
     return false;

@@ -916,9 +916,13 @@ def _gain_args(gain, x, dim):
     return int(is_float), _hip.typed_ptr(gain, torch.float32 if is_float else x.dtype, x.device, 'gain')
 
 
+NORM_MAX_DIM = 1 << 24       # elements of a row that the kernels normalise
+
+
 def _norm_dim(x):
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise _hip.KfacHipError('cannot normalise a tensor of shape %s' % (tuple(x.shape),))
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= NORM_MAX_DIM:
+        raise _hip.KfacHipError('cannot normalise a tensor of shape %s (rows have 1 to %d elements)'
+                                % (tuple(x.shape), NORM_MAX_DIM))
     return x.shape[-1]
 
 
