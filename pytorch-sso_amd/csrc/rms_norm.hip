@@ -434,22 +434,24 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(const BackArgs
   }
 }
 
-// The partial sums of the units, added up in an order that depends on their number alone.  A workgroup
-// takes 32 columns, E of them to a thread, in G groups of threads over the units (1024 units of 4096 columns in
-// 7 to 8 us; in 24 with 16 groups of a column to a thread).
+// The partial sums of the units, added up in 64 bits (rounded once on the way, a group's sum) and in an order
+// that depends on their number alone.  A workgroup
+// takes 32 columns, E of them to a thread, in G groups of threads over the units (1024 units of 4096 columns,
+// a sample each 6.4 us, of 8 samples 7.0; in 24 with 16 groups of a column to a thread).
 constexpr int REDUCE_COLUMNS = 32, REDUCE_THREADS = 1024;
 template <int E>
 __global__ __launch_bounds__(REDUCE_THREADS) void norm_reduce_kernel(const float* partial, Deal d, int dim, void* dw,
                                                                      int w_type, float* curvature) {
-  constexpr int LANES = REDUCE_COLUMNS / E, G = REDUCE_THREADS / LANES;
+  constexpr int LANES = REDUCE_COLUMNS / E, G = REDUCE_THREADS / LANES, TEAMS = REDUCE_THREADS / REDUCE_COLUMNS;
   __shared__ float part[2][G][REDUCE_COLUMNS + 1];
+  __shared__ double sums[2][TEAMS][REDUCE_COLUMNS];
   const int group = threadIdx.x / LANES, column = threadIdx.x % LANES * E, c = blockIdx.x * REDUCE_COLUMNS + column;
-  float sum[E], sq[E];
+  double sum[E], sq[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) sum[e] = sq[e] = 0.f;
+  for (int e = 0; e < E; ++e) sum[e] = sq[e] = 0.;
   const bool squares = curvature != nullptr;
-  // to = sum over `count` units from `first` on, `step` apart, several in flight
-  const auto add = [&](long first, long step, int count, float (&to)[E]) {
+  // to = sum over `count` units from `first` on, `step` apart, several in flight; squared: sq, of their squares
+  const auto add = [&](long first, long step, int count, double (&to)[E], bool squared = false) {
     if (c >= dim) return;
     const float* at = partial + first * dim + c;
     constexpr int K = 8;
@@ -464,22 +466,29 @@ __global__ __launch_bounds__(REDUCE_THREADS) void norm_reduce_kernel(const float
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int e = 0; e < E; ++e) to[e] += v[k][e];
+        for (int e = 0; e < E; ++e) to[e] += (double)v[k][e];
+      if (squared)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int e = 0; e < E; ++e) sq[e] = fma((double)v[k][e], (double)v[k][e], sq[e]);
     }
   };
   // few samples in many parts: several groups a sample
-  const int share = d.parts > 0 && d.samples < G ? G / d.samples : 1;
-  if (d.parts > 0) {
+  const int share = d.parts > 1 && d.samples < G ? G / d.samples : 1;
+  if (d.parts == 1) {
+    add(group, G, group < d.samples ? (d.samples - group + G - 1) / G : 0, sum, true);
+  } else if (d.parts > 1) {
     for (int n = group / share; n < d.samples; n += G / share) {
-      float s[E];
+      double s[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) s[e] = 0.f;
+      for (int e = 0; e < E; ++e) s[e] = 0.;
       const int p = group % share;
       add((long)n * d.parts + p, share, p < d.parts ? (d.parts - p + share - 1) / share : 0, s);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         sum[e] += s[e];
-        if (share == 1) sq[e] = fmaf(s[e], s[e], sq[e]);
+        if (share == 1) sq[e] = fma(s[e], s[e], sq[e]);
       }
     }
   } else {
@@ -489,32 +498,42 @@ __global__ __launch_bounds__(REDUCE_THREADS) void norm_reduce_kernel(const float
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    part[0][group][column + e] = sum[e];
-    part[1][group][column + e] = sq[e];
+    part[0][group][column + e] = (float)sum[e];
+    part[1][group][column + e] = (float)sq[e];
   }
   __syncthreads();
-  const int mine = threadIdx.x, to = blockIdx.x * REDUCE_COLUMNS + mine;
-  if (mine >= REDUCE_COLUMNS || to >= dim) return;
-  float total = 0.f, square = 0.f;
+  // the groups' sums, or with several groups a sample the samples': dealt to 32 threads a column, then added up
+  const int mine = threadIdx.x % REDUCE_COLUMNS, team = threadIdx.x / REDUCE_COLUMNS;
+  double total = 0., square = 0.;
   if (share > 1) {
-    for (int n = 0; n < d.samples; ++n) {
-      float s = 0.f;
-      for (int i = 0; i < share; ++i) s += part[0][n * share + i][mine];
+    for (int n = team; n < d.samples; n += TEAMS) {
+      double s = 0.;
+      for (int i = 0; i < share; ++i) s += (double)part[0][n * share + i][mine];
       total += s;
-      square = fmaf(s, s, square);
+      square = fma(s, s, square);
     }
   } else {
-    for (int i = 0; i < G; ++i) {
-      total += part[0][i][mine];
-      square += part[1][i][mine];
+    for (int i = team; i < G; i += TEAMS) {
+      total += (double)part[0][i][mine];
+      square += (double)part[1][i][mine];
     }
   }
-  if (dw) {
-    if (w_type == TYPE_F32) ((float*)dw)[to] = total;
-    else if (w_type == TYPE_BF16) ((__hip_bfloat16*)dw)[to] = Element<__hip_bfloat16>::put(total);
-    else ((_Float16*)dw)[to] = Element<_Float16>::put(total);
+  sums[0][team][mine] = total;
+  sums[1][team][mine] = square;
+  __syncthreads();
+  const int to = blockIdx.x * REDUCE_COLUMNS + mine;
+  if (team > 1 || to >= dim) return;
+  double t[4] = {0., 0., 0., 0.};          // (an addition in 64 bits waits for the one before it)
+#pragma unroll
+  for (int i = 0; i < TEAMS; ++i) t[i & 3] += sums[team][i][mine];
+  const double all = (t[0] + t[1]) + (t[2] + t[3]);
+  if (team == 1) {
+    if (squares) curvature[to] = (float)((double)d.samples * all);
+  } else if (dw) {
+    if (w_type == TYPE_F32) ((float*)dw)[to] = (float)all;
+    else if (w_type == TYPE_BF16) ((__hip_bfloat16*)dw)[to] = Element<__hip_bfloat16>::put((float)all);
+    else ((_Float16*)dw)[to] = Element<_Float16>::put((float)all);
   }
-  if (squares) curvature[to] = (float)d.samples * square;
 }
 
 // Threads a row and accesses of `e` elements a thread; 0: longer than the registers of 1024 threads.
