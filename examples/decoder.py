@@ -78,17 +78,26 @@ class Decoder(nn.Module):
     def forward(self, tokens):
         return self.head(self.norm(*self.body(tokens))[0]).float()
 
+    def head_8(self):
+        """The last layer's weight in 8 bits, with a scale for each symbol."""
+        scale = (self.head.weight.float().abs().amax(1, keepdim=True) / 448.).clamp_(min=1e-12)
+        return (self.head.weight.float() / scale).to(torch.float8_e4m3fn), scale
+
+    @torch.no_grad()
+    def logits_8(self, x, stream, weight, scale):
+        """Of one token of each text, through the last norm and layer in 8 bits."""
+        q, q_scale, _ = torchsso.nn.add_rms_norm(x, stream, self.norm.weight, self.norm.eps,
+                                                 out_dtype=torch.float8_e4m3fn)
+        return torch._scaled_mm(q, weight.t(), scale_a=q_scale, scale_b=scale.t().contiguous(),
+                                out_dtype=torch.bfloat16).float()
+
     @torch.no_grad()
     def generate(self, tokens, count):
-        scale = (self.head.weight.float().abs().amax(1, keepdim=True) / 448.).clamp_(min=1e-12)
-        weight = (self.head.weight.float() / scale).to(torch.float8_e4m3fn)
+        weight, scale = self.head_8()
         for _ in range(count):
             x, stream = self.body(tokens)
-            q, q_scale, _ = torchsso.nn.add_rms_norm(x[:, -1], stream[:, -1], self.norm.weight, self.norm.eps,
-                                                     out_dtype=torch.float8_e4m3fn)
-            logits = torch._scaled_mm(q, weight.t(), scale_a=q_scale, scale_b=scale.t().contiguous(),
-                                      out_dtype=torch.bfloat16)
-            tokens = torch.cat([tokens, logits.float().argmax(-1, keepdim=True)], 1)
+            logits = self.logits_8(x[:, -1], stream[:, -1], weight, scale)
+            tokens = torch.cat([tokens, logits.argmax(-1, keepdim=True)], 1)
         return tokens
 
 
