@@ -221,6 +221,23 @@ struct OrthClock {
 constexpr int ORTH_MIN_PIECE = 4;                 // a shorter one writes its sums for too little work
 constexpr long ORTH_PARTIAL_BYTES = 64L << 20;    // of all pieces
 
+// What the pieces of a batch's launches can take at most: a reduction is cut into 16 pieces or fewer, of
+// ORTH_MIN_PIECE or more.
+inline long orth_partial_bytes(const OrthBatch& b) {
+  long most = 0;
+  for (int product : {ORTH_GRAM, ORTH_POLY, ORTH_APPLY})
+    for (const OrthKind& K : ORTH_KIND) {
+      if (K.tile > b.pad) continue;
+      long pieces = 0;
+      for (const OrthGroup& g : b.groups) {
+        const long c = std::min(16, (orth_length(g, product) + ORTH_MIN_PIECE - 1) / ORTH_MIN_PIECE);
+        if (c > 1) pieces += orth_tiles(g, std::min(K.tile, g.pad), product) * c;
+      }
+      most = std::max(most, pieces * K.tile * K.tile * 4);
+    }
+  return std::min(most, ORTH_PARTIAL_BYTES);
+}
+
 // The schedule of one kind, and its time: whole tiles as long as they keep all slots busy, the rest cut
 // if that gains more than the second launch and the pieces' sums cost.
 inline float orth_schedule(const OrthBatch& b, int product, int kind, OrthLaunch& out) {

@@ -904,14 +904,15 @@ Layout layout(const OrthPlan& plan) {
   Layout l{0, 0, 0, 0, 0, 256};
   if (plan.order.empty()) return l;        // small matrices alone
   l.sums = up(plan.order.size() * sizeof(OrthMat));
-  long sums = 0, count = 0;
+  long sums = 0, count = 0, partials = 0;
   for (const OrthBatch& b : plan.batches) {
     sums = std::max(sums, (long)b.count * SUM_MAX);
     count = std::max(count, (long)b.count);
+    partials = std::max(partials, orth_partial_bytes(b));
   }
   l.lifts = l.sums + up((size_t)sums * sizeof(double));
   l.partials = l.lifts + up((size_t)count * sizeof(int));
-  l.operands = l.partials + (size_t)ORTH_PARTIAL_BYTES;
+  l.operands = l.partials + up((size_t)partials);
   l.bytes = l.operands + (size_t)plan.halves * sizeof(half_t);
   return l;
 }

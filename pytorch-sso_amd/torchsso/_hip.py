@@ -315,9 +315,13 @@ class _Workspace(threading.local):
             if buf is not None and stream is not None:
                 # kernels of that stream may still use the buffer that is dropped here
                 buf.record_stream(stream)
-            # round up so that a slowly growing request does not reallocate each time
+            # round up so that a slowly growing request does not reallocate each time: to a power
+            # of two, a large one (of which twice as much would be felt) to an eighth of it
             size = max(nbytes, 1 << 20)
-            size = 1 << (size - 1).bit_length()
+            step = 1 << (size - 1).bit_length()
+            if step > 1 << 28:
+                step >>= 4
+            size = -(-size // step) * step
             buf = torch.empty(size, dtype=torch.uint8, device=device)
             self.bufs[key] = buf
         return buf, buf.numel()
