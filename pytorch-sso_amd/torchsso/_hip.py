@@ -271,10 +271,13 @@ def stream_ptr(device=None, stream=None):
     return torch._C._cuda_getCurrentRawStream(index)     # (no Stream object around the handle)
 
 
+_UNCHANGED = contextlib.nullcontext()
+
+
 def on_device(device):
     """Context in which `device` is current (the handle of a null stream means that of the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return _UNCHANGED
     return torch.cuda.device(device)
 
 

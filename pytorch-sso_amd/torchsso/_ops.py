@@ -795,13 +795,14 @@ ORTH_MAX_SIDE = 16384        # rows and columns of a matrix that the kernels ort
 
 
 def _matrix_dims(mats, what):
-    for i, m in enumerate(mats):
-        if m.dim() != 2:
-            raise _hip.KfacHipError('%s %d is not a matrix: %s' % (what, i, tuple(m.shape)))
-        if max(m.shape) > ORTH_MAX_SIDE:
+    shapes = [m.shape for m in mats]
+    for i, s in enumerate(shapes):
+        if len(s) != 2:
+            raise _hip.KfacHipError('%s %d is not a matrix: %s' % (what, i, tuple(s)))
+        if s[0] > ORTH_MAX_SIDE or s[1] > ORTH_MAX_SIDE:
             raise _hip.KfacHipError('%s %d is %d x %d: orthogonalisation takes sides of up to %d'
-                                    % (what, i, m.shape[0], m.shape[1], ORTH_MAX_SIDE))
-    return _hip.ints([m.shape[0] for m in mats]), _hip.ints([m.shape[1] for m in mats])
+                                    % (what, i, s[0], s[1], ORTH_MAX_SIDE))
+    return _hip.ints([s[0] for s in shapes]), _hip.ints([s[1] for s in shapes])
 
 
 @functools.lru_cache(maxsize=64)

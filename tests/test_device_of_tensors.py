@@ -51,7 +51,7 @@ def launches(monkeypatch):
         current.append(device.index)
         yield
         current.pop()
-    monkeypatch.setattr(torch.cuda, 'current_device', lambda: current[-1])
+    monkeypatch.setattr(torch._C, '_cuda_getDevice', lambda: current[-1])
     monkeypatch.setattr(torch.cuda, 'device', use)
     monkeypatch.setattr(_hip, 'load', lambda: Lib())
     monkeypatch.setattr(_hip, 'typed_ptr', lambda t, *args: t.data_ptr())
