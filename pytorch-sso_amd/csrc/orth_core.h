@@ -5,9 +5,9 @@
 // x = h + l with h = fp16(x), l = fp16(x - h), 22 bits and the sign of l, or h alone.  A product of
 // two such numbers is
 //     x y = h h' + h l' + l h' + [l l']
-// where the bracket is at most 2^-24 of |x y|, as much as one float32 rounding, and is left out:
-// three v_mfma_f32_16x16x32_f16 with exact products and float32 sums, where three bf16 parts, which
-// hold any float32, take six.
+// where the bracket is at most 2^-22 of |x y|, on average (l is 2^-12.2 of x) 2^-24.5, about what rounding to
+// float32 makes, and is left out: three v_mfma_f32_16x16x32_f16 with exact products and float32 sums, where
+// three bf16 parts, which hold any float32, take six.
 //
 // In memory a row of a matrix in two parts is made of pieces of 32 elements, 64 bytes of high parts and
 // 64 of low ones, so that what a tile reads of a row at a time, both parts of 32 elements, is one cache

@@ -526,8 +526,10 @@ __device__ __forceinline__ void orth_item(const OrthProduct& p, const OrthGroup&
 // (BX of AlexNet's layers, three products a number: 463 of float32 quality; the matrix cores busy 81 % of the
 // cycles at the 1.6 GHz that the power leaves), 1200 where a launch is one round of tiles and its tail; 128-wide
 // ones, two workgroups to a unit, at 1140 (A of 16 matrices of 1024 x 2752), both near what the library's own
-// fp16 product of 8192^3 reaches, 1250.  64-wide ones load 51 GB/s a unit, 13 TB/s in all, which bounds them: 635
-// (A of a ResNet-50's matrices), but they fill the chip where there are few tiles.
+// fp16 product of 8192^3 reaches, 1250.  64-wide ones wait for their loads: at 635 (A of
+// a ResNet-50's matrices) they ask the dies' caches for 13 TB/s, 36 % of which miss there and come from the last
+// cache at 4.8 TB/s (which of the two is the limit was not measured); but they fill the chip where there are few
+// tiles.
 template <class TILE, bool SPLIT, int MODE>
 __global__ __launch_bounds__(TILE::THREADS, TILE::LDS > 80 * 1024 ? 2 : 4) void orth_product_kernel(const OrthProduct p) {
   extern __shared__ __align__(16) char smem[];
