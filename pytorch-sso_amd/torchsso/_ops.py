@@ -809,31 +809,44 @@ def _matrix_dims(mats, what):
 def late_steps(dtype, coefficients):
     """In how many steps at the end of an orthogonalisation operands are kept in 11 bits instead of 22.
 
-    None of them where the result holds 11 bits or more.  Rounding X to 11 bits loses an eighth of what
-    rounding the result to bfloat16's 8 loses; in that unit a late step, f(t) = a t + b t^3 + c t^5 on
-    singular values t, turns an error e of X into at most
-        e' = max |t / f(t)| * sqrt(L^2 (e^2 + 1) + P^2),   L = max |f'|,  P = max |f(t) / t|:
-    X is rounded, and so is the diagonal of B; the factor in front is that of a matrix whose norm lies
-    in one direction while the errors lie in weak ones.  (What A rounds away is spread over all of it, and
-    that direction meets but a small part.)  As many steps are late as keep the result, at worst, within
-    1.5 times the error that its own rounding makes: e' <= 8 sqrt(1.5^2 - 1) = 8.9.  Of five steps of the
-    default coefficients that is one (8.1; a second one would make it 50): rank one with noise of 10^-3
-    is then 1.86e-3 from 64 bits, where the rounding alone makes 1.63e-3."""
+    None of them where the result holds 11 bits or more.  Rounding to 11 bits loses an eighth of what
+    rounding the result to bfloat16's 8 bits loses; in units of it a late step, f(t) = a t + b t^3 + c t^5 on
+    singular values t, leaves (to first order)
+      * of an error e that is spread over X, where one direction holds the norm and the error lies in weak ones,
+          e' = max |t / f| * sqrt(L^2 (e^2 + 1) + P^2),   L = max |f'|,  P = max |f / t|
+        on average: X is rounded, and so is the diagonal of B.  (What A rounds away is spread over all of it, and
+        that direction meets but a small part);
+      * of a single element that holds the norm, whose three roundings do not average out,
+          r' = max |f' t / f| * r + max (|f'| + |b t^2 + 2 c t^4|) |t / f| + 1   at most.
+    As many steps are late as keep both within 8.9: spread errors make the result's error 1.5 times (sqrt(1 +
+    (8.9 / 8)^2)) what its own rounding makes, an element is 1.1 times its largest rounding (2^-8) off.  Of five steps of
+    the default coefficients that is one (8.2 and 8.1; a second one would make it 50): rank one with noise of
+    10^-3 is then 1.86e-3 from 64 bits, where the rounding alone makes 1.63e-3."""
     if dtype != torch.bfloat16:
         return 0
-    steps, bound = [], 1.               # (slope, largest and smallest factor) of each
+    steps, bound = [], 1.
     for a, b, c in zip(*[iter(coefficients)] * 3):
         ts = [bound * i / 256 for i in range(257)]
         factors = [abs(a + b * t ** 2 + c * t ** 4) for t in ts]
-        steps.append((max(abs(a + 3 * b * t ** 2 + 5 * c * t ** 4) for t in ts), max(factors), min(factors)))
+        slopes = [abs(a + 3 * b * t ** 2 + 5 * c * t ** 4) for t in ts]
+        if min(factors) == 0.:
+            steps.append(None)
+        else:
+            own = [s + abs(b * t ** 2 + 2 * c * t ** 4) for s, t in zip(slopes, ts)]
+            steps.append((max(slopes), max(factors), min(factors), max(s / f for s, f in zip(slopes, factors)),
+                          max(o / f for o, f in zip(own, factors)) + 1))
         bound = max(t * f for t, f in zip(ts, factors))
     late = 0
     while late < len(steps):
-        error = 0.
-        for slope, most, least in steps[len(steps) - late - 1:]:
-            error = math.inf if least == 0. else math.sqrt(slope ** 2 * (error ** 2 + 1) + most ** 2) / least
-        if error > 8.9:
-            break
+        spread = single = 0.
+        for step in steps[len(steps) - late - 1:]:
+            if step is None:             # (a direction may vanish)
+                return late
+            slope, most, least, gain, own = step
+            spread = math.sqrt(slope ** 2 * (spread ** 2 + 1) + most ** 2) / least
+            single = gain * single + own
+        if max(spread, single) > 8.9:
+            return late
         late += 1
     return late
 

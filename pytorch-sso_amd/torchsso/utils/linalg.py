@@ -96,8 +96,8 @@ def orthogonalize(mats, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     tensors of the same shapes and type.  `coefficients`: (a, b, c), or one triple per step.
 
     Products run on the fp16 matrix cores in two parts a number (as good as float32).  Of a bfloat16
-    matrix the last steps run in one part, as many as leave at most 1.5 times the error that rounding the
-    result makes (of the default steps one)."""
+    matrix the last steps run in one part, as many as add about as much error at most as rounding the
+    result does (of the default steps one)."""
     schedule = newton_schulz_schedule(steps, coefficients)
     check_orthogonalize_eps(eps)
     single = isinstance(mats, torch.Tensor)

@@ -54,3 +54,22 @@ def test_more_late_steps_than_that_are_not_taken():
     assert late == {'default': 1, 'one': 1, 'cubic': 3, 'steep': 0, 'falling': 2}
     for dtype in (torch.float32, torch.float16):
         assert all(_ops.late_steps(dtype, s) == 0 for s in flat.values())
+
+
+@pytest.mark.parametrize('shape', [(65, 300), (256, 512), (3, 4000), (1000, 40)])
+@pytest.mark.parametrize('schedule', list(SCHEDULES.values()) + [
+    ((1.5262, -1.7437, 0.8985), (2.7571, -1.7730, 1.9739), (0.9136, -0.6772, 0.2028))])
+def test_single_elements_that_hold_the_norm(shape, schedule):
+    """Their roundings do not average out: they may be 1.1 times the largest rounding of an element of the result, 2^-8, off."""
+    gen = torch.Generator().manual_seed(0)
+    for count, value in ((1, 1.), (1, 1.37), (1, 1.999), (2, 1.3)):
+        m = 1e-3 * torch.randn(shape, generator=gen)
+        for i in range(count):
+            m[i, i + 5] = value
+        g = m.to(torch.bfloat16)
+        want = reference(g if shape[0] <= shape[1] else g.t(), schedule)
+        want = want if shape[0] <= shape[1] else want.t()
+        rounding = (want.to(torch.bfloat16).double() - want).norm()
+        out = torchsso.utils.orthogonalize(g.cuda(), len(schedule), schedule)
+        error = (out.cpu().double() - want).norm()
+        assert error <= 1.5 * rounding + 8.9 / 8 * 2 ** -8 * want.norm(), (count, value, (error / want.norm()).item())
