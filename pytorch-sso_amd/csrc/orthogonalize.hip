@@ -375,7 +375,8 @@ __device__ __forceinline__ half_t* orth_target(const OrthProduct& p, const OrthG
 // 113 us on writing.
 template <class TILE, bool SPLIT, int MODE>
 __device__ __forceinline__ void orth_write(const OrthProduct& p, const OrthFactors& factors, const OrthGroup& g,
-                                           const OrthMat& mat, int k, int m0, int n0, bool mirror, f4 (&acc)[TILE::FM][TILE::FN], lds_char* lds, int lane) {
+                                           const OrthMat& mat, int k, int m0, int n0, bool mirror,
+                                           f4 (&acc)[TILE::FM][TILE::FN], lds_char* lds, int lane) {
   constexpr int FM = TILE::FM, FN = TILE::FN;
   typedef __attribute__((address_space(3))) half_t lds_half;
   typedef __attribute__((address_space(3))) h4 lds_h4;
@@ -518,18 +519,17 @@ __device__ __forceinline__ void orth_item(const OrthProduct& p, const OrthGroup&
   OrthMat mat;
   if (MODE == LAST) mat = p.mats[g.first + k];
   const OrthFactors factors = orth_factors<MODE>(p, lift);
-  orth_write<TILE, SPLIT, MODE>(p, factors, g, mat, k, tm * T + wm * FM * 16, tn * T + wn * FN * 16, SYM && tm != tn, acc,
-                                lds + TILE::SUMS + wave * TILE::WRITE, lane);
+  orth_write<TILE, SPLIT, MODE>(p, factors, g, mat, k, tm * T + wm * FM * 16, tn * T + wn * FN * 16, SYM && tm != tn,
+                                acc, lds + TILE::SUMS + wave * TILE::WRITE, lane);
 }
 
 // One launch: the tiles of all groups, or pieces of them.  256-wide tiles run at 1390 TFLOP/s of fp16 products
 // (BX of AlexNet's layers, three products a number: 463 of float32 quality; the matrix cores busy 81 % of the
 // cycles at the 1.6 GHz that the power leaves), 1200 where a launch is one round of tiles and its tail; 128-wide
 // ones, two workgroups to a unit, at 1140 (A of 16 matrices of 1024 x 2752), both near what the library's own
-// fp16 product of 8192^3 reaches, 1250.  64-wide ones wait for their loads: at 635 (A of
-// a ResNet-50's matrices) they ask the dies' caches for 13 TB/s, 36 % of which miss there and come from the last
-// cache at 4.8 TB/s (which of the two is the limit was not measured); but they fill the chip where there are few
-// tiles.
+// fp16 product of 8192^3 reaches, 1250.  64-wide ones wait for their loads: at 660 (A of a ResNet-50's matrices)
+// they ask the dies' caches for 13 TB/s, of which 36 % miss and come from the last cache at 4.8 TB/s (which of
+// the two is the limit was not measured); but they fill the chip where there are few tiles.
 template <class TILE, bool SPLIT, int MODE>
 __global__ __launch_bounds__(TILE::THREADS, TILE::LDS > 80 * 1024 ? 2 : 4) void orth_product_kernel(const OrthProduct p) {
   extern __shared__ __align__(16) char smem[];
