@@ -221,8 +221,9 @@ struct OrthClock {
 constexpr int ORTH_MIN_PIECE = 4;                 // a shorter one writes its sums for too little work
 constexpr long ORTH_PARTIAL_BYTES = 64L << 20;    // of all pieces
 
-// What the pieces of a batch's launches can take at most: a reduction is cut into 16 pieces or fewer, of
-// ORTH_MIN_PIECE or more.
+// Room for the pieces of a batch's launches, which no schedule exceeds.  A piece is a sixteenth or more of the
+// longest tile's length, in which ORTH_NARROW of a narrow tile's reduction count, and ORTH_MIN_PIECE or more.
+constexpr float ORTH_NARROW = 0.6f;
 inline long orth_partial_bytes(const OrthBatch& b) {
   long most = 0;
   for (int product : {ORTH_GRAM, ORTH_POLY, ORTH_APPLY})
@@ -230,8 +231,10 @@ inline long orth_partial_bytes(const OrthBatch& b) {
       if (K.tile > b.pad) continue;
       long pieces = 0;
       for (const OrthGroup& g : b.groups) {
-        const long c = std::min(16, (orth_length(g, product) + ORTH_MIN_PIECE - 1) / ORTH_MIN_PIECE);
-        if (c > 1) pieces += orth_tiles(g, std::min(K.tile, g.pad), product) * c;
+        const int all = orth_length(g, product), tile = std::min(K.tile, g.pad);
+        const long c = std::min((int)((tile < K.tile ? 16.f / ORTH_NARROW : 16.f) + 1.f),
+                                (all + ORTH_MIN_PIECE - 1) / ORTH_MIN_PIECE);
+        if (c > 1) pieces += orth_tiles(g, tile, product) * c;
       }
       most = std::max(most, pieces * K.tile * K.tile * 4);
     }
@@ -255,7 +258,7 @@ inline float orth_schedule(const OrthBatch& b, int product, int kind, OrthLaunch
     OrthSlice& s = out.slices[i];
     s.tile = std::min(K.tile, g.pad);
     s.tiles = s.whole = (int)orth_tiles(g, s.tile, product);
-    length[i] = orth_length(g, product) * (s.tile < K.tile ? 0.6f : 1.f) + ends;
+    length[i] = orth_length(g, product) * (s.tile < K.tile ? ORTH_NARROW : 1.f) + ends;
     work += (double)length[i] * s.tiles;
     longest = std::max(longest, length[i]);
     order[i] = i;
@@ -299,7 +302,7 @@ inline float orth_schedule(const OrthBatch& b, int product, int kind, OrthLaunch
       }
       const long bytes = pieces * K.tile * K.tile * 4;
       const float t = clock.end * K.unit + 5.f + 2.f * bytes / 3.5e6f;
-      if (bytes <= ORTH_PARTIAL_BYTES && t < best - 10.f) {
+      if (t < best - 10.f && bytes <= orth_partial_bytes(b)) {
         best = t;
         out.slices = cut;
       }

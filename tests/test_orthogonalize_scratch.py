@@ -6,6 +6,7 @@ import subprocess
 import pytest
 import torch
 
+import torchsso
 from torchsso import _hip
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'pytorch-sso_amd', 'csrc')
@@ -67,3 +68,29 @@ def test_large_scratch_is_not_doubled(monkeypatch):
         assert size <= max(2 * nbytes, 1 << 20) if nbytes <= 1 << 28 else size <= nbytes * 1.125
         # what grows slowly does not allocate each time
         assert workspace.get(device, size)[0] is buf
+
+
+def test_the_pieces_of_narrow_matrices_beside_wider_ones_fit(tmp_path):
+    """(64-wide tiles in a launch of 128-wide ones, whose reductions are cut into more pieces)"""
+    (tmp_path / 'main.cpp').write_text(PROGRAM)
+    subprocess.run(['g++', '-O2', '-std=c++17', '-I', CSRC, str(tmp_path / 'main.cpp'), '-o', str(tmp_path / 'plan')], check=True)
+    rng = random.Random(1)
+    side = lambda low, high: int(round(2 ** rng.uniform(low, high)))
+    lists = [[(9, 5835), (65, 65), (16, 628)], [(51, 5863), (288, 343)], [(50, 5329), (329, 185)], [(64, 16384), (65, 70)]]
+    lists += [[(side(0, 6), side(6, 14)) for _ in range(rng.randint(1, 4))] + [(side(6, 10), side(6, 12)) for _ in range(rng.randint(1, 5))]
+              for _ in range(3000)]
+    text = '\n'.join('%d %s' % (len(s), ' '.join('%d %d' % m for m in s)) for s in lists)
+    assert subprocess.run([str(tmp_path / 'plan')], input=text, text=True).returncode == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shapes', [[(9, 5835), (65, 65), (16, 628)], [(51, 5863), (288, 343)], [(64, 16384), (65, 70)]])
+def test_narrow_matrices_beside_wider_ones(shapes):
+    mats = [torch.randn(s, generator=torch.Generator().manual_seed(i)).cuda() for i, s in enumerate(shapes)]
+    for m, o in zip(mats, torchsso.utils.orthogonalize(mats)):
+        x = m.double() / (m.double().norm() + 1e-7)
+        for _ in range(5):
+            a = x @ x.t().contiguous()
+            x = 3.4445 * x + (-4.7750 * a + 2.0315 * (a @ a)) @ x
+        # (15 products round operands to 2^-23, which grows by 1.5 in each step behind, if all errors are of one sign)
+        assert (o.double() - x).norm() <= 4.7e-5 * x.norm()
