@@ -562,6 +562,34 @@ int kfac_rms_norm_backward(int type, int gain_is_float, int64_t rows, int dim, i
                            float eps, void* dx, void* dgain, float* curvature, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* ---- Layer norm ------------------------------------------------------------- */
+
+/* h = x + residual, rounded to its type;  y = (h - mean(h)) / sqrt(var(h) + eps) * gain + bias,  with the
+ * arguments of kfac_rms_norm and bias of the gain's type, or NULL (gain NULL: no bias either).  stats != NULL:
+ * receives what the backward pass needs of each row, 3 floats [rows][3]: a mean m of h, the mean e of
+ * h - m (what rounding has lost of m), and 1 / sqrt(var + eps); y may be NULL then.
+ * The normalisation in front of the layers of a decoder, as the reference has BatchNorm in front of
+ * its (curv/cov/batchnorm.py:10-49). */
+int kfac_layer_norm(int type, int gain_is_float, int64_t rows, int dim, const void* x, int64_t ldx,
+                    const void* residual, int64_t ldr, const void* gain, const void* bias, float eps, void* y, void* h,
+                    float* scale, float* stats, void* stream);
+
+/* Backward pass of kfac_layer_norm from the gradient dy of y and dh of h (NULL: none), with
+ * xh = (h - mean) / sqrt(var + eps) and u = gain dy:
+ *   dx = dh + (u - mean(u) - xh mean(u xh)) / sqrt(var + eps)   (also the residual's gradient; NULL: not wanted)
+ *   s_n = sum over the rows of sample n of dy xh (and of dy)        (rows / samples consecutive ones)
+ *   dgain, dbias = sum_n s_n          (of the gain's type; NULL: not wanted)
+ *   curvature = samples * sum_n s_n^2 (float32 [vectors][dim]; NULL: not wanted), the diagonal curvature of gain
+ *        and bias, scaled as kfac_rms_norm_backward's (curvature.py:154-158)
+ * vectors: 2 with the sums of dy, 1 without (dbias NULL then).  The sums over rows are formed in an order that
+ * depends on the sizes alone.  `squares` of the workspace query: whether a curvature is wanted; without dgain,
+ * dbias and curvature no workspace is. */
+size_t kfac_layer_norm_backward_workspace_bytes(int type, int64_t rows, int dim, int samples, int vectors, int squares);
+int kfac_layer_norm_backward(int type, int gain_is_float, int64_t rows, int dim, int samples, int vectors,
+                             const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh,
+                             const float* stats, const void* gain, void* dx, void* dgain, void* dbias,
+                             float* curvature, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

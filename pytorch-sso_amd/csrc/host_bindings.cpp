@@ -20,6 +20,8 @@
 // (host_norm.cpp)
 PyObject* host_bind_norm(PyObject*, PyObject* const*, Py_ssize_t);
 PyObject* host_rms_norm(PyObject*, PyObject* const*, Py_ssize_t);
+PyObject* host_bind_layer_norm(PyObject*, PyObject* const*, Py_ssize_t);
+PyObject* host_layer_norm(PyObject*, PyObject* const*, Py_ssize_t);
 
 namespace {
 
@@ -381,6 +383,9 @@ PyMethodDef methods[] = {
     {"order", KFAC_FAST(order), "order(device, waiting stream, stream waited for)"},
     {"bind_norm", KFAC_FAST(host_bind_norm), "bind_norm(norm, workspace, backward): the library's entry points"},
     {"rms_norm", KFAC_FAST(host_rms_norm), "rms_norm(x, residual, gain, eps, curvature, eight), or None"},
+    {"bind_layer_norm", KFAC_FAST(host_bind_layer_norm),
+     "bind_layer_norm(norm, workspace, backward): the library's entry points"},
+    {"layer_norm", KFAC_FAST(host_layer_norm), "layer_norm(x, residual, gain, bias, eps, curvature, eight), or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,

@@ -14,6 +14,7 @@ from torchsso.curv.cov.linear import CovLinear, DiagCovLinear, KronCovLinear  # 
 from torchsso.curv.cov.conv import CovConv2d, DiagCovConv2d, KronCovConv2d  # NOQA
 from torchsso.curv.cov.batchnorm import CovBatchNorm1d, DiagCovBatchNorm1d, CovBatchNorm2d, DiagCovBatchNorm2d  # NOQA
 from torchsso.curv.cov.rms_norm import DiagCovRMSNorm  # NOQA
+from torchsso.curv.cov.layer_norm import DiagCovLayerNorm  # NOQA
 
 from torchsso.curv.fisher import Fisher, get_closure_for_fisher  # NOQA
 from torchsso.curv.fisher import KronFisherLinear, KronFisherConv2d, DiagFisherBatchNorm2d  # NOQA

@@ -141,6 +141,12 @@ _SIGNATURES = {
     'kfac_rms_norm_backward': (c_int, [c_int, c_int, c_i64, c_int, c_int, c_ptr, c_i64, c_ptr, c_i64,
                                        c_ptr, c_i64, c_ptr, c_f32, c_ptr, c_ptr, c_ptr, c_ptr, c_size,
                                        c_ptr]),
+    'kfac_layer_norm': (c_int, [c_int, c_int, c_i64, c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_f32,
+                                c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
+    'kfac_layer_norm_backward_workspace_bytes': (c_size, [c_int, c_i64, c_int, c_int, c_int, c_int]),
+    'kfac_layer_norm_backward': (c_int, [c_int, c_int, c_i64, c_int, c_int, c_int, c_ptr, c_i64, c_ptr, c_i64,
+                                         c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size,
+                                         c_ptr]),
 }
 
 # element types of the entry points that take more than float32
@@ -216,6 +222,8 @@ def load():
         _addresses['kfac_rowsq_sum'] = ctypes.cast(lib.kfac_rowsq_sum, ctypes.c_void_p).value
         _host.bind_norm(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             'kfac_rms_norm', 'kfac_rms_norm_backward_workspace_bytes', 'kfac_rms_norm_backward')])
+        _host.bind_layer_norm(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            'kfac_layer_norm', 'kfac_layer_norm_backward_workspace_bytes', 'kfac_layer_norm_backward')])
         _lib = lib
     return _lib
 

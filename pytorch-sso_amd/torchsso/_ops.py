@@ -1020,3 +1020,104 @@ def rms_norm_backward(dy, dh, h, gain, eps, samples, want_dx=True, want_dgain=Tr
             _ws_ptr(ws), ws_bytes, _hip.stream_ptr(h.device))
     _hip.check(st, 'kfac_rms_norm_backward')
     return dx, dgain
+
+
+def _check_layer_norm(x, residual, gain, bias, curvature):
+    """Raises what is wrong with the arguments of a layer norm."""
+    dim = _norm_dim(x)
+    _element_type(x, 'input')
+    _row_ptr(x, x, 'input')
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise _hip.KfacHipError('residual has shape %s, expected %s'
+                                    % (tuple(residual.shape), tuple(x.shape)))
+        _row_ptr(residual, x, 'residual')
+    _gain_args(gain, x, dim)
+    if bias is not None:
+        if tuple(bias.shape) != (dim,):
+            raise _hip.KfacHipError('bias has shape %s, expected (%d,)' % (tuple(bias.shape), dim))
+        _hip.typed_ptr(bias, gain.dtype, x.device, 'bias')
+    if curvature is not None:
+        want = (dim,) if bias is None else (2, dim)
+        if tuple(curvature.shape) != want:
+            raise _hip.KfacHipError('curvature has shape %s, expected %s' % (tuple(curvature.shape), want))
+        _hip.typed_ptr(curvature, torch.float32, x.device, 'curvature')
+    raise _hip.KfacHipError('layer_norm cannot take these arguments')
+
+
+def layer_norm_autograd(x, residual, gain, bias, eps, curvature=None, eight_bit=False):
+    """y or (y, h) with h = x + residual and y = (h - mean(h)) / std(h) * gain + bias, with its backward pass
+    (csrc/host_norm.cpp); in 8 bits (y, scale) or (y, scale, h), without one."""
+    _hip.load()
+    out = _hip._host.layer_norm(x, residual, gain, bias, eps, curvature, eight_bit)
+    if out is None:
+        _check_layer_norm(x, residual, gain, bias, curvature)
+    return out
+
+
+def layer_norm_stats(h, eps):
+    """What layer_norm_backward needs of each row of h: [rows, 3]."""
+    lib = _hip.load()
+    dim = _norm_dim(h)
+    kind = _element_type(h, 'stream')
+    rows, ldh = _rows(h, dim)
+    address = _row_ptr(rows, h, 'stream')
+    stats = torch.empty((rows.shape[0], 3), dtype=torch.float32, device=h.device)
+    with _hip.on_device(h.device):
+        st = lib.kfac_layer_norm(kind, 0, rows.shape[0], dim, address, ldh, None, 0, None, None, float(eps), None,
+                                 None, None, stats.data_ptr(), _hip.stream_ptr(h.device))
+    _hip.check(st, 'kfac_layer_norm')
+    return stats
+
+
+def layer_norm_backward(dy, dh, h, stats, gain, samples, want_dx=True, want_dgain=True, want_dbias=True,
+                        curvature=None):
+    """(dx, dgain, dbias) of a layer norm from the gradients of y and of h (None: none), each None where it is not
+    wanted (dgain, dbias: of the gain's type, or without a gain None); `curvature`: a float32 tensor that receives the
+    diagonal curvature over `samples` samples, of the gain [dim] or of gain and bias [2, dim]."""
+    lib = _hip.load()
+    dim = _norm_dim(h)
+    kind = _element_type(h, 'stream')
+    is_float, gain_ptr = _gain_args(gain, h, dim)
+    stream_rows, ldh = _rows(h, dim)
+    rows = stream_rows.shape[0]
+    for what, g in (('gradient', dy), ('stream gradient', dh)):
+        if g is not None and g.shape != h.shape:
+            raise _hip.KfacHipError('%s has shape %s, expected %s' % (what, tuple(g.shape), tuple(h.shape)))
+    if tuple(stats.shape) != (rows, 3):
+        raise _hip.KfacHipError('statistics have shape %s, expected (%d, 3)' % (tuple(stats.shape), rows))
+    if rows > 0 and (samples < 1 or rows % samples != 0):
+        raise _hip.KfacHipError('%d rows are not %d samples' % (rows, samples))
+    want_dgain, want_dbias = want_dgain and gain is not None, want_dbias and gain is not None
+    vectors, c_ptr = (2 if want_dbias else 1), None
+    if curvature is not None:
+        if tuple(curvature.shape) not in ((dim,), (2, dim)) or (vectors == 2 and curvature.dim() == 1):
+            raise _hip.KfacHipError('curvature has shape %s, expected %s' % (
+                tuple(curvature.shape), '(2, %d)' % dim if vectors == 2 else '(%d,) or (2, %d)' % (dim, dim)))
+        vectors = curvature.dim()
+        c_ptr = _hip.typed_ptr(curvature, torch.float32, h.device, 'curvature')
+    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device) if want_dx else None
+    dgain = torch.empty_like(gain) if want_dgain else None
+    dbias = torch.empty_like(gain) if want_dbias else None
+    if rows == 0:
+        for t in (dgain, dbias, curvature):
+            if t is not None:
+                t.zero_()
+        return dx, dgain, dbias
+    dy, lddy = _rows(dy, dim)
+    args = [_row_ptr(dy, h, 'gradient'), lddy, None, 0]
+    if dh is not None and want_dx:
+        dh, lddh = _rows(dh, dim)
+        args[2:] = [_row_ptr(dh, h, 'stream gradient'), lddh]
+    ws, ws_bytes = None, 0
+    with _hip.on_device(h.device):
+        if dgain is not None or dbias is not None or curvature is not None:
+            ws, ws_bytes = _hip.workspace(h.device, lib.kfac_layer_norm_backward_workspace_bytes(
+                kind, rows, dim, samples, vectors, int(curvature is not None)))
+        st = lib.kfac_layer_norm_backward(
+            kind, is_float, rows, dim, samples, vectors, *args, _row_ptr(stream_rows, h, 'stream'), ldh,
+            _hip.typed_ptr(stats, torch.float32, h.device, 'statistics'), gain_ptr,
+            *[None if t is None else t.data_ptr() for t in (dx, dgain, dbias)], c_ptr,
+            _ws_ptr(ws), ws_bytes, _hip.stream_ptr(h.device))
+    _hip.check(st, 'kfac_layer_norm_backward')
+    return dx, dgain, dbias
