@@ -533,6 +533,32 @@ int kfac_muon_update_batched(int count, const int* rows, const int* cols, int ty
                              const float* coefficients, float eps, int late_steps, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* AdamW's update of a list of tensors (HOST arrays of length `count`) of numel[i] consecutive elements of `type`
+ * (0 float32, 1 bfloat16, 2 float16; parameters and gradients alike), number t = steps[i] >= 1 of each:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ * in float32, each result rounded once.  state_bits 32: m and v are float32.  8: by blocks of 128 consecutive elements
+ * m is m / scale in float8 e4m3fn with scale = max |m| / 448 of the block, and v is v / scale in float8 e5m2 with scale =
+ * max v / 57344, m_scales[i] and v_scales[i] holding (numel[i] + 127) / 128 of them (a block whose largest number is
+ * below 2^-100 becomes zeros, with scale 0; numbers that are not finite are left out of the maximum).  Both are rounded to one of
+ * their neighbours by 16 random bits R each, up where the fraction + R / 65536 reaches 1, of the word that element
+ * k of unit u = 8 u .. 8 u + 7 of tensor i has, with all arithmetic modulo 2^32:
+ *   mix(x): x ^= x >> 16; x *= 0x9E3779B1; x ^= x >> 15; x *= 0xB504F333; x ^= x >> 16
+ *   w_0 = mix(mix(mix(mix(seed) + t) + i) + u),  w_(k+1) = w_k after w ^= w << 13; w ^= w >> 17; w ^= w << 5
+ * the upper 16 for m, the lower for v, except that a v above 0 becomes at least the smallest number.
+ * eps >= 0, in 8 bits at least 1e-12.  A call may hold one tensor once.
+ * counters != NULL (steps NULL then): device addresses of int32 numbers of updates so far, which the call raises by
+ * one and goes by, so that a recorded call counts on when it is replayed; lr_on_device != NULL (only with them): a
+ * float that is read in the place of lr.  Either needs the workspace.
+ * Stands where optim/secondorder.py:225-312 of the reference applies momentum, weight decay and the update, for the
+ * parameters whose curvature is not formed. */
+size_t kfac_adamw_workspace_bytes(int count, int counters_on_device);
+int kfac_adamw_batched(int count, const int64_t* numel, int type, int state_bits, void* const* params,
+                       const void* const* grads, void* const* m, void* const* v, float* const* m_scales,
+                       float* const* v_scales, const int64_t* steps, int* const* counters, double lr,
+                       const float* lr_on_device, double beta1, double beta2, double eps, double weight_decay,
+                       unsigned seed, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- Root-mean-square norm ------------------------------------------------- */
 
 /* h = x + residual, rounded to its type;  y = h / sqrt(mean(h^2) + eps) * gain  for `rows` rows of

@@ -15,7 +15,7 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'torchsso', 'libkfac_hip.so')
-HOST_SOURCES = [os.path.join(CSRC, name) for name in ('host_bindings.cpp', 'host_norm.cpp')]
+HOST_SOURCES = [os.path.join(CSRC, name) for name in ('host_bindings.cpp', 'host_norm.cpp', 'host_adamw.cpp')]
 HOST_OUT = os.path.join(HERE, 'torchsso', '_host.so')
 
 HIPCC_FLAGS = [

@@ -1,0 +1,210 @@
+// AdamW's update of a list of tensors: what the engine needs of them is looked up and checked here, without a loop in
+// Python (for the 160 tensors of a ResNet-50 the checks and addresses of five lists).
+//
+// Arguments that the engine cannot take make adamw return False, and the caller finds out which and raises.
+#include <Python.h>
+
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_strided.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "../../include/kfac_hip.h"
+
+namespace {
+
+using at::Tensor;
+
+decltype(&kfac_adamw_batched) adamw_entry = nullptr;
+decltype(&kfac_adamw_workspace_bytes) adamw_workspace_entry = nullptr;
+
+constexpr int64_t STATE_BLOCK = 128;          // elements of an 8-bit state with one scale
+
+int adamw_type(at::ScalarType t) {
+  return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1;
+}
+
+// A list or tuple of tensors
+bool tensors_of(PyObject* o, std::vector<Tensor>& out) {
+  PyObject* const seq = PySequence_Fast(o, "expected a list or tuple");
+  if (!seq) {
+    PyErr_Clear();
+    return false;
+  }
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+  out.reserve((size_t)n);
+  bool ok = true;
+  for (Py_ssize_t i = 0; ok && i < n; ++i) {
+    PyObject* const t = PySequence_Fast_GET_ITEM(seq, i);
+    ok = THPVariable_Check(t);
+    if (ok) out.push_back(THPVariable_Unpack(t));
+  }
+  Py_DECREF(seq);
+  return ok;
+}
+
+bool strided_on(const Tensor& t, at::Device device, at::ScalarType type) {
+  return t.defined() && t.layout() == at::kStrided && t.device() == device && t.scalar_type() == type;
+}
+// The elements of `t` lie in memory as those of `like` do.
+bool lies_as(const Tensor& t, const Tensor& like) {
+  if (t.sizes() != like.sizes()) return false;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) != like.stride(d)) return false;
+  return true;
+}
+
+struct WithoutInterpreter {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~WithoutInterpreter() { PyEval_RestoreThread(state); }
+};
+
+// No element is written twice.
+bool apart(const std::vector<Tensor>& written) {
+  std::vector<std::pair<const char*, const char*>> ranges;
+  ranges.reserve(written.size());
+  for (const Tensor& t : written)
+    if (t.numel() > 0) {
+      const char* const at = (const char*)t.const_data_ptr();
+      ranges.emplace_back(at, at + t.numel() * (int64_t)t.element_size());
+    }
+  std::sort(ranges.begin(), ranges.end());
+  for (size_t i = 1; i < ranges.size(); ++i)
+    if (ranges[i].first < ranges[i - 1].second) return false;
+  return true;
+}
+
+}  // namespace
+
+// bind_adamw(addresses of the two entry points)
+PyObject* host_bind_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 2) {
+    PyErr_SetString(PyExc_TypeError, "bind_adamw(update, workspace)");
+    return nullptr;
+  }
+  adamw_entry = (decltype(adamw_entry))PyLong_AsVoidPtr(args[0]);
+  adamw_workspace_entry = (decltype(adamw_workspace_entry))PyLong_AsVoidPtr(args[1]);
+  if (PyErr_Occurred()) return nullptr;
+  Py_RETURN_NONE;
+}
+
+// adamw(params, grads, m, v, scales of m or None, scales of v or None, steps (a number, a list of numbers or a list of
+// tensors), lr (a number or a tensor), beta1, beta2, eps, weight decay, seed) -> True, or False
+PyObject* host_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 13) {
+    PyErr_SetString(PyExc_TypeError,
+                    "adamw(params, grads, m, v, m_scales, v_scales, steps, lr, beta1, beta2, eps, weight_decay, seed)");
+    return nullptr;
+  }
+  const bool lr_on_device = THPVariable_Check(args[7]);
+  const double lr = lr_on_device ? 0. : PyFloat_AsDouble(args[7]), beta1 = PyFloat_AsDouble(args[8]),
+               beta2 = PyFloat_AsDouble(args[9]), eps = PyFloat_AsDouble(args[10]), decay = PyFloat_AsDouble(args[11]);
+  const unsigned long long seed = PyLong_AsUnsignedLongLongMask(args[12]);
+  if (PyErr_Occurred()) return nullptr;
+  try {
+    const bool eight = args[4] != Py_None;
+    std::vector<Tensor> params, grads, states[4], counters;
+    if (!adamw_entry || !tensors_of(args[0], params) || !tensors_of(args[1], grads) || params.empty() ||
+        grads.size() != params.size())
+      Py_RETURN_FALSE;
+    const size_t n = params.size();
+    for (int k = 0; k < (eight ? 4 : 2); ++k)
+      if (!tensors_of(args[2 + k], states[k]) || states[k].size() != n) Py_RETURN_FALSE;
+    const at::Device device = params[0].device();
+    const at::ScalarType type = params[0].scalar_type();
+    if (!params[0].is_cuda() || adamw_type(type) < 0) Py_RETURN_FALSE;
+    // the numbers of the updates
+    std::vector<int64_t> steps;
+    if (PyLong_Check(args[6])) {
+      steps.assign(n, PyLong_AsLongLong(args[6]));
+    } else if (!tensors_of(args[6], counters)) {
+      counters.clear();
+      PyObject* const seq = PySequence_Fast(args[6], "expected a list or tuple");
+      if (!seq) {
+        PyErr_Clear();
+        Py_RETURN_FALSE;
+      }
+      for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i)
+        steps.push_back(PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq, i)));
+      Py_DECREF(seq);
+    }
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      Py_RETURN_FALSE;
+    }
+    if ((steps.empty() ? counters.size() : steps.size()) != n) Py_RETURN_FALSE;
+    for (const int64_t t : steps)
+      if (t < 1) Py_RETURN_FALSE;
+    for (const Tensor& t : counters)
+      if (!strided_on(t, device, at::kInt) || t.numel() != 1) Py_RETURN_FALSE;
+    Tensor rate;
+    if (lr_on_device) {
+      rate = THPVariable_Unpack(args[7]);
+      if (counters.empty() || !strided_on(rate, device, at::kFloat) || rate.numel() != 1) Py_RETURN_FALSE;
+    }
+    const at::ScalarType state_types[4] = {eight ? at::kFloat8_e4m3fn : at::kFloat, eight ? at::kFloat8_e5m2 : at::kFloat,
+                                           at::kFloat, at::kFloat};
+    std::vector<Tensor> written(params);
+    for (size_t i = 0; i < n; ++i) {
+      const Tensor& p = params[i];
+      if (!strided_on(p, device, type) || !p.unsafeGetTensorImpl()->is_non_overlapping_and_dense() ||
+          !strided_on(grads[i], device, type) || grads[i].sizes() != p.sizes())
+        Py_RETURN_FALSE;
+      for (int k = 0; k < (eight ? 4 : 2); ++k) {
+        const Tensor& t = states[k][i];
+        if (!strided_on(t, device, state_types[k])) Py_RETURN_FALSE;
+        if (k < 2 ? !lies_as(t, p)
+                  : t.dim() != 1 || !t.is_contiguous() || t.size(0) != (p.numel() + STATE_BLOCK - 1) / STATE_BLOCK)
+          Py_RETURN_FALSE;
+        written.push_back(t);
+      }
+    }
+    written.insert(written.end(), counters.begin(), counters.end());
+    if (!apart(written)) Py_RETURN_FALSE;
+    int status;
+    {
+      const WithoutInterpreter released;
+      const c10::DeviceGuard guard(device);
+      std::vector<int64_t> numel(n);
+      std::vector<const void*> g(n);
+      std::vector<void*> at[5];
+      for (auto& a : at) a.resize(n);
+      for (size_t i = 0; i < n; ++i) {
+        Tensor& grad = grads[i];
+        if (!lies_as(grad, params[i]) || grad.is_neg()) {
+          Tensor copy = at::empty_strided(params[i].sizes(), params[i].strides(), grad.options());
+          copy.copy_(grad.detach());
+          grad = copy;
+        }
+        numel[i] = params[i].numel();
+        g[i] = grad.const_data_ptr();
+        at[0][i] = params[i].mutable_data_ptr();
+        for (int k = 0; k < (eight ? 4 : 2); ++k) at[1 + k][i] = states[k][i].mutable_data_ptr();
+      }
+      std::vector<int*> counter(counters.size());
+      for (size_t i = 0; i < counters.size(); ++i) counter[i] = (int*)counters[i].mutable_data_ptr();
+      Tensor scratch;
+      const size_t bytes = adamw_workspace_entry((int)n, !counters.empty());
+      if (bytes > 0) scratch = at::empty({(int64_t)bytes}, params[0].options().dtype(at::kByte).requires_grad(false));
+      status = adamw_entry((int)n, numel.data(), adamw_type(type), eight ? 8 : 32, at[0].data(), g.data(), at[1].data(),
+                           at[2].data(), eight ? (float* const*)at[3].data() : nullptr,
+                           eight ? (float* const*)at[4].data() : nullptr, steps.empty() ? nullptr : steps.data(),
+                           counters.empty() ? nullptr : counter.data(), lr,
+                           rate.defined() ? (const float*)rate.const_data_ptr() : nullptr, beta1, beta2, eps, decay,
+                           (unsigned)seed, scratch.defined() ? scratch.mutable_data_ptr() : nullptr, bytes,
+                           c10::hip::getCurrentHIPStream(device.index()).stream());
+    }
+    TORCH_CHECK(status == KFAC_OK, "kfac_adamw_batched failed (code ", status, ")");
+    // (a graph from before the update that goes through these is refused by its backward pass)
+    for (const Tensor& t : written) t.unsafeGetTensorImpl()->bump_version();
+    Py_RETURN_TRUE;
+  } catch (...) {
+    torch::translate_exception_to_python(std::current_exception());      // (each as torch's own calls raise it)
+    return nullptr;
+  }
+}

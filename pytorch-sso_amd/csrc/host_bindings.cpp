@@ -22,6 +22,9 @@ PyObject* host_bind_norm(PyObject*, PyObject* const*, Py_ssize_t);
 PyObject* host_rms_norm(PyObject*, PyObject* const*, Py_ssize_t);
 PyObject* host_bind_layer_norm(PyObject*, PyObject* const*, Py_ssize_t);
 PyObject* host_layer_norm(PyObject*, PyObject* const*, Py_ssize_t);
+// (host_adamw.cpp)
+PyObject* host_bind_adamw(PyObject*, PyObject* const*, Py_ssize_t);
+PyObject* host_adamw(PyObject*, PyObject* const*, Py_ssize_t);
 
 namespace {
 
@@ -386,6 +389,9 @@ PyMethodDef methods[] = {
     {"bind_layer_norm", KFAC_FAST(host_bind_layer_norm),
      "bind_layer_norm(norm, workspace, backward): the library's entry points"},
     {"layer_norm", KFAC_FAST(host_layer_norm), "layer_norm(x, residual, gain, bias, eps, curvature, eight), or None"},
+    {"bind_adamw", KFAC_FAST(host_bind_adamw), "bind_adamw(update, workspace): the library's entry points"},
+    {"adamw", KFAC_FAST(host_adamw),
+     "adamw(params, grads, m, v, m_scales, v_scales, steps, lr, beta1, beta2, eps, weight_decay, seed): done"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,

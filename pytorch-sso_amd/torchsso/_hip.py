@@ -25,6 +25,7 @@ _lock = threading.Lock()
 c_int = ctypes.c_int
 c_i64 = ctypes.c_int64
 c_f32 = ctypes.c_float
+c_f64 = ctypes.c_double
 c_ptr = ctypes.c_void_p
 c_size = ctypes.c_size_t
 
@@ -135,6 +136,9 @@ _SIGNATURES = {
                                            c_int, c_ptr, c_size, c_ptr]),
     'kfac_muon_update_batched': (c_int, [c_int, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
                                          c_f32, c_int, c_int, c_ptr, c_f32, c_int, c_ptr, c_size, c_ptr]),
+    'kfac_adamw_workspace_bytes': (c_size, [c_int, c_int]),
+    'kfac_adamw_batched': (c_int, [c_int, c_ptr, c_int, c_int] + [c_ptr] * 8 + [c_f64, c_ptr] + [c_f64] * 4
+                           + [ctypes.c_uint, c_ptr, c_size, c_ptr]),
     'kfac_rms_norm': (c_int, [c_int, c_int, c_i64, c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_f32,
                               c_ptr, c_ptr, c_ptr, c_ptr]),
     'kfac_rms_norm_backward_workspace_bytes': (c_size, [c_int, c_i64, c_int, c_int, c_int]),
@@ -224,6 +228,8 @@ def load():
             'kfac_rms_norm', 'kfac_rms_norm_backward_workspace_bytes', 'kfac_rms_norm_backward')])
         _host.bind_layer_norm(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             'kfac_layer_norm', 'kfac_layer_norm_backward_workspace_bytes', 'kfac_layer_norm_backward')])
+        _host.bind_adamw(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            'kfac_adamw_batched', 'kfac_adamw_workspace_bytes')])
         _lib = lib
     return _lib
 

@@ -901,6 +901,79 @@ def muon_update_batched(params, grads, buffers, step_sizes, keeps, momentum, nes
     _hip.check(st, 'kfac_muon_update_batched')
 
 
+STATE_BLOCK = 128            # elements of an 8-bit state that share a scale
+
+
+def _check_on(t, dtype, device, what):
+    if not isinstance(t, torch.Tensor):
+        raise _hip.KfacHipError('%s: expected a torch.Tensor' % what)
+    if not t.is_cuda:
+        raise _hip.KfacHipError('%s is on %s: the kernels run on a HIP device only '
+                                '(no CPU path exists in this package)' % (what, t.device))
+    if t.device != device:
+        raise _hip.KfacHipError('%s is on %s, expected %s' % (what, t.device, device))
+    if t.dtype != dtype:
+        raise _hip.KfacHipError('%s has dtype %s, expected %s' % (what, t.dtype, dtype))
+
+
+def _strides(t):
+    return [s for s, n in zip(t.stride(), t.shape) if n > 1]
+
+
+def _check_adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr):
+    """Raises what is wrong with the arguments of an update."""
+    first = params[0]
+    device = first.device
+    _element_type(first, 'parameter 0')
+    eight = m_scales is not None
+    for i, (p, g, m, v) in enumerate(zip(params, grads, ms, vs)):
+        _check_on(p, first.dtype, device, 'parameter %d' % i)
+        if not torch._C._has_storage(p) or not torch.ops.aten.is_non_overlapping_and_dense(p):
+            raise _hip.KfacHipError('the elements of parameter %d do not lie side by side' % i)
+        _check_on(g, first.dtype, device, 'gradient %d' % i)
+        if g.shape != p.shape:
+            raise _hip.KfacHipError('gradient %d has shape %s, expected %s' % (i, tuple(g.shape), tuple(p.shape)))
+        types = (torch.float8_e4m3fn, torch.float8_e5m2) if eight else (torch.float32, torch.float32)
+        for t, dtype, what in ((m, types[0], 'first moment'), (v, types[1], 'second moment')):
+            _check_on(t, dtype, device, '%s %d' % (what, i))
+            if t.shape != p.shape or (p.numel() > 0 and _strides(t) != _strides(p)):
+                raise _hip.KfacHipError('%s %d of shape %s and strides %s does not lie in memory as its parameter, %s and %s'
+                                        % (what, i, tuple(t.shape), t.stride(), tuple(p.shape), p.stride()))
+        if eight:
+            want = (-(-p.numel() // STATE_BLOCK),)
+            for t, what in ((m_scales[i], "first moment's scale"), (v_scales[i], "second moment's scale")):
+                _hip.typed_ptr(t, torch.float32, device, '%s %d' % (what, i))
+                if tuple(t.shape) != want:
+                    raise _hip.KfacHipError('%s %d has shape %s, expected %s' % (what, i, tuple(t.shape), want))
+    on_device = isinstance(steps, (list, tuple)) and any(isinstance(t, torch.Tensor) for t in steps)
+    if on_device:
+        for i, t in enumerate(steps):
+            _check_on(t, torch.int32, device, 'step %d' % i)
+            if t.numel() != 1:
+                raise _hip.KfacHipError('step %d has shape %s, expected one number' % (i, tuple(t.shape)))
+    if isinstance(lr, torch.Tensor):
+        if not on_device:
+            raise _hip.KfacHipError('a learning rate on the device needs steps on the device')
+        _check_on(lr, torch.float32, device, 'learning rate')
+        if lr.numel() != 1:
+            raise _hip.KfacHipError('the learning rate has shape %s, expected one number' % (tuple(lr.shape),))
+    written = [t for ts in (params, ms, vs, m_scales or (), v_scales or (), steps if on_device else ()) for t in ts
+               if t.numel() > 0]
+    ranges = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written)
+    if any(b[0] < a[1] for a, b in zip(ranges, ranges[1:])):
+        raise _hip.KfacHipError('parameters, states or steps share memory, or one is in the list twice')
+    raise _hip.KfacHipError('adamw cannot take these arguments')
+
+
+def adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr, beta1, beta2, eps, weight_decay, seed):
+    """AdamW's update of a list of tensors of one type in place (csrc/host_adamw.cpp); m_scales, v_scales: None where
+    the states are float32.  steps: a number, a number each, or an int32 tensor each."""
+    _hip.load()
+    if len(params) > 0 and not _hip._host.adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr, beta1, beta2, eps,
+                                                weight_decay, seed):
+        _check_adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr)
+
+
 def _rows(t, dim):
     """(2-D tensor [rows, dim] with its elements of a row side by side, elements between rows)."""
     t = t.reshape(-1, dim)
