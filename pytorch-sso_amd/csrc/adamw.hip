@@ -26,7 +26,7 @@ constexpr int ADAM_ROUND = ADAM_THREADS * UNIT;      // elements that a workgrou
 constexpr int ADAM_ROUNDS = 2;                       // ... how many times
 constexpr long ADAM_GROUP = (long)ADAM_ROUND * ADAM_ROUNDS;
 constexpr long ADAM_MOST_GROUPS = (1L << 32) / ADAM_THREADS - 1;      // a launch has fewer than 2^32 threads
-constexpr float LARGEST_M = 448.f, LARGEST_V = 57344.f;
+constexpr float LARGEST_M = 448.f, LARGEST_V = 57344.f, LEAST_V = 0x1p-16f;
 // A block whose largest number is below this is kept as zeros (its reciprocal scale would overflow).
 constexpr float LEAST_TOP = 0x1p-100f;
 constexpr unsigned INFINITE = 0x7f800000u;
@@ -87,18 +87,24 @@ __device__ __forceinline__ unsigned next_word(unsigned x) {
 
 // ---- 8-bit states ----------------------------------------------------------
 
-// a >= 0 to one of its two neighbours by 16 random bits: they are added below the last bit that is kept, below the type's
-// normal numbers (of exponent field LOWEST in float32) to a in units of 2^-16 of their steps.
-template <int DROPPED, int LOWEST, int TOP>
-__device__ __forceinline__ unsigned round_at_random(float a, unsigned random16) {
-  constexpr unsigned below = ((unsigned)LOWEST - 1) << (23 - DROPPED);
-  const float per_step = __uint_as_float((unsigned)(127 - LOWEST + 127 + 23 - DROPPED + 16) << 23);
-  const unsigned normal = ((__float_as_uint(a) + (random16 << (DROPPED - 16))) >> DROPPED) - below;
-  const unsigned small = ((unsigned)(a * per_step) + random16) >> 16;
-  return min(__float_as_uint(a) < (unsigned)LOWEST << 23 ? small : normal, (unsigned)TOP);
+// x to one of its two neighbours, four numbers into a word: the instructions add the upper 20 (e4m3) or 21 bits (e5m2) of
+// a random word below the last bit that is kept, also among the numbers below the type's normal ones (all 2^16
+// random numbers compared with that formula).  Of those the upper 16 are random and the others 0, so that a number some
+// last bits above the largest one, as the reciprocal of the scale may make it, stays that.
+template <int BYTE>
+__device__ __forceinline__ int encode_m(float x, unsigned word, int into) {
+  return __builtin_amdgcn_cvt_sr_fp8_f32(x, word & 0xffff0000u, into, BYTE);
 }
-__device__ __forceinline__ unsigned encode_m(float a, unsigned random16) { return round_at_random<20, 121, 0x7e>(a, random16); }
-__device__ __forceinline__ unsigned encode_v(float a, unsigned random16) { return round_at_random<21, 113, 0x7b>(a, random16); }
+template <int BYTE>
+__device__ __forceinline__ int encode_v(float x, unsigned word, int into) {
+  return __builtin_amdgcn_cvt_sr_bf8_f32(x, word << 16, into, BYTE);
+}
+template <int BYTE>
+__device__ __forceinline__ void encode(const float (&m)[UNIT], const float (&v)[UNIT], int k, unsigned& word, int& mq, int& vq) {
+  mq = encode_m<BYTE>(m[4 * k + BYTE], word, mq);
+  vq = encode_v<BYTE>(v[4 * k + BYTE], word, vq);
+  word = next_word(word);
+}
 
 __device__ __forceinline__ void decode_m(uint2 q, float (&x)[UNIT]) {
 #pragma unroll
@@ -159,13 +165,17 @@ __device__ __forceinline__ void store_all(V* p, const float (&v)[N]) {
 
 // (m and v without fused products: an 8-bit state that is off by a bit before it is rounded may become another
 // number, and this is the sequence that the formula has in float32 operations)
+// FAST: root and reciprocal by the instructions alone, 2^-23 off, of numbers that are not below 2^-126 where it matters
+// (with states in 8 bits eps is at least 1e-12).
+template <bool FAST>
 __device__ __forceinline__ void update(const AdamRates& r, const AdamScalars& s, float g, float& p, float& m, float& v) {
   {
 #pragma clang fp contract(off)
     m = r.b1 * m + r.c1 * g;
     v = r.b2 * v + r.c2 * g * g;
   }
-  p = fmaf(p, s.keep, -s.size * (m / fmaf(sqrtf(v), s.root, r.eps)));
+  if (FAST) p = fmaf(p, s.keep, -s.size * m * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(v), s.root, r.eps)));
+  else p = fmaf(p, s.keep, -s.size * (m / fmaf(sqrtf(v), s.root, r.eps)));
 }
 
 // Elements i ... i + 7 of a tensor, `have` of them (8 where all streams can be accessed 16 bytes at a time: whole).
@@ -182,14 +192,14 @@ __device__ __forceinline__ void update_unit(const AdamTensor<32>& t, const AdamS
     load_all<float, UNIT>(mp, m);
     load_all<float, UNIT>(vp, v);
 #pragma unroll
-    for (int e = 0; e < UNIT; ++e) update(r, s, g[e], p[e], m[e], v[e]);
+    for (int e = 0; e < UNIT; ++e) update<false>(r, s, g[e], p[e], m[e], v[e]);
     store_all<V, UNIT>(pp, p);
     store_all<float, UNIT>(mp, m);
     store_all<float, UNIT>(vp, v);
   } else {
     for (int e = 0; e < have; ++e) {
       float p = Element<V>::get(pp[e]), m = mp[e], v = vp[e];
-      update(r, s, Element<V>::get(gp[e]), p, m, v);
+      update<false>(r, s, Element<V>::get(gp[e]), p, m, v);
       pp[e] = Element<V>::put(p);
       mp[e] = m;
       vp[e] = v;
@@ -234,7 +244,7 @@ __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamSc
   for (int e = 0; e < UNIT; ++e) {
     m[e] *= m_scale;
     v[e] *= v_scale;
-    update(r, s, g[e], p[e], m[e], v[e]);
+    update<true>(r, s, g[e], p[e], m[e], v[e]);
     top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
     top_v = max(top_v, __float_as_uint(v[e]));
   }
@@ -263,24 +273,27 @@ __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamSc
   float m_inverse, v_inverse;
   block_scale(top_m, LARGEST_M, m_scale, m_inverse);
   block_scale(top_v, LARGEST_V, v_scale, v_inverse);
-  if (odd && v_scale == 0.f) v_scale = 1.f;          // (an infinite v stays one)
-  unsigned word = mix(s.key + (unsigned)(i / UNIT));
-  mq = vq = make_uint2(0, 0);
+  // a v above 0 is at least the smallest number
+  const float least = v_inverse > 0.f ? LEAST_V : 0.f;
+  if (odd && v_scale == 0.f) {                       // (an infinite v stays one beside zeros)
+    v_scale = 1.f;
+    v_inverse = 0x1p-126f;
+  }
 #pragma unroll
   for (int e = 0; e < UNIT; ++e) {
-    const unsigned bits = __float_as_uint(m[e]), v_bits = __float_as_uint(v[e]);
-    unsigned cm = encode_m(fabsf(m[e]) * m_inverse, word >> 16);
-    unsigned cv = encode_v(v[e] * v_inverse, word & 0xffffu);
-    if (v_inverse > 0.f) cv = max(cv, min(v_bits, 1u));
-    if (odd) {
-      // (e4m3 has no infinity)
-      if ((bits & 0x7fffffffu) >= INFINITE) cm = 0x7f;
-      if (v_bits >= INFINITE) cv = v_bits == INFINITE ? 0x7c : 0x7f;
-    }
-    cm |= bits >> 24 & 0x80u;
-    (e < 4 ? mq.x : mq.y) |= cm << (8 * (e & 3));
-    (e < 4 ? vq.x : vq.y) |= cv << (8 * (e & 3));
-    word = next_word(word);
+    m[e] *= m_inverse;
+    v[e] = v[e] > 0.f ? fmaxf(v[e] * v_inverse, least) : v[e];
+  }
+  unsigned word = mix(s.key + (unsigned)(i / UNIT));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    int mw = 0, vw = 0;
+    encode<0>(m, v, k, word, mw, vw);
+    encode<1>(m, v, k, word, mw, vw);
+    encode<2>(m, v, k, word, mw, vw);
+    encode<3>(m, v, k, word, mw, vw);
+    (k ? mq.y : mq.x) = (unsigned)mw;
+    (k ? vq.y : vq.x) = (unsigned)vw;
   }
   if (whole) {
     *(uint2*)mp = mq;
