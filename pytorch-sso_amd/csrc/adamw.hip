@@ -13,6 +13,8 @@
 // Bound by memory: 3 s + 16 bytes an element with states in 32 bits (s: a parameter's), 3 s + 4.25 in 8.  A thread takes
 // 8 consecutive elements, so 16 threads hold a block, and every stream is read and written once, 16 bytes at a time (8
 // of an 8-bit state).  The list travels as a kernel argument, as that of the other element-wise passes (elementwise.hip).
+// 244 million bfloat16 parameters: 958 us in 32 bits, 5.6 TB/s, and 390 in 8, 6.3, where a large copy reaches 5.2; a
+// ResNet-50 in float32 143 us, 5.0 TB/s.  With twice and four times the elements to a workgroup the last takes 146 and 151.
 #include <cmath>
 
 #include "common.h"
@@ -22,9 +24,7 @@ namespace kfac {
 namespace {
 
 constexpr int ADAM_THREADS = 256, UNIT = 8, BLOCK = 128, LANES = BLOCK / UNIT;
-constexpr int ADAM_ROUND = ADAM_THREADS * UNIT;      // elements that a workgroup takes at a time
-constexpr int ADAM_ROUNDS = 2;                       // ... how many times
-constexpr long ADAM_GROUP = (long)ADAM_ROUND * ADAM_ROUNDS;
+constexpr long ADAM_GROUP = ADAM_THREADS * UNIT;     // elements of a workgroup
 constexpr long ADAM_MOST_GROUPS = (1L << 32) / ADAM_THREADS - 1;      // a launch has fewer than 2^32 threads
 constexpr float LARGEST_M = 448.f, LARGEST_V = 57344.f, LEAST_V = 0x1p-16f;
 // A block whose largest number is below this is kept as zeros (its reciprocal scale would overflow).
@@ -34,7 +34,7 @@ constexpr unsigned INFINITE = 0x7f800000u;
 // What depends on the number of the update
 struct AdamScalars {
   float keep, size, root;                 // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
-  unsigned key;                           // of the tensor's random numbers
+  unsigned key;                           // of its random numbers
 };
 struct AdamRates {
   float b1, c1, b2, c2, eps;              // c: 1 - b
@@ -45,25 +45,29 @@ template <> struct AdamTensor<32> {
   void *p, *m, *v;
   const void* g;
   long n;
-  AdamScalars s;
 };
 template <> struct AdamTensor<8> {
   void *p, *m, *v;
   const void* g;
   float *m_scale, *v_scale;
   long n;
-  AdamScalars s;
 };
 
-constexpr int ADAM_SHORT = 8, ADAM_LONG = 48;
+// Tensors of a launch.  A launch more costs 5 us and the end of another one: all of a ResNet-50 in two launches of up
+// to 80 150 us, in four of up to 48 156.  The numbers of their updates are few as a rule, and are kept apart.
+constexpr int ADAM_SHORT = 8, ADAM_SETS = 8;
+template <int BITS> constexpr int adam_long() { return BITS == 32 ? 80 : 60; }
 template <int BITS, int N>
 struct AdamList {
   AdamTensor<BITS> d[N];
   int first[N + 1];                       // workgroup of each
-  int n;
-  const AdamScalars* scalars;             // on the device: in the place of those above
+  int n, index;                           // of the launch's first tensor in the call
+  const AdamScalars* scalars;             // on the device, one for each tensor: in the place of the sets
+  AdamScalars sets[ADAM_SETS];
+  unsigned char set[N];
 };
-static_assert(sizeof(AdamList<8, ADAM_LONG>) + sizeof(AdamRates) <= 4096, "kernel arguments");
+static_assert(sizeof(AdamList<8, adam_long<8>()>) + sizeof(AdamRates) <= 4096, "kernel arguments");
+static_assert(sizeof(AdamList<32, adam_long<32>()>) + sizeof(AdamRates) <= 4096, "kernel arguments");
 
 // ---- random numbers --------------------------------------------------------
 
@@ -76,14 +80,15 @@ __host__ __device__ inline unsigned mix(unsigned x) {
   x *= 0xB504F333u;
   return x ^ (x >> 16);
 }
-__host__ __device__ inline unsigned tensor_key(unsigned seed, unsigned step, unsigned index) {
-  return mix(mix(mix(seed) + step) + index);
-}
+__host__ __device__ inline unsigned update_key(unsigned seed, unsigned step) { return mix(mix(seed) + step); }
 __device__ __forceinline__ unsigned next_word(unsigned x) {
   x ^= x << 13;
   x ^= x >> 17;
   return x ^ (x << 5);
 }
+
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 // ---- 8-bit states ----------------------------------------------------------
 
@@ -106,18 +111,18 @@ __device__ __forceinline__ void encode(const float (&m)[UNIT], const float (&v)[
   word = next_word(word);
 }
 
-__device__ __forceinline__ void decode_m(uint2 q, float (&x)[UNIT]) {
+__device__ __forceinline__ void decode_m(u2 q, float (&x)[UNIT]) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int w = (int)(k ? q.y : q.x);
+    const int w = (int)q[k];
     const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
     x[4 * k] = low[0], x[4 * k + 1] = low[1], x[4 * k + 2] = high[0], x[4 * k + 3] = high[1];
   }
 }
-__device__ __forceinline__ void decode_v(uint2 q, float (&x)[UNIT]) {
+__device__ __forceinline__ void decode_v(u2 q, float (&x)[UNIT]) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int w = (int)(k ? q.y : q.x);
+    const int w = (int)q[k];
     const auto low = __builtin_amdgcn_cvt_pk_f32_bf8(w, false), high = __builtin_amdgcn_cvt_pk_f32_bf8(w, true);
     x[4 * k] = low[0], x[4 * k + 1] = low[1], x[4 * k + 2] = high[0], x[4 * k + 3] = high[1];
   }
@@ -141,30 +146,40 @@ __device__ __forceinline__ void block_scale(unsigned top_bits, float largest, fl
 
 // ---- the update --------------------------------------------------------------
 
-template <class V, int N>
-__device__ __forceinline__ void load_all(const V* p, float (&v)[N]) {
-  constexpr int E = 16 / sizeof(V) < N ? 16 / sizeof(V) : N;
+// ONCE: past the caches.  States in 8 bits of calls that access more than the last cache holds: 244 million bfloat16
+// parameters 435 us without that, 390 with it.  (In 32 bits it costs: 958 and 977.)
+constexpr double LAST_CACHE = 256. * (1 << 20);
+template <bool ONCE, class W>
+__device__ __forceinline__ W access_load(const void* p) {
+  return ONCE ? __builtin_nontemporal_load((const W*)p) : *(const W*)p;
+}
+template <bool ONCE, class W>
+__device__ __forceinline__ void access_store(void* p, W w) {
+  if (ONCE) __builtin_nontemporal_store(w, (W*)p);
+  else *(W*)p = w;
+}
+template <bool ONCE, class V>
+__device__ __forceinline__ void load_unit(const V* p, float (&v)[UNIT]) {
+  constexpr int E = 16 / sizeof(V);
 #pragma unroll
-  for (int i = 0; i < N; i += E) {
-    const Pack<V, E> a = *(const Pack<V, E>*)(p + i);
+  for (int i = 0; i < UNIT; i += E) {
+    const Pack<V, E> a = __builtin_bit_cast(Pack<V, E>, access_load<ONCE, u4>(p + i));
 #pragma unroll
     for (int e = 0; e < E; ++e) v[i + e] = Element<V>::get(a.v[e]);
   }
 }
-template <class V, int N>
-__device__ __forceinline__ void store_all(V* p, const float (&v)[N]) {
-  constexpr int E = 16 / sizeof(V) < N ? 16 / sizeof(V) : N;
+template <bool ONCE, class V>
+__device__ __forceinline__ void store_unit(V* p, const float (&v)[UNIT]) {
+  constexpr int E = 16 / sizeof(V);
 #pragma unroll
-  for (int i = 0; i < N; i += E) {
+  for (int i = 0; i < UNIT; i += E) {
     Pack<V, E> a;
 #pragma unroll
     for (int e = 0; e < E; ++e) a.v[e] = Element<V>::put(v[i + e]);
-    *(Pack<V, E>*)(p + i) = a;
+    access_store<ONCE>(p + i, __builtin_bit_cast(u4, a));
   }
 }
 
-// (m and v without fused products: an 8-bit state that is off by a bit before it is rounded may become another
-// number, and this is the sequence that the formula has in float32 operations)
 // FAST: root and reciprocal by the instructions alone, 2^-23 off, of numbers that are not below 2^-126 where it matters
 // (with states in 8 bits eps is at least 1e-12).
 template <bool FAST>
@@ -179,7 +194,7 @@ __device__ __forceinline__ void update(const AdamRates& r, const AdamScalars& s,
 }
 
 // Elements i ... i + 7 of a tensor, `have` of them (8 where all streams can be accessed 16 bytes at a time: whole).
-template <class V>
+template <bool ONCE, class V>
 __device__ __forceinline__ void update_unit(const AdamTensor<32>& t, const AdamScalars& s, const AdamRates& r, long i, int have,
                                             bool whole) {
   V* const pp = (V*)t.p + i;
@@ -187,15 +202,15 @@ __device__ __forceinline__ void update_unit(const AdamTensor<32>& t, const AdamS
   float *const mp = (float*)t.m + i, *const vp = (float*)t.v + i;
   if (whole) {
     float p[UNIT], g[UNIT], m[UNIT], v[UNIT];
-    load_all<V, UNIT>(gp, g);
-    load_all<V, UNIT>(pp, p);
-    load_all<float, UNIT>(mp, m);
-    load_all<float, UNIT>(vp, v);
+    load_unit<ONCE>(gp, g);
+    load_unit<ONCE>(pp, p);
+    load_unit<ONCE>(mp, m);
+    load_unit<ONCE>(vp, v);
 #pragma unroll
     for (int e = 0; e < UNIT; ++e) update<false>(r, s, g[e], p[e], m[e], v[e]);
-    store_all<V, UNIT>(pp, p);
-    store_all<float, UNIT>(mp, m);
-    store_all<float, UNIT>(vp, v);
+    store_unit<ONCE>(pp, p);
+    store_unit<ONCE>(mp, m);
+    store_unit<ONCE>(vp, v);
   } else {
     for (int e = 0; e < have; ++e) {
       float p = Element<V>::get(pp[e]), m = mp[e], v = vp[e];
@@ -207,24 +222,24 @@ __device__ __forceinline__ void update_unit(const AdamTensor<32>& t, const AdamS
   }
 }
 
-template <class V>
+template <bool ONCE, class V>
 __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamScalars& s, const AdamRates& r, long i, int have,
                                             bool whole) {
   V* const pp = (V*)t.p + i;
   const V* const gp = (const V*)t.g + i;
   unsigned char *const mp = (unsigned char*)t.m + i, *const vp = (unsigned char*)t.v + i;
   float p[UNIT], g[UNIT], m[UNIT], v[UNIT];
-  uint2 mq = make_uint2(0, 0), vq = make_uint2(0, 0);
+  u2 mq = {0, 0}, vq = {0, 0};
   float m_scale = 0.f, v_scale = 0.f;
   if (have > 0) {
     m_scale = t.m_scale[i / BLOCK];
     v_scale = t.v_scale[i / BLOCK];
   }
   if (whole) {
-    load_all<V, UNIT>(gp, g);
-    load_all<V, UNIT>(pp, p);
-    mq = *(const uint2*)mp;
-    vq = *(const uint2*)vp;
+    load_unit<ONCE>(gp, g);
+    load_unit<ONCE>(pp, p);
+    mq = access_load<ONCE, u2>(mp);
+    vq = access_load<ONCE, u2>(vp);
   } else {
 #pragma unroll
     for (int e = 0; e < UNIT; ++e) {
@@ -232,8 +247,8 @@ __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamSc
       if (e < have) {
         p[e] = Element<V>::get(pp[e]);
         g[e] = Element<V>::get(gp[e]);
-        (e < 4 ? mq.x : mq.y) |= (unsigned)mp[e] << (8 * (e & 3));
-        (e < 4 ? vq.x : vq.y) |= (unsigned)vp[e] << (8 * (e & 3));
+        mq[e / 4] |= (unsigned)mp[e] << (8 * (e & 3));
+        vq[e / 4] |= (unsigned)vp[e] << (8 * (e & 3));
       }
     }
   }
@@ -249,7 +264,7 @@ __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamSc
     top_v = max(top_v, __float_as_uint(v[e]));
   }
   if (whole) {
-    store_all<V, UNIT>(pp, p);
+    store_unit<ONCE>(pp, p);
   } else {
 #pragma unroll
     for (int e = 0; e < UNIT; ++e)
@@ -292,18 +307,18 @@ __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamSc
     encode<1>(m, v, k, word, mw, vw);
     encode<2>(m, v, k, word, mw, vw);
     encode<3>(m, v, k, word, mw, vw);
-    (k ? mq.y : mq.x) = (unsigned)mw;
-    (k ? vq.y : vq.x) = (unsigned)vw;
+    mq[k] = (unsigned)mw;
+    vq[k] = (unsigned)vw;
   }
   if (whole) {
-    *(uint2*)mp = mq;
-    *(uint2*)vp = vq;
+    access_store<ONCE>(mp, mq);
+    access_store<ONCE>(vp, vq);
   } else {
 #pragma unroll
     for (int e = 0; e < UNIT; ++e)
       if (e < have) {
-        mp[e] = (unsigned char)((e < 4 ? mq.x : mq.y) >> (8 * (e & 3)));
-        vp[e] = (unsigned char)((e < 4 ? vq.x : vq.y) >> (8 * (e & 3)));
+        mp[e] = (unsigned char)(mq[e / 4] >> (8 * (e & 3)));
+        vp[e] = (unsigned char)(vq[e / 4] >> (8 * (e & 3)));
       }
   }
   if (have > 0 && i % BLOCK == 0) {
@@ -318,7 +333,7 @@ __device__ __forceinline__ bool accesses_whole(const AdamTensor<BITS>& t) {
   return ((wide | (BITS == 32 ? states : 0)) & 15) == 0 && (states & 7) == 0;
 }
 
-template <class V, int BITS, int N>
+template <class V, int BITS, int N, bool ONCE>
 __global__ __launch_bounds__(ADAM_THREADS) void adamw_kernel(const AdamList<BITS, N> list, const AdamRates r) {
   int j = 0, end = list.n;
   while (end - j > 1) {
@@ -326,19 +341,26 @@ __global__ __launch_bounds__(ADAM_THREADS) void adamw_kernel(const AdamList<BITS
     if (list.first[mid] <= (int)blockIdx.x) j = mid; else end = mid;
   }
   const AdamTensor<BITS> t = list.d[j];
-  const AdamScalars s = list.scalars ? list.scalars[j] : t.s;
-  const bool whole = accesses_whole<BITS>(t);
-  const long from = (long)((int)blockIdx.x - list.first[j]) * ADAM_GROUP;
-#pragma unroll
-  for (int k = 0; k < ADAM_ROUNDS; ++k) {
-    const long i = from + k * ADAM_ROUND + (long)threadIdx.x * UNIT;
-    const int have = (int)min(max(t.n - i, 0L), (long)UNIT);
-    // (in 8 bits a block's threads go on together)
-    if (BITS == 32 ? have > 0 : i / BLOCK * BLOCK < t.n) update_unit<V>(t, s, r, i, have, whole && have == UNIT);
-  }
+  AdamScalars s = list.scalars ? list.scalars[j] : list.sets[list.set[j]];
+  if (BITS == 8) s.key = mix(s.key + (unsigned)(list.index + j));
+  const long i = (long)((int)blockIdx.x - list.first[j]) * ADAM_GROUP + (long)threadIdx.x * UNIT;
+  const int have = (int)min(max(t.n - i, 0L), (long)UNIT);
+  // (in 8 bits a block's threads go on together)
+  if (BITS == 32 ? have > 0 : i / BLOCK * BLOCK < t.n)
+    update_unit<ONCE, V>(t, s, r, i, have, have == UNIT && accesses_whole<BITS>(t));
 }
 
 // ---- numbers of the update on the device -----------------------------------------
+
+__host__ __device__ inline AdamScalars scalars_of(double t, unsigned step, double lr, double b1, double b2, double decay,
+                                                  unsigned seed) {
+  AdamScalars s;
+  s.keep = (float)(1. - lr * decay);
+  s.size = (float)(lr / (b1 > 0. ? -expm1(t * log(b1)) : 1.));
+  s.root = (float)(1. / sqrt(b2 > 0. ? -expm1(t * log(b2)) : 1.));
+  s.key = update_key(seed, step);
+  return s;
+}
 
 struct AdamCounters {
   int* step[256];
@@ -352,34 +374,47 @@ __global__ __launch_bounds__(256) void adamw_scalars_kernel(const AdamCounters c
   const int t = *c.step[i] + 1;
   *c.step[i] = t;
   if (lr_on_device) lr = (double)*lr_on_device;
-  AdamScalars s;
-  s.keep = (float)(1. - lr * decay);
-  s.size = (float)(lr / (b1 > 0. ? -expm1((double)t * log(b1)) : 1.));
-  s.root = (float)(1. / sqrt(b2 > 0. ? -expm1((double)t * log(b2)) : 1.));
-  s.key = tensor_key(seed, (unsigned)t, (unsigned)(first + i));
-  out[first + i] = s;
+  out[first + i] = scalars_of((double)t, (unsigned)t, lr, b1, b2, decay, seed);
 }
 
 long groups_of(int64_t elements) { return ((long)elements + ADAM_GROUP - 1) / ADAM_GROUP; }
 
 struct AdamCall {
-  int count, type;
-  const int64_t* numel;
+  int count;
+  const int64_t *numel, *steps;
   void *const *params, *const *m, *const *v;
   const void* const* grads;
   float *const *m_scales, *const *v_scales;
+  const AdamScalars* scalars;             // on the device, where there are no steps
+  double lr, beta1, beta2, decay;
+  unsigned seed;
   AdamRates rates;
+  bool once;
 };
 
+// The tensors from `first` on, as many as a launch takes; how many those are.
 template <class V, int BITS, int N>
-void launch_adamw(const AdamCall& c, int first, int count, const AdamScalars* scalars, const AdamScalars* on_device,
-                  hipStream_t stream) {
+int launch_adamw(const AdamCall& c, int first, hipStream_t stream) {
   AdamList<BITS, N> list;
-  list.n = count;
-  list.first[0] = 0;
-  list.scalars = on_device ? on_device + first : nullptr;
-  for (int k = 0; k < count; ++k) {
+  list.n = list.first[0] = 0;
+  list.index = first;
+  list.scalars = c.scalars ? c.scalars + first : nullptr;
+  int sets = 0;
+  int64_t step[ADAM_SETS];
+  for (int k = 0; k < N && first + k < c.count; ++k) {
     const int i = first + k;
+    const long groups = groups_of(c.numel[i]);
+    if (k > 0 && list.first[k] + groups > ADAM_MOST_GROUPS) break;
+    if (c.steps) {
+      int at = 0;
+      while (at < sets && step[at] != c.steps[i]) ++at;
+      if (at == ADAM_SETS) break;
+      if (at == sets) {
+        step[sets] = c.steps[i];
+        list.sets[sets++] = scalars_of((double)c.steps[i], (unsigned)c.steps[i], c.lr, c.beta1, c.beta2, c.decay, c.seed);
+      }
+      list.set[k] = (unsigned char)at;
+    }
     AdamTensor<BITS>& t = list.d[k];
     t.p = c.params[i];
     t.g = c.grads[i];
@@ -390,19 +425,22 @@ void launch_adamw(const AdamCall& c, int first, int count, const AdamScalars* sc
       t.v_scale = c.v_scales[i];
     }
     t.n = (long)c.numel[i];
-    t.s = on_device ? AdamScalars{} : scalars[k];
-    list.first[k + 1] = list.first[k] + (int)groups_of(t.n);
+    list.first[k + 1] = list.first[k] + (int)groups;
+    ++list.n;
   }
-  if (list.first[count] > 0)
-    hipLaunchKernelGGL((adamw_kernel<V, BITS, N>), dim3((unsigned)list.first[count]), dim3(ADAM_THREADS), 0, stream, list, c.rates);
+  const dim3 grid((unsigned)list.first[list.n]), block(ADAM_THREADS);
+  if (grid.x > 0) {
+    if (BITS == 8 && c.once) hipLaunchKernelGGL((adamw_kernel<V, BITS, N, BITS == 8>), grid, block, 0, stream, list, c.rates);
+    else hipLaunchKernelGGL((adamw_kernel<V, BITS, N, false>), grid, block, 0, stream, list, c.rates);
+  }
+  return list.n;
 }
 
-template <int BITS, int N>
-void launch_adamw(const AdamCall& c, int first, int count, const AdamScalars* scalars, const AdamScalars* on_device,
-                  hipStream_t stream) {
-  if (c.type == TYPE_F32) launch_adamw<float, BITS, N>(c, first, count, scalars, on_device, stream);
-  else if (c.type == TYPE_BF16) launch_adamw<__hip_bfloat16, BITS, N>(c, first, count, scalars, on_device, stream);
-  else launch_adamw<_Float16, BITS, N>(c, first, count, scalars, on_device, stream);
+template <class V, int BITS>
+void launch_all(const AdamCall& c, hipStream_t stream) {
+  for (int first = 0; first < c.count;)
+    first += c.count - first <= ADAM_SHORT ? launch_adamw<V, BITS, ADAM_SHORT>(c, first, stream)
+                                           : launch_adamw<V, BITS, adam_long<BITS>()>(c, first, stream);
 }
 
 }  // namespace
@@ -429,8 +467,10 @@ int kfac_adamw_batched(int count, const int64_t* numel, int type, int state_bits
     return KFAC_ERR_ARG;
   constexpr int64_t most = ADAM_MOST_GROUPS * ADAM_GROUP;
   bool some = counters != nullptr;
+  double elements = 0.;
   for (int i = 0; i < count; ++i) {
     some = some || numel[i] > 0;
+    elements += (double)numel[i];
     if (numel[i] < 0 || numel[i] > most || (steps && steps[i] < 1)) return KFAC_ERR_ARG;
     if (numel[i] > 0 && (!params[i] || !grads[i] || !m[i] || !v[i] || (state_bits == 8 && (!m_scales[i] || !v_scales[i]))))
       return KFAC_ERR_ARG;
@@ -447,30 +487,13 @@ int kfac_adamw_batched(int count, const int64_t* numel, int type, int state_bits
     hipLaunchKernelGGL(adamw_scalars_kernel, dim3(1), dim3(256), 0, s, c, lr_on_device, lr, beta1, beta2, weight_decay, seed, first,
                        on_device);
   }
-  const AdamCall c{count, type, numel, params, m, v, grads, m_scales, v_scales,
-                   {(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps}};
-  for (int first = 0, n; first < count; first += n) {
-    long groups = groups_of(numel[first]);
-    for (n = 1; n < ADAM_LONG && first + n < count; ++n)
-      if ((groups += groups_of(numel[first + n])) > ADAM_MOST_GROUPS) break;
-    AdamScalars scalars[ADAM_LONG];
-    for (int k = 0; steps && k < n; ++k) {
-      const int64_t t = steps[first + k];
-      if (k > 0 && t == steps[first + k - 1]) {
-        scalars[k] = scalars[k - 1];
-      } else {
-        scalars[k].keep = (float)(1. - lr * weight_decay);
-        scalars[k].size = (float)(lr / (beta1 > 0. ? -std::expm1((double)t * std::log(beta1)) : 1.));
-        scalars[k].root = (float)(1. / std::sqrt(beta2 > 0. ? -std::expm1((double)t * std::log(beta2)) : 1.));
-      }
-      scalars[k].key = tensor_key(seed, (unsigned)t, (unsigned)(first + k));
-    }
-    const bool few = n <= ADAM_SHORT;
-    if (state_bits == 32) few ? launch_adamw<32, ADAM_SHORT>(c, first, n, scalars, on_device, s)
-                              : launch_adamw<32, ADAM_LONG>(c, first, n, scalars, on_device, s);
-    else few ? launch_adamw<8, ADAM_SHORT>(c, first, n, scalars, on_device, s)
-             : launch_adamw<8, ADAM_LONG>(c, first, n, scalars, on_device, s);
-  }
+  const AdamCall c{count, numel, steps, params, m, v, grads, m_scales, v_scales, on_device, lr, beta1, beta2, weight_decay, seed,
+                   {(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps},
+                   elements * (3 * type_size(type) + 4) > LAST_CACHE};
+  const bool wide = state_bits == 32;
+  if (type == TYPE_F32) wide ? launch_all<float, 32>(c, s) : launch_all<float, 8>(c, s);
+  else if (type == TYPE_BF16) wide ? launch_all<__hip_bfloat16, 32>(c, s) : launch_all<__hip_bfloat16, 8>(c, s);
+  else wide ? launch_all<_Float16, 32>(c, s) : launch_all<_Float16, 8>(c, s);
   return launch_status();
 }
 
