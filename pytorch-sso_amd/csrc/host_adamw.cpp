@@ -24,28 +24,41 @@ decltype(&kfac_adamw_batched) adamw_entry = nullptr;
 decltype(&kfac_adamw_workspace_bytes) adamw_workspace_entry = nullptr;
 
 constexpr int64_t STATE_BLOCK = 128;          // elements of an 8-bit state with one scale
+constexpr double LEAST_EPS_8 = 1e-12;         // of updates with such states
 
 int adamw_type(at::ScalarType t) {
   return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1;
 }
 
-// A list or tuple of tensors
+// `take(object, index)` for every object of a list or tuple; false where one of them is, or it is none
+template <class F>
+bool each_of(PyObject* o, F&& take) {
+  if (!PyList_Check(o) && !PyTuple_Check(o)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (!take(PySequence_Fast_GET_ITEM(o, i), i)) return false;
+  return true;
+}
 bool tensors_of(PyObject* o, std::vector<Tensor>& out) {
-  PyObject* const seq = PySequence_Fast(o, "expected a list or tuple");
-  if (!seq) {
-    PyErr_Clear();
-    return false;
-  }
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
-  out.reserve((size_t)n);
-  bool ok = true;
-  for (Py_ssize_t i = 0; ok && i < n; ++i) {
-    PyObject* const t = PySequence_Fast_GET_ITEM(seq, i);
-    ok = THPVariable_Check(t);
-    if (ok) out.push_back(THPVariable_Unpack(t));
-  }
-  Py_DECREF(seq);
-  return ok;
+  return each_of(o, [&](PyObject* t, Py_ssize_t) {
+    if (!THPVariable_Check(t)) return false;
+    out.push_back(THPVariable_Unpack(t));
+    return true;
+  });
+}
+// States: tensors, or (numbers, scales)
+bool states_of(PyObject* o, std::vector<Tensor>& numbers, std::vector<Tensor>& scales) {
+  return each_of(o, [&](PyObject* t, Py_ssize_t) {
+    if (THPVariable_Check(t)) {
+      numbers.push_back(THPVariable_Unpack(t));
+      return true;
+    }
+    std::vector<Tensor> both;
+    if (!tensors_of(t, both) || both.size() != 2) return false;
+    numbers.push_back(both[0]);
+    scales.push_back(both[1]);
+    return true;
+  });
 }
 
 bool strided_on(const Tensor& t, at::Device device, at::ScalarType type) {
@@ -93,45 +106,42 @@ PyObject* host_bind_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Py_RETURN_NONE;
 }
 
-// adamw(params, grads, m, v, scales of m or None, scales of v or None, steps (a number, a list of numbers or a list of
+// adamw(params, grads, m, v (tensors, or all of them (numbers, scales)), steps (a number, a list of numbers or a list of
 // tensors), lr (a number or a tensor), beta1, beta2, eps, weight decay, seed) -> True, or False
 PyObject* host_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 13) {
-    PyErr_SetString(PyExc_TypeError,
-                    "adamw(params, grads, m, v, m_scales, v_scales, steps, lr, beta1, beta2, eps, weight_decay, seed)");
+  if (nargs != 11) {
+    PyErr_SetString(PyExc_TypeError, "adamw(params, grads, m, v, steps, lr, beta1, beta2, eps, weight_decay, seed)");
     return nullptr;
   }
-  const bool lr_on_device = THPVariable_Check(args[7]);
-  const double lr = lr_on_device ? 0. : PyFloat_AsDouble(args[7]), beta1 = PyFloat_AsDouble(args[8]),
-               beta2 = PyFloat_AsDouble(args[9]), eps = PyFloat_AsDouble(args[10]), decay = PyFloat_AsDouble(args[11]);
-  const unsigned long long seed = PyLong_AsUnsignedLongLongMask(args[12]);
+  const bool lr_on_device = THPVariable_Check(args[5]);
+  const double lr = lr_on_device ? 0. : PyFloat_AsDouble(args[5]), beta1 = PyFloat_AsDouble(args[6]),
+               beta2 = PyFloat_AsDouble(args[7]), eps = PyFloat_AsDouble(args[8]), decay = PyFloat_AsDouble(args[9]);
+  const unsigned long long seed = PyLong_AsUnsignedLongLongMask(args[10]);
   if (PyErr_Occurred()) return nullptr;
   try {
-    const bool eight = args[4] != Py_None;
     std::vector<Tensor> params, grads, states[4], counters;
     if (!adamw_entry || !tensors_of(args[0], params) || !tensors_of(args[1], grads) || params.empty() ||
-        grads.size() != params.size())
+        !states_of(args[2], states[0], states[2]) || !states_of(args[3], states[1], states[3]))
       Py_RETURN_FALSE;
     const size_t n = params.size();
-    for (int k = 0; k < (eight ? 4 : 2); ++k)
-      if (!tensors_of(args[2 + k], states[k]) || states[k].size() != n) Py_RETURN_FALSE;
+    const bool eight = !states[2].empty();
+    if (grads.size() != n || states[0].size() != n || states[1].size() != n || states[2].size() != (eight ? n : 0) ||
+        states[3].size() != (eight ? n : 0) || (eight && !(eps >= LEAST_EPS_8)))
+      Py_RETURN_FALSE;
     const at::Device device = params[0].device();
     const at::ScalarType type = params[0].scalar_type();
     if (!params[0].is_cuda() || adamw_type(type) < 0) Py_RETURN_FALSE;
     // the numbers of the updates
     std::vector<int64_t> steps;
-    if (PyLong_Check(args[6])) {
-      steps.assign(n, PyLong_AsLongLong(args[6]));
-    } else if (!tensors_of(args[6], counters)) {
+    if (PyLong_Check(args[4])) {
+      steps.assign(n, PyLong_AsLongLong(args[4]));
+    } else if (!tensors_of(args[4], counters)) {
       counters.clear();
-      PyObject* const seq = PySequence_Fast(args[6], "expected a list or tuple");
-      if (!seq) {
-        PyErr_Clear();
+      if (!each_of(args[4], [&](PyObject* t, Py_ssize_t) {
+            steps.push_back(THPVariable_Check(t) ? 0 : PyLong_AsLongLong(t));
+            return true;
+          }))
         Py_RETURN_FALSE;
-      }
-      for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i)
-        steps.push_back(PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq, i)));
-      Py_DECREF(seq);
     }
     if (PyErr_Occurred()) {
       PyErr_Clear();
@@ -144,7 +154,7 @@ PyObject* host_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (!strided_on(t, device, at::kInt) || t.numel() != 1) Py_RETURN_FALSE;
     Tensor rate;
     if (lr_on_device) {
-      rate = THPVariable_Unpack(args[7]);
+      rate = THPVariable_Unpack(args[5]);
       if (counters.empty() || !strided_on(rate, device, at::kFloat) || rate.numel() != 1) Py_RETURN_FALSE;
     }
     const at::ScalarType state_types[4] = {eight ? at::kFloat8_e4m3fn : at::kFloat, eight ? at::kFloat8_e5m2 : at::kFloat,

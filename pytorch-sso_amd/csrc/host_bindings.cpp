@@ -391,7 +391,7 @@ PyMethodDef methods[] = {
     {"layer_norm", KFAC_FAST(host_layer_norm), "layer_norm(x, residual, gain, bias, eps, curvature, eight), or None"},
     {"bind_adamw", KFAC_FAST(host_bind_adamw), "bind_adamw(update, workspace): the library's entry points"},
     {"adamw", KFAC_FAST(host_adamw),
-     "adamw(params, grads, m, v, m_scales, v_scales, steps, lr, beta1, beta2, eps, weight_decay, seed): done"},
+     "adamw(params, grads, m, v, steps, lr, beta1, beta2, eps, weight_decay, seed): done"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,

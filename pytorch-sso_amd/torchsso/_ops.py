@@ -920,8 +920,8 @@ def _strides(t):
     return [s for s, n in zip(t.stride(), t.shape) if n > 1]
 
 
-def _check_adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr):
-    """Raises what is wrong with the arguments of an update."""
+def check_adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr):
+    """Raises what is wrong with the tensors of an update."""
     first = params[0]
     device = first.device
     _element_type(first, 'parameter 0')
@@ -965,13 +965,12 @@ def _check_adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr):
     raise _hip.KfacHipError('adamw cannot take these arguments')
 
 
-def adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr, beta1, beta2, eps, weight_decay, seed):
-    """AdamW's update of a list of tensors of one type in place (csrc/host_adamw.cpp); m_scales, v_scales: None where
-    the states are float32.  steps: a number, a number each, or an int32 tensor each."""
+def adamw(params, grads, ms, vs, steps, lr, beta1, beta2, eps, weight_decay, seed):
+    """AdamW's update of a list of tensors of one type in place (csrc/host_adamw.cpp): done, or False where the engine
+    cannot take the arguments, which `check_adamw` says more about.  ms, vs: float32 tensors, or (numbers in 8 bits,
+    scales); steps: a number, a number each, or an int32 tensor each."""
     _hip.load()
-    if len(params) > 0 and not _hip._host.adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr, beta1, beta2, eps,
-                                                weight_decay, seed):
-        _check_adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr)
+    return _hip._host.adamw(params, grads, ms, vs, steps, lr, beta1, beta2, eps, weight_decay, seed)
 
 
 def _rows(t, dim):

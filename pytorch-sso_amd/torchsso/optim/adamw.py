@@ -19,18 +19,19 @@ from torch.optim import Optimizer
 from torchsso import _ops
 
 LEAST_EPS_8 = 1e-12          # of updates with states in 8 bits, where small enough a v is 0
+_INF = float('inf')
 
 
 def _check(lr, betas, eps, weight_decay, eight=False):
-    if not isinstance(lr, torch.Tensor) and not 0 <= lr < float('inf'):
+    if not isinstance(lr, torch.Tensor) and not 0 <= lr < _INF:
         raise ValueError('Invalid learning rate: {}'.format(lr))
     for i, beta in enumerate(betas):
         if not 0 <= beta < 1:
             raise ValueError('Invalid beta parameter at index {}: {}'.format(i, beta))
-    if not (LEAST_EPS_8 if eight else 0) <= eps < float('inf'):
+    if not (LEAST_EPS_8 if eight else 0) <= eps < _INF:
         raise ValueError('Invalid epsilon value: {}{}'.format(
             eps, ' (with states in 8 bits at least {})'.format(LEAST_EPS_8) if eight else ''))
-    if not 0 <= weight_decay < float('inf'):
+    if not 0 <= weight_decay < _INF:
         raise ValueError('Invalid weight_decay value: {}'.format(weight_decay))
 
 
@@ -47,7 +48,6 @@ def adamw_states(param, bits=32):
                  for dtype in (torch.float8_e4m3fn, torch.float8_e5m2))
 
 
-@torch.no_grad()
 def adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0):
     """One update of a list of parameters and their states, in place, in few launches.
 
@@ -59,34 +59,42 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999
     at every replay.  lr: a number, or with such a list a float32 tensor of one element on the device.
     A parameter in bfloat16 or float16 is rounded to its nearest number: what an update adds has to reach half a
     step of that type, or it is lost (gains of size 1 in bfloat16 move by 2^-9 or not at all)."""
-    lists = [list(t) for t in (params, grads, exp_avgs, exp_avg_sqs)]
-    if len(set(len(t) for t in lists)) != 1:
-        raise ValueError('%d parameters, %d gradients, %d first and %d second moments' % tuple(len(t) for t in lists))
-    params, grads, ms, vs = lists
-    pairs = [isinstance(t, (tuple, list)) for t in ms + vs]
+    beta1, beta2 = betas
+    if not isinstance(step, (int, list, tuple)):
+        step = int(step)
+    if not ((isinstance(lr, torch.Tensor) or 0 <= lr < _INF) and 0 <= beta1 < 1 and 0 <= beta2 < 1 and 0 <= eps < _INF
+            and 0 <= weight_decay < _INF and len(params) > 0
+            and _ops.adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, seed)):
+        _refuse(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay)
+
+
+def _refuse(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay):
+    """Raises what is wrong with the arguments of an update (nothing, if there is nothing to update)."""
+    lengths = tuple(len(t) for t in (params, grads, exp_avgs, exp_avg_sqs))
+    if len(set(lengths)) != 1:
+        raise ValueError('%d parameters, %d gradients, %d first and %d second moments' % lengths)
+    pairs = [isinstance(t, (tuple, list)) for t in list(exp_avgs) + list(exp_avg_sqs)]
     eight = len(pairs) > 0 and all(pairs)
     if any(pairs) and not eight:
         raise ValueError('states in 32 bits and in 8 in one list')
     _check(lr, betas, eps, weight_decay, eight)
-    if any(g.is_sparse for g in grads):
+    if any(isinstance(g, torch.Tensor) and g.is_sparse for g in grads):
         raise RuntimeError('AdamW does not take sparse gradients')
-    if isinstance(step, (tuple, list)):
-        if len(step) != len(params):
-            raise ValueError('%d parameters, %d steps' % (len(params), len(step)))
-        step = list(step)
-        if len(set(isinstance(t, torch.Tensor) for t in step)) > 1:
-            raise ValueError('steps on the device and numbers in one list')
-        if step and not isinstance(step[0], torch.Tensor):
-            step = [int(t) for t in step]
-    else:
-        step = int(step)
-    if any(t < 1 for t in ([step] if isinstance(step, int) else step) if isinstance(t, int)):
+    steps = step if isinstance(step, (tuple, list)) else [step] * len(params)
+    if len(steps) != len(params):
+        raise ValueError('%d parameters, %d steps' % (len(params), len(steps)))
+    if len(set(isinstance(t, torch.Tensor) for t in steps)) > 1:
+        raise ValueError('steps on the device and numbers in one list')
+    if any(not isinstance(t, torch.Tensor) and t < 1 for t in steps):
         raise ValueError('Invalid step: {}'.format(step))
-    m_scales = v_scales = None
+    if len(params) == 0:
+        return
+    scales = [None, None]
     if eight:
-        (ms, m_scales), (vs, v_scales) = ([list(t) for t in zip(*pairs)] for pairs in (ms, vs))
-    _ops.adamw(params, grads, ms, vs, m_scales, v_scales, step, lr, float(betas[0]), float(betas[1]), float(eps),
-               float(weight_decay), int(seed))
+        if any(len(t) != 2 for t in list(exp_avgs) + list(exp_avg_sqs)):
+            raise ValueError('a state in 8 bits is (numbers, scales)')
+        (exp_avgs, scales[0]), (exp_avg_sqs, scales[1]) = (zip(*states) for states in (exp_avgs, exp_avg_sqs))
+    _ops.check_adamw(params, grads, exp_avgs, exp_avg_sqs, *scales, step, lr)
 
 
 class AdamW(Optimizer):

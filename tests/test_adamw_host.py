@@ -50,7 +50,7 @@ def test_refusals():
         with pytest.raises(ValueError):
             adamw([p], [p], [m], [v], **dict(dict(step=1), **more))
     for lists in (([p], [], [m], [v]), ([p], [p], [m, m], [v]), ([p, p], [p, p], [m, states(p, 8)[0]], [v, states(p, 8)[1]]),
-                  ([p], [p], [states(p, 8)[0]], [v])):
+                  ([p], [p], [states(p, 8)[0]], [v]), ([p], [p], [states(p, 8)[0] * 2], [states(p, 8)[1] * 2])):
         with pytest.raises(ValueError):
             adamw(*lists, 1)
     m8, v8 = states(p, 8)
@@ -117,7 +117,7 @@ def reason(monkeypatch):
         ms, vs = ms or Fake((2,), address=4 << 20), vs or Fake((2,), address=5 << 20)
         n = 2 if twice else 1
         with pytest.raises(_hip.KfacHipError) as e:
-            _ops._check_adamw([p] * n, [g] * n, [m] * n, [v] * n, [ms] * n if bits == 8 else None,
+            _ops.check_adamw([p] * n, [g] * n, [m] * n, [v] * n, [ms] * n if bits == 8 else None,
                               [vs] * n if bits == 8 else None, steps, lr)
         return str(e.value)
     return of
@@ -197,10 +197,11 @@ def test_state_lies_as_the_parameter_does():
 
 
 def fake_update(calls):
-    def update(params, grads, ms, vs, m_scales, v_scales, steps, lr, *rest):
-        calls.append((len(params), m_scales is not None, list(steps) if isinstance(steps, list) else steps, lr, rest))
+    def update(params, grads, ms, vs, steps, lr, *rest):
+        calls.append((len(params), isinstance(ms[0], tuple), list(steps) if isinstance(steps, list) else steps, lr, rest))
         for p in params:
             p.sub_(1)
+        return True
     return update
 
 
@@ -231,7 +232,7 @@ def test_class_keeps_steps_and_bits_of_each_parameter(monkeypatch):
 
 @pytest.mark.parametrize('capturable', [False, True])
 def test_state_dict_keeps_types(monkeypatch, capturable, tmp_path):
-    monkeypatch.setattr(_ops, 'adamw', lambda *a: None)
+    monkeypatch.setattr(_ops, 'adamw', lambda *a: True)
     made = []
     for _ in range(2):
         params = [torch.nn.Parameter(torch.zeros(5000, dtype=torch.bfloat16)), torch.nn.Parameter(torch.zeros(3, 4).t())]
