@@ -97,14 +97,36 @@ struct Max {
   static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
 };
 
+// x of the lane that is O away (xor), in registers: lanes of 16 rotate (what is added or compared has come to
+// repeat every 2 O lanes by then, so that a rotation by O is that), rows and halves are swapped.  In the caller's order
+// 32, 16, 8, 4, 2, 1.
+template <class OP, int O>
+__device__ __forceinline__ float with_other(float x) {
+  const unsigned u = __float_as_uint(x);
+  if constexpr (O == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return OP::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  } else if constexpr (O == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return OP::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  } else {
+    return OP::of(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, u, 0x120 + O, 0xf, 0xf, true)));
+  }
+}
+
 // Over the threads of a unit, the same in each: a wave, or a workgroup of T threads (`tmp`: room for
 // 2 K T / 64 floats, `turn` alternates so that one barrier is enough).
 template <class OP, int T, int K>
 __device__ __forceinline__ void unit_reduce(float (&v)[K], float* tmp, int& turn) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1)
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = OP::of(v[k], __shfl_xor(v[k], o));
+  for (int k = 0; k < K; ++k) {
+    v[k] = with_other<OP, 32>(v[k]);
+    v[k] = with_other<OP, 16>(v[k]);
+    v[k] = with_other<OP, 8>(v[k]);
+    v[k] = with_other<OP, 4>(v[k]);
+    v[k] = with_other<OP, 2>(v[k]);
+    v[k] = with_other<OP, 1>(v[k]);
+  }
   if constexpr (T > 64) {
     constexpr int W = T / 64;
     float* const at = tmp + turn * K * W;
@@ -122,7 +144,8 @@ __device__ __forceinline__ void unit_reduce(float (&v)[K], float* tmp, int& turn
   }
 }
 
-constexpr int block_threads(int T) { return T < 256 ? 256 : T; }
+// threads of a workgroup of units of T threads: waves by fours, larger units by themselves
+constexpr int block_threads(int T) { return T == 64 ? 256 : T; }
 
 // How the rows are dealt to units.  parts > 0: a unit takes one of `parts` pieces (of `rows` rows)
 // of a sample, and leaves its part of s_n; parts == 0: it takes `rows` / tokens whole samples, or
@@ -260,9 +283,9 @@ Shape norm_shape(int dim, int e) {
       if (n <= t * k) return Shape{t, k};
   return Shape{0, 0};
 }
-Deal deal_rows(long rows, int samples, bool squares, int threads) {
+// to about `target` units
+Deal deal_rows(long rows, int samples, bool squares, long target) {
   Deal d;
-  const long target = threads == 64 ? 4096 : threads == 0 || threads == 1024 ? 512 : 1024;
   d.samples = samples;
   d.tokens = rows / samples;
   const long per = std::max(1L, (rows + target - 1) / target);       // rows of a unit

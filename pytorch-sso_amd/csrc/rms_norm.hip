@@ -379,7 +379,10 @@ int run_norm(int type, const NormArgs& a, hipStream_t stream) {
 }
 
 // the deal must not depend on alignment (the caller asks for scratch by sizes alone)
-int deal_threads(int type, int dim) { return backward_shape(dim, type == TYPE_F32 ? 4 : 8).threads; }
+Deal norm_deal(int type, int64_t rows, int dim, int samples, bool squares) {
+  const int threads = backward_shape(dim, type == TYPE_F32 ? 4 : 8).threads;
+  return deal_rows((long)rows, samples, squares, threads == 64 ? 4096 : threads == 0 || threads == 1024 ? 512 : 1024);
+}
 
 }  // namespace
 }  // namespace kfac
@@ -400,7 +403,7 @@ int kfac_rms_norm(int type, int gain_is_float, int64_t rows, int dim, const void
 
 size_t kfac_rms_norm_backward_workspace_bytes(int type, int64_t rows, int dim, int samples, int squares) {
   if (!norm_args_ok(type, 0, rows, dim, 0.f) || samples <= 0 || rows == 0 || rows % samples != 0) return 0;
-  return sizeof(float) * backward_floats(deal_rows((long)rows, samples, squares != 0, deal_threads(type, dim)), dim);
+  return sizeof(float) * backward_floats(norm_deal(type, rows, dim, samples, squares != 0), dim);
 }
 
 int kfac_rms_norm_backward(int type, int gain_is_float, int64_t rows, int dim, int samples, const void* dy,
@@ -411,7 +414,7 @@ int kfac_rms_norm_backward(int type, int gain_is_float, int64_t rows, int dim, i
   if (rows == 0 || !dy || !h || lddy < 0 || lddh < 0 || ldh < 0 || (dh && !dx)) return KFAC_ERR_ARG;
   const bool sums = dgain || curvature;
   BackArgs a{dy, dh, h, gain, dx, nullptr, (long)rows, (long)lddy, (long)lddh, (long)ldh, dim, gain_is_float, eps, {}};
-  a.deal = deal_rows((long)rows, samples, curvature != nullptr, deal_threads(type, dim));
+  a.deal = norm_deal(type, rows, dim, samples, curvature != nullptr);
   float* current = nullptr;
   if (sums) {
     if (!workspace || workspace_bytes < sizeof(float) * backward_floats(a.deal, dim)) return KFAC_ERR_WORKSPACE;
