@@ -553,13 +553,13 @@ __global__ __launch_bounds__(COLUMN_THREADS) void layer_norm_columns_kernel(cons
   sums.template leave<RAGGED>(a, unit, place);
 }
 
-// Threads a row and accesses of a thread.  Forward: a wave up to four accesses, then 256 threads, then 1024.  (8193 rows of
-// 5120 with their residual to 8 bits: three accesses on 256 threads 61 us, four of which a third is idle 65, ten on a
-// wave 77.)
+// Threads a row and accesses of a thread.  Forward: a wave with up to two accesses, then 128 threads with two, 256 and 1024
+// with two to four.  (8193 rows of 5120 with their residual to 8 bits: three accesses on 256 threads 61 us, four of which a
+// third is idle 65, ten on a wave 77; 16000 rows of 2048 with their residual: 128 threads 45, a wave with four accesses 52.)
+constexpr Shape LAYER_SHAPES[] = {{64, 1}, {64, 2}, {128, 2}, {256, 2}, {256, 3}, {256, 4}, {1024, 2}, {1024, 3}, {1024, 4}};
 Shape layer_norm_shape(int n) {
-  for (int t : {64, 256, 1024})
-    for (int k : {1, 2, 3, 4})
-      if (n <= t * k) return Shape{t, k};
+  for (const Shape& s : LAYER_SHAPES)
+    if (n <= s.threads * s.accesses) return s;
   return Shape{0, 0};
 }
 
@@ -612,7 +612,7 @@ void launch_layer_norm(const LayerNormArgs& a, hipStream_t stream) {
     });                                                                                                   \
     return;                                                                                               \
   }
-  NORM_CASE(64, 1) NORM_CASE(64, 2) NORM_CASE(64, 3) NORM_CASE(64, 4)
+  NORM_CASE(64, 1) NORM_CASE(64, 2) NORM_CASE(128, 2)
   NORM_CASE(256, 2) NORM_CASE(256, 3) NORM_CASE(256, 4)
   NORM_CASE(1024, 2) NORM_CASE(1024, 3) NORM_CASE(1024, 4)
 #undef NORM_CASE
