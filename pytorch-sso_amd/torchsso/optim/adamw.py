@@ -124,7 +124,16 @@ class AdamW(Optimizer):
              'exp_avg_scale': (torch.float32,), 'exp_avg_sq_scale': (torch.float32,)}
 
     def load_state_dict(self, state_dict):
+        """What state_dict of this class has saved, or of torch.optim.AdamW (states that are neither float32 nor 8 bits
+        become float32)."""
+        for group in state_dict['param_groups']:
+            for name in ('amsgrad', 'maximize'):
+                if group.get(name):
+                    raise ValueError('AdamW has no option {}'.format(name))
         super(AdamW, self).load_state_dict(state_dict)
+        for group in self.param_groups:
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
         # (the base class gives states their parameter's type; these keep their own, and a parameter's order in memory)
         ids = [i for group in state_dict['param_groups'] for i in group['params']]
         params = [(p, group) for group in self.param_groups for p in group['params']]
@@ -133,30 +142,29 @@ class AdamW(Optimizer):
             if not saved:
                 continue
             state = self.state[p]
-            for name in self._KEPT:
+            for name, types in self._KEPT.items():
                 if name in saved:
                     t = saved[name].detach()
-                    like = torch.empty_like(p, dtype=t.dtype, requires_grad=False) if t.shape == p.shape \
-                        else torch.empty(t.shape, dtype=t.dtype, device=p.device)
+                    dtype = t.dtype if t.dtype in types else torch.float32
+                    like = torch.empty(t.shape, dtype=dtype, device=p.device) if name.endswith('scale') \
+                        else torch.empty_like(p, dtype=dtype, requires_grad=False)
                     state[name] = like.copy_(t)
             step = int(saved['step'])
             state['step'] = torch.full((), step, dtype=torch.int32, device=p.device) if group['capturable'] else step
 
-    def _state_of(self, p, group, capturing):
+    def _first_state(self, p, group, capturing):
+        if capturing:
+            raise RuntimeError('AdamW: a step has to be taken before one is recorded (it makes the states)')
         state = self.state[p]
-        if len(state) == 0:
-            if capturing:
-                raise RuntimeError('AdamW: a step has to be taken before one is recorded (it makes the states)')
-            state['step'] = torch.zeros((), dtype=torch.int32, device=p.device) if group['capturable'] else 0
-            eight = group['state_bits'] == 8 and p.numel() >= group['min_8bit_size']
-            m, v = adamw_states(p, 8 if eight else 32)
-            if eight:
-                (state['exp_avg'], state['exp_avg_scale']), (state['exp_avg_sq'], state['exp_avg_sq_scale']) = m, v
-            else:
-                state['exp_avg'], state['exp_avg_sq'] = m, v
+        state['step'] = torch.zeros((), dtype=torch.int32, device=p.device) if group['capturable'] else 0
+        eight = group['state_bits'] == 8 and p.numel() >= group['min_8bit_size']
+        m, v = adamw_states(p, 8 if eight else 32)
+        if eight:
+            (state['exp_avg'], state['exp_avg_scale']), (state['exp_avg_sq'], state['exp_avg_sq_scale']) = m, v
+        else:
+            state['exp_avg'], state['exp_avg_sq'] = m, v
         return state
 
-    @torch.no_grad()
     def step(self, closure=None):
         """One optimization step.  `closure` runs forward and backward and returns the loss or
         (loss, output); its return value is passed through."""
@@ -165,31 +173,35 @@ class AdamW(Optimizer):
             with torch.enable_grad():
                 loss = closure()
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
-        lists = 0
+        kept, lists = self.state, 0
         for group in self.param_groups:
-            if capturing and not group['capturable']:
+            capturable = group['capturable']
+            if capturing and not capturable:
                 raise RuntimeError('AdamW: capturable=True is needed to record a step')
-            alike = {}
+            alike, last = {}, None
             for p in group['params']:
-                if p.grad is None:
+                g = p.grad
+                if g is None:
                     continue
-                state = self._state_of(p, group, capturing)
-                eight = 'exp_avg_scale' in state
-                ps, gs, ms, vs, states = alike.setdefault((p.dtype, p.device, eight), ([], [], [], [], []))
+                state = kept.get(p) or self._first_state(p, group, capturing)
+                scale = state.get('exp_avg_scale')
+                key = (p.dtype, p.get_device(), scale is None)
+                if key != last:
+                    last = key
+                    ps, gs, ms, vs, states = alike.setdefault(key, ([], [], [], [], []))
                 ps.append(p)
-                gs.append(p.grad)
-                ms.append((state['exp_avg'], state['exp_avg_scale']) if eight else state['exp_avg'])
-                vs.append((state['exp_avg_sq'], state['exp_avg_sq_scale']) if eight else state['exp_avg_sq'])
+                gs.append(g)
+                ms.append(state['exp_avg'] if scale is None else (state['exp_avg'], scale))
+                vs.append(state['exp_avg_sq'] if scale is None else (state['exp_avg_sq'], state['exp_avg_sq_scale']))
                 states.append(state)
             for ps, gs, ms, vs, states in alike.values():
-                if group['capturable']:
-                    steps = [state['step'] for state in states]
-                else:
-                    steps = [state['step'] + 1 for state in states]
+                steps = [state['step'] for state in states]
+                if not capturable:
+                    steps = [step + 1 for step in steps]
                 adamw(ps, gs, ms, vs, steps, lr=group['lr'], betas=group['betas'], eps=group['eps'],
                       weight_decay=group['weight_decay'], seed=group['seed'] + lists)
                 lists += 1
-                if not group['capturable']:
+                if not capturable:
                     for state, step in zip(states, steps):
                         state['step'] = step
         return loss

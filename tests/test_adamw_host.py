@@ -199,8 +199,9 @@ def test_state_lies_as_the_parameter_does():
 def fake_update(calls):
     def update(params, grads, ms, vs, steps, lr, *rest):
         calls.append((len(params), isinstance(ms[0], tuple), list(steps) if isinstance(steps, list) else steps, lr, rest))
-        for p in params:
-            p.sub_(1)
+        with torch.no_grad():
+            for p in params:
+                p.sub_(1)
         return True
     return update
 
@@ -263,6 +264,35 @@ def test_state_dict_keeps_types(monkeypatch, capturable, tmp_path):
     loaded.load_state_dict(saved)
     a, b = saved['state'][0]['exp_avg'], loaded.state[loaded.param_groups[0]['params'][0]]['exp_avg']
     assert a.data_ptr() != b.data_ptr()
+
+
+def test_states_of_torchs_class_are_taken(monkeypatch):
+    calls = []
+    monkeypatch.setattr(_ops, 'adamw', fake_update(calls))
+    params = [torch.nn.Parameter(torch.randn(4, 5, dtype=torch.bfloat16)), torch.nn.Parameter(torch.randn(3))]
+    other = torch.optim.AdamW(params, lr=3e-3, betas=(.8, .95), eps=1e-7, weight_decay=.2, foreach=False)
+    for p in params:
+        p.grad = torch.randn_like(p)
+    for _ in range(2):
+        other.step()
+    for capturable in (False, True):
+        opt = torchsso.optim.AdamW(params, seed=3, capturable=capturable)
+        saved = other.state_dict()
+        for group in saved['param_groups']:
+            group.pop('capturable')               # (torch's is False: a step is a number then)
+        opt.load_state_dict(saved)
+        for p in params:
+            state = opt.state[p]
+            assert sorted(state) == ['exp_avg', 'exp_avg_sq', 'step'] and state['step'] == 2
+            assert state['exp_avg'].dtype == state['exp_avg_sq'].dtype == torch.float32
+            assert torch.equal(state['exp_avg'], other.state[p]['exp_avg'].float())
+        calls.clear()
+        if not capturable:
+            opt.step()
+            assert [c[2:] for c in calls] == [([3], 3e-3, (.8, .95, 1e-7, .2, 3)), ([3], 3e-3, (.8, .95, 1e-7, .2, 4))]
+    for name in ('amsgrad', 'maximize'):
+        with pytest.raises(ValueError, match=name):
+            torchsso.optim.AdamW(params).load_state_dict(torch.optim.AdamW(params, **{name: True}).state_dict())
 
 
 def test_lr_scheduler(monkeypatch):
