@@ -1,14 +1,14 @@
 """A small pre-norm decoder trained with second-order updates of all its parts, on synthetic text:
 
-    python examples/decoder.py [--steps 400]
+    python examples/decoder.py [--steps 400] [--norm layer]
 
   matrices (bfloat16)   torchsso.optim.Muon: momentum, orthogonalised
-  gains of the norms    torchsso.optim.SecondOrderOptimizer with DiagCovRMSNorm, whose curvature the
-                        norms' backward passes form beside the gradients
-  embedding             torch.optim.AdamW
+  norms                 torchsso.optim.SecondOrderOptimizer with DiagCovRMSNorm (with --norm layer
+                        DiagCovLayerNorm), whose curvature the norms' backward passes form beside the gradients
+  embedding             torchsso.optim.AdamW, its states in 8 bits
 
 Every block adds its input to the residual stream and normalises the sum in one pass
-(torchsso.nn.RMSNorm with two arguments).  Afterwards the model continues a text; the product behind
+(torchsso.nn.RMSNorm or LayerNorm with two arguments).  Afterwards the model continues a text; the product behind
 the last norm then runs in 8 bits, on what the norm has left in 8 bits with a scale per token.
 
 The text follows a rule (the next symbol is a fixed function of the last two, one time in ten any),
@@ -40,13 +40,13 @@ def text(batch, tokens, gen, device):
 
 class Block(nn.Module):
 
-    def __init__(self, dim, heads, device):
+    def __init__(self, dim, heads, device, norm):
         super().__init__()
         self.heads = heads
         linear = lambda i, o: nn.Linear(i, o, bias=False, device=device, dtype=torch.bfloat16)
-        self.norm1 = torchsso.nn.RMSNorm(dim, device=device)
+        self.norm1 = norm(dim, device=device)
         self.q, self.k, self.v, self.o = (linear(dim, dim) for _ in range(4))
-        self.norm2 = torchsso.nn.RMSNorm(dim, device=device)
+        self.norm2 = norm(dim, device=device)
         self.up, self.gate, self.down = linear(dim, 4 * dim), linear(dim, 4 * dim), linear(4 * dim, dim)
 
     def forward(self, x, stream):
@@ -61,11 +61,11 @@ class Block(nn.Module):
 
 class Decoder(nn.Module):
 
-    def __init__(self, dim=128, heads=4, layers=2, device='cuda'):
+    def __init__(self, dim=128, heads=4, layers=2, device='cuda', norm=torchsso.nn.RMSNorm):
         super().__init__()
         self.embedding = nn.Embedding(VOCAB, dim, device=device)
-        self.blocks = nn.ModuleList(Block(dim, heads, device) for _ in range(layers))
-        self.norm = torchsso.nn.RMSNorm(dim, device=device)
+        self.blocks = nn.ModuleList(Block(dim, heads, device, norm) for _ in range(layers))
+        self.norm = norm(dim, device=device)
         self.head = nn.Linear(dim, VOCAB, bias=False, device=device, dtype=torch.bfloat16)
 
     def body(self, tokens):
@@ -86,8 +86,11 @@ class Decoder(nn.Module):
     @torch.no_grad()
     def logits_8(self, x, stream, weight, scale):
         """Of one token of each text, through the last norm and layer in 8 bits."""
-        q, q_scale, _ = torchsso.nn.add_rms_norm(x, stream, self.norm.weight, self.norm.eps,
-                                                 out_dtype=torch.float8_e4m3fn)
+        more = dict(eps=self.norm.eps, out_dtype=torch.float8_e4m3fn)
+        if isinstance(self.norm, torchsso.nn.LayerNorm):
+            q, q_scale, _ = torchsso.nn.add_layer_norm(x, stream, self.norm.weight, self.norm.bias, **more)
+        else:
+            q, q_scale, _ = torchsso.nn.add_rms_norm(x, stream, self.norm.weight, **more)
         return torch._scaled_mm(q, weight.t(), scale_a=q_scale, scale_b=scale.t().contiguous(),
                                 out_dtype=torch.bfloat16).float()
 
@@ -106,16 +109,18 @@ def main(argv=None):
     parser.add_argument('--steps', type=int, default=400)
     parser.add_argument('--batch', type=int, default=64)
     parser.add_argument('--tokens', type=int, default=64)
+    parser.add_argument('--norm', choices=('rms', 'layer'), default='rms')
     args = parser.parse_args(argv)
     torch.manual_seed(0)
     gen = torch.Generator().manual_seed(0)
-    model = Decoder()
-    norms = nn.ModuleList(m for m in model.modules() if isinstance(m, torchsso.nn.RMSNorm))
+    norm = torchsso.nn.LayerNorm if args.norm == 'layer' else torchsso.nn.RMSNorm
+    model = Decoder(norm=norm)
+    norms = nn.ModuleList(m for m in model.modules() if isinstance(m, norm))
     matrices = [m.weight for m in model.modules() if isinstance(m, nn.Linear)]
     optimizers = [torchsso.optim.Muon(matrices, lr=0.02, weight_decay=0.01),
-                  torchsso.optim.SecondOrderOptimizer(norms, 'Cov', {'RMSNorm': 'Diag'},
+                  torchsso.optim.SecondOrderOptimizer(norms, 'Cov', {norm.__name__: 'Diag'},
                                                       {'damping': 1e-2, 'ema_decay': 0.1}, lr=1e-2, momentum=0.9),
-                  torch.optim.AdamW(model.embedding.parameters(), lr=1e-2)]
+                  torchsso.optim.AdamW(model.embedding.parameters(), lr=1e-2, state_bits=8)]
     losses = []
     for step in range(args.steps):
         x = text(args.batch, args.tokens + 1, gen, 'cuda')
