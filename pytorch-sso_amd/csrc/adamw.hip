@@ -1,7 +1,8 @@
 // AdamW: one update of a list of tensors, with states in 32 or in 8 bits.
 //
 //   m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2
-//   p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//   p = (1 - lr wd) p - m / (root sqrt(v) + eps'),   root = 1 / (size sqrt(1 - b2^t)),  eps' = eps / size,
+//                                                    size = lr / (1 - b1^t)
 //
 // In 8 bits a state is kept by blocks of 128 consecutive elements with a float32 scale each: m / scale in e4m3 with
 // scale = max |m| / 448 of the block, v / scale in e5m2 with scale = max v / 57344.  Both are rounded at random to one of
@@ -33,11 +34,11 @@ constexpr unsigned INFINITE = 0x7f800000u;
 
 // What depends on the number of the update
 struct AdamScalars {
-  float keep, size, root;                 // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  float keep, root, eps;                  // 1 - lr wd, and what stands above
   unsigned key;                           // of its random numbers
 };
 struct AdamRates {
-  float b1, c1, b2, c2, eps;              // c: 1 - b
+  float b1, c1, b2, c2;                   // c: 1 - b
 };
 
 template <int BITS> struct AdamTensor;
@@ -128,11 +129,13 @@ __device__ __forceinline__ void decode_v(u2 q, float (&x)[UNIT]) {
   }
 }
 
-// Largest of the 16 threads that hold a block
+// Largest of the 16 threads that hold a block, a row of the wave: rotated in registers
+static_assert(LANES == 16, "a row of a wave");
 __device__ __forceinline__ unsigned block_max(unsigned x) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, o));
-  return x;
+  x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true));
+  x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, true));
+  x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, true));
+  return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, true));
 }
 
 // Scale and its reciprocal from the bits of the block's largest number (products with reciprocals that are rounded:
@@ -189,8 +192,8 @@ __device__ __forceinline__ void update(const AdamRates& r, const AdamScalars& s,
     m = r.b1 * m + r.c1 * g;
     v = r.b2 * v + r.c2 * g * g;
   }
-  if (FAST) p = fmaf(p, s.keep, -s.size * m * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(v), s.root, r.eps)));
-  else p = fmaf(p, s.keep, -s.size * (m / fmaf(sqrtf(v), s.root, r.eps)));
+  if (FAST) p = fmaf(-m, __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(v), s.root, s.eps)), p * s.keep);
+  else p = fmaf(p, s.keep, -(m / fmaf(sqrtf(v), s.root, s.eps)));
 }
 
 // Elements i ... i + 7 of a tensor, `have` of them (8 where all streams can be accessed 16 bytes at a time: whole).
@@ -288,25 +291,32 @@ __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamSc
   float m_inverse, v_inverse;
   block_scale(top_m, LARGEST_M, m_scale, m_inverse);
   block_scale(top_v, LARGEST_V, v_scale, v_inverse);
-  // a v above 0 is at least the smallest number
   const float least = v_inverse > 0.f ? LEAST_V : 0.f;
   if (odd && v_scale == 0.f) {                       // (an infinite v stays one beside zeros)
     v_scale = 1.f;
     v_inverse = 0x1p-126f;
   }
+  float scaled[UNIT], lowest = LARGEST_V;
 #pragma unroll
   for (int e = 0; e < UNIT; ++e) {
     m[e] *= m_inverse;
-    v[e] = v[e] > 0.f ? fmaxf(v[e] * v_inverse, least) : v[e];
+    scaled[e] = v[e] * v_inverse;
+    lowest = fminf(lowest, scaled[e]);
+  }
+  // a v above 0 is at least the smallest number (they are rarely below it: few threads come here)
+  if (lowest < least) {
+#pragma unroll
+    for (int e = 0; e < UNIT; ++e)
+      if (v[e] > 0.f) scaled[e] = fmaxf(scaled[e], least);
   }
   unsigned word = mix(s.key + (unsigned)(i / UNIT));
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     int mw = 0, vw = 0;
-    encode<0>(m, v, k, word, mw, vw);
-    encode<1>(m, v, k, word, mw, vw);
-    encode<2>(m, v, k, word, mw, vw);
-    encode<3>(m, v, k, word, mw, vw);
+    encode<0>(m, scaled, k, word, mw, vw);
+    encode<1>(m, scaled, k, word, mw, vw);
+    encode<2>(m, scaled, k, word, mw, vw);
+    encode<3>(m, scaled, k, word, mw, vw);
     mq[k] = (unsigned)mw;
     vq[k] = (unsigned)vw;
   }
@@ -352,12 +362,16 @@ __global__ __launch_bounds__(ADAM_THREADS) void adamw_kernel(const AdamList<BITS
 
 // ---- numbers of the update on the device -----------------------------------------
 
-__host__ __device__ inline AdamScalars scalars_of(double t, unsigned step, double lr, double b1, double b2, double decay,
-                                                  unsigned seed) {
+// (an update by less than LEAST_SIZE is none: the quotients above would leave float32)
+constexpr double LEAST_SIZE = 1e-30;
+__host__ __device__ inline AdamScalars scalars_of(double t, unsigned step, double lr, double b1, double b2, double eps,
+                                                  double decay, unsigned seed) {
   AdamScalars s;
+  const double size = lr / (b1 > 0. ? -expm1(t * log(b1)) : 1.);
+  const bool some = !(size < LEAST_SIZE);
   s.keep = (float)(1. - lr * decay);
-  s.size = (float)(lr / (b1 > 0. ? -expm1(t * log(b1)) : 1.));
-  s.root = (float)(1. / sqrt(b2 > 0. ? -expm1(t * log(b2)) : 1.));
+  s.root = some ? (float)(1. / (size * sqrt(b2 > 0. ? -expm1(t * log(b2)) : 1.))) : 0.f;
+  s.eps = some ? (float)(eps / size) : INFINITY;
   s.key = update_key(seed, step);
   return s;
 }
@@ -367,14 +381,14 @@ struct AdamCounters {
   int n;
 };
 __global__ __launch_bounds__(256) void adamw_scalars_kernel(const AdamCounters c, const float* lr_on_device, double lr, double b1,
-                                                            double b2, double decay, unsigned seed, int first,
+                                                            double b2, double eps, double decay, unsigned seed, int first,
                                                             AdamScalars* out) {
   const int i = threadIdx.x;
   if (i >= c.n) return;
   const int t = *c.step[i] + 1;
   *c.step[i] = t;
   if (lr_on_device) lr = (double)*lr_on_device;
-  out[first + i] = scalars_of((double)t, (unsigned)t, lr, b1, b2, decay, seed);
+  out[first + i] = scalars_of((double)t, (unsigned)t, lr, b1, b2, eps, decay, seed);
 }
 
 long groups_of(int64_t elements) { return ((long)elements + ADAM_GROUP - 1) / ADAM_GROUP; }
@@ -386,7 +400,7 @@ struct AdamCall {
   const void* const* grads;
   float *const *m_scales, *const *v_scales;
   const AdamScalars* scalars;             // on the device, where there are no steps
-  double lr, beta1, beta2, decay;
+  double lr, beta1, beta2, eps, decay;
   unsigned seed;
   AdamRates rates;
   bool once;
@@ -411,7 +425,7 @@ int launch_adamw(const AdamCall& c, int first, hipStream_t stream) {
       if (at == ADAM_SETS) break;
       if (at == sets) {
         step[sets] = c.steps[i];
-        list.sets[sets++] = scalars_of((double)c.steps[i], (unsigned)c.steps[i], c.lr, c.beta1, c.beta2, c.decay, c.seed);
+        list.sets[sets++] = scalars_of((double)c.steps[i], (unsigned)c.steps[i], c.lr, c.beta1, c.beta2, c.eps, c.decay, c.seed);
       }
       list.set[k] = (unsigned char)at;
     }
@@ -484,11 +498,11 @@ int kfac_adamw_batched(int count, const int64_t* numel, int type, int state_bits
     AdamCounters c;
     c.n = std::min(256, count - first);
     for (int k = 0; k < c.n; ++k) c.step[k] = counters[first + k];
-    hipLaunchKernelGGL(adamw_scalars_kernel, dim3(1), dim3(256), 0, s, c, lr_on_device, lr, beta1, beta2, weight_decay, seed, first,
+    hipLaunchKernelGGL(adamw_scalars_kernel, dim3(1), dim3(256), 0, s, c, lr_on_device, lr, beta1, beta2, eps, weight_decay, seed, first,
                        on_device);
   }
-  const AdamCall c{count, numel, steps, params, m, v, grads, m_scales, v_scales, on_device, lr, beta1, beta2, weight_decay, seed,
-                   {(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps},
+  const AdamCall c{count, numel, steps, params, m, v, grads, m_scales, v_scales, on_device, lr, beta1, beta2, eps, weight_decay, seed,
+                   {(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2)},
                    elements * (3 * type_size(type) + 4) > LAST_CACHE};
   const bool wide = state_bits == 32;
   if (type == TYPE_F32) wide ? launch_all<float, 32>(c, s) : launch_all<float, 8>(c, s);
