@@ -591,7 +591,7 @@ int kfac_rms_norm_backward(int type, int gain_is_float, int64_t rows, int dim, i
 /* ---- Layer norm ------------------------------------------------------------- */
 
 /* h = x + residual, rounded to its type;  y = (h - mean(h)) / sqrt(var(h) + eps) * gain + bias,  with the
- * arguments of kfac_rms_norm and bias of the gain's type, or NULL (gain NULL: no bias either).  stats != NULL:
+ * arguments of kfac_rms_norm (a scale is at least 2^-120) and bias of the gain's type, or NULL (gain NULL: no bias either).  stats != NULL:
  * receives what the backward pass needs of each row, 3 floats [rows][3]: a mean m of h, the mean e of
  * h - m (what rounding has lost of m), and 1 / sqrt(var + eps); y may be NULL then.
  * The normalisation in front of the layers of a decoder, as the reference has BatchNorm in front of

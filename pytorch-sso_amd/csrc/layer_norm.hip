@@ -105,23 +105,24 @@ __device__ __forceinline__ void row_gain(const void* w, int w_f32, const Place<R
     for (int e = 0; e < N; ++e) v[e] = e < at.count ? ((const float*)w)[e] : 0.f;
   }
 }
-// ... divided by `scale` in 8 bits
+// ... in 8 bits, times the reciprocal of the row's scale (a division an element is a third of the pass's arithmetic: 8193
+// rows of 5120 61 us, without it 57)
 template <bool RAGGED, int N>
-__device__ __forceinline__ void row_store8(unsigned char* p, const Place<RAGGED, N>& at, const float (&v)[N], float scale) {
+__device__ __forceinline__ void row_store8(unsigned char* p, const Place<RAGGED, N>& at, const float (&v)[N], float inverse) {
   p += at.c;
-  if constexpr (!RAGGED) {
-    store8<N>(p, v, scale);
-  } else {
-    alignas(8) unsigned q[N / 4];
-    store8<N>((unsigned char*)q, v, scale);
-    if (at.count == N) {
-      if constexpr (N == 8) *(loose2*)p = loose2{q[0], q[1]};
-      else *(loose1*)p = q[0];
-    } else {
+  unsigned q[N / 4];
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (e < at.count) p[e] = (unsigned char)(q[e / 4] >> (8 * (e & 3)));
-    }
+  for (int e = 0; e < N; e += 4) {
+    const int low = __builtin_amdgcn_cvt_pk_fp8_f32(v[e] * inverse, v[e + 1] * inverse, 0, false);
+    q[e / 4] = __builtin_amdgcn_cvt_pk_fp8_f32(v[e + 2] * inverse, v[e + 3] * inverse, low, true);
+  }
+  if (at.count == N) {
+    if constexpr (N == 8) *(loose2*)p = loose2{q[0], q[1]};
+    else *(loose1*)p = q[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < at.count) p[e] = (unsigned char)(q[e / 4] >> (8 * (e & 3)));
   }
 }
 
@@ -138,6 +139,9 @@ struct LayerNormArgs {
 __device__ __forceinline__ float row_scale(float squares, float mean, float eps) {
   return rsqrtf(fmaxf(fmaf(-mean, mean, squares), 0.f) + eps);
 }
+
+// Scale of a row whose largest |y| is `top`: not so small that its reciprocal would leave float32
+__device__ __forceinline__ float eight_scale(float top) { return top > 0.f ? fmaxf(top / LARGEST_8, 0x1p-120f) : 1.f; }
 
 // T threads a row, N accesses each.
 template <class V, int T, int N, bool RAGGED, bool ONCE>
@@ -225,12 +229,12 @@ __global__ __launch_bounds__(block_threads(T)) void layer_norm_kernel(const Laye
   if (!a.scale) return;
   turn = 0;
   unit_reduce<Max, T, 1>(top, tmp, turn);
-  const float scale = top[0] > 0.f ? top[0] / LARGEST_8 : 1.f;
+  const float scale = eight_scale(top[0]), inverse = 1.f / scale;
   if (t == 0) a.scale[row] = scale;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const Place<RAGGED, E> at((n * T + t) * E, a.dim);
-    if (at.any) row_store8<RAGGED, E>((unsigned char*)a.y + row * a.dim, at, h[n], scale);
+    if (at.any) row_store8<RAGGED, E>((unsigned char*)a.y + row * a.dim, at, h[n], inverse);
   }
 }
 
@@ -286,7 +290,7 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(const LayerNormAr
     turn = 0;
     unit_reduce<Max, 1024, 1>(top, tmp, turn);
   }
-  const float scale = top[0] > 0.f ? top[0] / LARGEST_8 : 1.f;
+  const float scale = eight_scale(top[0]);
   if (a.scale && threadIdx.x == 0) a.scale[row] = scale;
   for (int c = threadIdx.x; c < a.dim; c += 1024) {
     const float v[1] = {result(c)};

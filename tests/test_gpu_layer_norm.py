@@ -322,6 +322,19 @@ def test_eight_bits(dtype, dim):
         assert bool(((got - want.y).abs() <= bound).all())
 
 
+@pytest.mark.parametrize('dim', [1000, 33000])
+@pytest.mark.parametrize('size', [1e-30, 1e-37, 1e-42, 1e30])
+def test_eight_bits_of_small_and_large_results(dim, size):
+    x, gain = random((3, dim)), torch.full((dim,), size, device='cuda')
+    want = Want(x, None, gain, None)
+    q, scale = torchsso.nn.layer_norm(x, gain, None, EPS, out_dtype=EIGHT)
+    assert bool((scale >= 2. ** -120).all()) and torch.isfinite(q.float()).all()
+    got = q.cpu().float().double() * scale.cpu().double()
+    # (half a unit of an element, or of the smallest numbers, and of y the half of float32's smallest step)
+    bound = torch.maximum(want.y.abs() * 2 ** -4, scale.cpu().double() * 2 ** -10) * (1 + 1e-4) + 2. ** -149
+    assert bool(((got - want.y).abs() <= bound).all())
+
+
 def test_in_a_recorded_graph_and_on_another_stream():
     x, res, gain, bias, dy = (random(s, seed=i) for i, s in enumerate([(6, 20, 300), (6, 20, 300), (300,), (300,), (6, 20, 300)]))
 
