@@ -14,7 +14,7 @@
 // Bound by memory: 3 s + 16 bytes an element with states in 32 bits (s: a parameter's), 3 s + 4.25 in 8.  A thread takes
 // 8 consecutive elements, so 16 threads hold a block, and every stream is read and written once, 16 bytes at a time (8
 // of an 8-bit state).  The list travels as a kernel argument, as that of the other element-wise passes (elementwise.hip).
-// 244 million bfloat16 parameters: 958 us in 32 bits, 5.6 TB/s, and 390 in 8, 6.3, where a large copy reaches 5.2; a
+// 244 million bfloat16 parameters: 958 us in 32 bits, 5.6 TB/s, and 383 in 8, 6.5, where a large copy reaches 5.2; a
 // ResNet-50 in float32 143 us, 5.0 TB/s.  With twice and four times the elements to a workgroup the last takes 146 and 151.
 #include <cmath>
 
@@ -54,8 +54,8 @@ template <> struct AdamTensor<8> {
   long n;
 };
 
-// Tensors of a launch.  A launch more costs 5 us and the end of another one: all of a ResNet-50 in two launches of up
-// to 80 150 us, in four of up to 48 156.  The numbers of their updates are few as a rule, and are kept apart.
+// Tensors of a launch.  A launch more costs 5 us and the end of another one: all of a ResNet-50 in three launches of up
+// to 80 146 us, in four of up to 48 151.  The numbers of their updates are few as a rule, and are kept apart.
 constexpr int ADAM_SHORT = 8, ADAM_SETS = 8;
 template <int BITS> constexpr int adam_long() { return BITS == 32 ? 80 : 60; }
 template <int BITS, int N>
@@ -88,8 +88,11 @@ __device__ __forceinline__ unsigned next_word(unsigned x) {
   return x ^ (x << 5);
 }
 
+// 8 and 16 bytes of elements of 1, 2 and 4 bytes that may begin anywhere (as parts of a buffer do): one access all the same
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned loose2 __attribute__((ext_vector_type(2), aligned(1), may_alias));
+typedef unsigned loose4 __attribute__((ext_vector_type(4), aligned(2), may_alias));
 
 // ---- 8-bit states ----------------------------------------------------------
 
@@ -152,21 +155,30 @@ __device__ __forceinline__ void block_scale(unsigned top_bits, float largest, fl
 // ONCE: past the caches.  States in 8 bits of calls that access more than the last cache holds: 244 million bfloat16
 // parameters 435 us without that, 390 with it.  (In 32 bits it costs: 958 and 977.)
 constexpr double LAST_CACHE = 256. * (1 << 20);
-template <bool ONCE, class W>
-__device__ __forceinline__ W access_load(const void* p) {
-  return ONCE ? __builtin_nontemporal_load((const W*)p) : *(const W*)p;
+template <bool ONCE>
+__device__ __forceinline__ u4 load16(const void* p) {
+  return ONCE ? __builtin_nontemporal_load((const loose4*)p) : *(const loose4*)p;
 }
-template <bool ONCE, class W>
-__device__ __forceinline__ void access_store(void* p, W w) {
-  if (ONCE) __builtin_nontemporal_store(w, (W*)p);
-  else *(W*)p = w;
+template <bool ONCE>
+__device__ __forceinline__ u2 load8(const void* p) {
+  return ONCE ? __builtin_nontemporal_load((const loose2*)p) : *(const loose2*)p;
+}
+template <bool ONCE>
+__device__ __forceinline__ void store16(void* p, u4 w) {
+  if (ONCE) __builtin_nontemporal_store(w, (loose4*)p);
+  else *(loose4*)p = w;
+}
+template <bool ONCE>
+__device__ __forceinline__ void store8(void* p, u2 w) {
+  if (ONCE) __builtin_nontemporal_store(w, (loose2*)p);
+  else *(loose2*)p = w;
 }
 template <bool ONCE, class V>
 __device__ __forceinline__ void load_unit(const V* p, float (&v)[UNIT]) {
   constexpr int E = 16 / sizeof(V);
 #pragma unroll
   for (int i = 0; i < UNIT; i += E) {
-    const Pack<V, E> a = __builtin_bit_cast(Pack<V, E>, access_load<ONCE, u4>(p + i));
+    const Pack<V, E> a = __builtin_bit_cast(Pack<V, E>, load16<ONCE>(p + i));
 #pragma unroll
     for (int e = 0; e < E; ++e) v[i + e] = Element<V>::get(a.v[e]);
   }
@@ -179,7 +191,7 @@ __device__ __forceinline__ void store_unit(V* p, const float (&v)[UNIT]) {
     Pack<V, E> a;
 #pragma unroll
     for (int e = 0; e < E; ++e) a.v[e] = Element<V>::put(v[i + e]);
-    access_store<ONCE>(p + i, __builtin_bit_cast(u4, a));
+    store16<ONCE>(p + i, __builtin_bit_cast(u4, a));
   }
 }
 
@@ -196,10 +208,10 @@ __device__ __forceinline__ void update(const AdamRates& r, const AdamScalars& s,
   else p = fmaf(p, s.keep, -(m / fmaf(sqrtf(v), s.root, s.eps)));
 }
 
-// Elements i ... i + 7 of a tensor, `have` of them (8 where all streams can be accessed 16 bytes at a time: whole).
+// Elements i ... i + 7 of a tensor, or the `have` of them that there are
 template <bool ONCE, class V>
-__device__ __forceinline__ void update_unit(const AdamTensor<32>& t, const AdamScalars& s, const AdamRates& r, long i, int have,
-                                            bool whole) {
+__device__ __forceinline__ void update_unit(const AdamTensor<32>& t, const AdamScalars& s, const AdamRates& r, long i, int have) {
+  const bool whole = have == UNIT;
   V* const pp = (V*)t.p + i;
   const V* const gp = (const V*)t.g + i;
   float *const mp = (float*)t.m + i, *const vp = (float*)t.v + i;
@@ -226,8 +238,8 @@ __device__ __forceinline__ void update_unit(const AdamTensor<32>& t, const AdamS
 }
 
 template <bool ONCE, class V>
-__device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamScalars& s, const AdamRates& r, long i, int have,
-                                            bool whole) {
+__device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamScalars& s, const AdamRates& r, long i, int have) {
+  const bool whole = have == UNIT;
   V* const pp = (V*)t.p + i;
   const V* const gp = (const V*)t.g + i;
   unsigned char *const mp = (unsigned char*)t.m + i, *const vp = (unsigned char*)t.v + i;
@@ -241,8 +253,8 @@ __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamSc
   if (whole) {
     load_unit<ONCE>(gp, g);
     load_unit<ONCE>(pp, p);
-    mq = access_load<ONCE, u2>(mp);
-    vq = access_load<ONCE, u2>(vp);
+    mq = load8<ONCE>(mp);
+    vq = load8<ONCE>(vp);
   } else {
 #pragma unroll
     for (int e = 0; e < UNIT; ++e) {
@@ -321,8 +333,8 @@ __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamSc
     vq[k] = (unsigned)vw;
   }
   if (whole) {
-    access_store<ONCE>(mp, mq);
-    access_store<ONCE>(vp, vq);
+    store8<ONCE>(mp, mq);
+    store8<ONCE>(vp, vq);
   } else {
 #pragma unroll
     for (int e = 0; e < UNIT; ++e)
@@ -335,12 +347,6 @@ __device__ __forceinline__ void update_unit(const AdamTensor<8>& t, const AdamSc
     t.m_scale[i / BLOCK] = m_scale;
     t.v_scale[i / BLOCK] = v_scale;
   }
-}
-
-template <int BITS>
-__device__ __forceinline__ bool accesses_whole(const AdamTensor<BITS>& t) {
-  const uintptr_t wide = (uintptr_t)t.p | (uintptr_t)t.g, states = (uintptr_t)t.m | (uintptr_t)t.v;
-  return ((wide | (BITS == 32 ? states : 0)) & 15) == 0 && (states & 7) == 0;
 }
 
 template <class V, int BITS, int N, bool ONCE>
@@ -356,8 +362,7 @@ __global__ __launch_bounds__(ADAM_THREADS) void adamw_kernel(const AdamList<BITS
   const long i = (long)((int)blockIdx.x - list.first[j]) * ADAM_GROUP + (long)threadIdx.x * UNIT;
   const int have = (int)min(max(t.n - i, 0L), (long)UNIT);
   // (in 8 bits a block's threads go on together)
-  if (BITS == 32 ? have > 0 : i / BLOCK * BLOCK < t.n)
-    update_unit<ONCE, V>(t, s, r, i, have, have == UNIT && accesses_whole<BITS>(t));
+  if (BITS == 32 ? have > 0 : i / BLOCK * BLOCK < t.n) update_unit<ONCE, V>(t, s, r, i, have);
 }
 
 // ---- numbers of the update on the device -----------------------------------------
@@ -368,7 +373,7 @@ __host__ __device__ inline AdamScalars scalars_of(double t, unsigned step, doubl
                                                   double decay, unsigned seed) {
   AdamScalars s;
   const double size = lr / (b1 > 0. ? -expm1(t * log(b1)) : 1.);
-  const bool some = !(size < LEAST_SIZE);
+  const bool some = !(fabs(size) < LEAST_SIZE);
   s.keep = (float)(1. - lr * decay);
   s.root = some ? (float)(1. / (size * sqrt(b2 > 0. ? -expm1(t * log(b2)) : 1.))) : 0.f;
   s.eps = some ? (float)(eps / size) : INFINITY;
