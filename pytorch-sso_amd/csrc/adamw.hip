@@ -15,7 +15,7 @@
 // 8 consecutive elements, so 16 threads hold a block, and every stream is read and written once, 16 bytes at a time (8
 // of an 8-bit state).  The list travels as a kernel argument, as that of the other element-wise passes (elementwise.hip).
 // 244 million bfloat16 parameters: 958 us in 32 bits, 5.6 TB/s, and 383 in 8, 6.5, where a large copy reaches 5.2; a
-// ResNet-50 in float32 143 us, 5.0 TB/s.  With twice and four times the elements to a workgroup the last takes 146 and 151.
+// ResNet-50 in float32 142 us, 5.0 TB/s.  With twice and four times the elements to a workgroup the last takes 3 and 6 % longer.
 #include <cmath>
 
 #include "common.h"
@@ -54,10 +54,11 @@ template <> struct AdamTensor<8> {
   long n;
 };
 
-// Tensors of a launch.  A launch more costs 5 us and the end of another one: all of a ResNet-50 in three launches of up
-// to 80 146 us, in four of up to 48 151.  The numbers of their updates are few as a rule, and are kept apart.
+// Tensors of a launch: as many as 4 KiB of arguments hold.  (A launch more costs 5 us and the end of another one: the 161 tensors
+// of a ResNet-50 in launches of up to 86 142 us, 80 146, 48 151.)  The numbers of their updates are few as a rule, and
+// are kept apart.
 constexpr int ADAM_SHORT = 8, ADAM_SETS = 8;
-template <int BITS> constexpr int adam_long() { return BITS == 32 ? 80 : 60; }
+template <int BITS> constexpr int adam_long() { return BITS == 32 ? 86 : 64; }
 template <int BITS, int N>
 struct AdamList {
   AdamTensor<BITS> d[N];

@@ -96,6 +96,8 @@ def test_many_tensors_with_steps_of_their_own(bits):
     ms, vs = [s[0] for s in states], [s[1] for s in states]
     update_and_check(params, grads, ms, vs, [1 + i % 5 for i in range(len(shapes))], **OPTIONS)
     update_and_check(params, grads, ms, vs, [2 + i % 5 for i in range(len(shapes))], **OPTIONS)
+    # (more different numbers than a launch holds)
+    update_and_check(params, grads, ms, vs, [3 + i % 5 + 7 * (i % 23) for i in range(len(shapes))], **OPTIONS)
 
 
 @BITS

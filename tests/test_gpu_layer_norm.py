@@ -265,6 +265,16 @@ def test_only_one_of_the_results_is_used():
     check(dx, want.dx, torch.float32, 1e-6, want.dx_size)
 
 
+def test_the_same_tensor_twice():
+    x, gain = random((4, 3, 100)).requires_grad_(), random((100,), seed=1).requires_grad_()
+    dy, dh = random((4, 3, 100), seed=2), random((4, 3, 100), seed=3)
+    y, h = torchsso.nn.add_layer_norm(x, x, gain, gain, EPS)
+    dx, dgain = torch.autograd.grad((y, h), (x, gain), (dy, dh))
+    want = Want(x, x, gain, gain, dy, dh, 4)
+    check(dx, 2 * want.dx, torch.float32, 1e-6, 2 * want.dx_size)
+    check(dgain, want.dgain + want.dbias, torch.float32, 2e-6, want.dgain.norm().item() + want.dbias.norm().item())
+
+
 def test_empty():
     gain, bias = (random((50,), seed=i).requires_grad_() for i in range(2))
     x = torch.zeros(0, 4, 50, device='cuda', requires_grad=True)
