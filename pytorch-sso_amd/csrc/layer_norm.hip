@@ -241,30 +241,43 @@ __global__ __launch_bounds__(block_threads(T)) void layer_norm_kernel(const Laye
 // Rows that do not fit registers: three passes over the row, or four, from cache as a rule.
 template <class V>
 __global__ __launch_bounds__(1024) void layer_norm_long_kernel(const LayerNormArgs a) {
+  constexpr int E = width<V>(), STEP = 1024 * E;
   __shared__ float tmp[4 * 16];
   const long row = blockIdx.x;
   const V* const x = (const V*)a.x + row * a.ldx;
   const V* const res = a.residual ? (const V*)a.residual + row * a.ldr : nullptr;
-  const auto value = [&](int c) {
-    float v[1];
-    load<V, 1>(x + c, v);
-    if (res) v[0] = Element<V>::get(Element<V>::put(v[0] + Element<V>::get(res[c])));
-    return v[0];
+  const int begin = (int)threadIdx.x * E;
+  const auto values = [&](const Place<true, E>& at, float (&v)[E]) {
+    row_load<true, false, V, E>(x, at, v);
+    if (!res) return;
+    float b[E];
+    row_load<true, false, V, E>(res, at, b);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = Element<V>::get(Element<V>::put(v[e] + b[e]));
   };
   int turn = 0;
   float s[1] = {0.f};
-  for (int c = threadIdx.x; c < a.dim; c += 1024) {
-    const float v = value(c);
-    if (a.h) ((V*)a.h)[row * a.dim + c] = Element<V>::put(v);
-    s[0] += v;
+  for (int c = begin; c < a.dim; c += STEP) {
+    const Place<true, E> at(c, a.dim);
+    float v[E];
+    values(at, v);
+    if (a.h) row_store<true, false, V, E>((V*)a.h + row * a.dim, at, v);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[0] += at.of_row(e) ? v[e] : 0.f;
   }
   unit_reduce<Sum, 1024, 1>(s, tmp, turn);
   const float inv_dim = 1.f / (float)a.dim, m = s[0] * inv_dim;
   float two[2] = {0.f, 0.f};
-  for (int c = threadIdx.x; c < a.dim; c += 1024) {
-    const float d = value(c) - m;
-    two[0] += d;
-    two[1] = fmaf(d, d, two[1]);
+  for (int c = begin; c < a.dim; c += STEP) {
+    const Place<true, E> at(c, a.dim);
+    float v[E];
+    values(at, v);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float d = at.of_row(e) ? v[e] - m : 0.f;
+      two[0] += d;
+      two[1] = fmaf(d, d, two[1]);
+    }
   }
   turn = 1;
   unit_reduce<Sum, 1024, 2>(two, tmp, turn);
@@ -276,26 +289,38 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(const LayerNormAr
     to[2] = r;
   }
   if (!a.y) return;
-  const auto result = [&](int c) {
-    float w[1], b[1] = {0.f};
-    load_gain<V, 1>(a.w, a.w_f32, c, w);
-    const float xh = ((value(c) - m) - e0) * r;
-    if (!a.b) return xh * w[0];
-    load_gain<V, 1>(a.b, a.w_f32, c, b);
-    return fmaf(xh, w[0], b[0]);
+  const auto results = [&](const Place<true, E>& at, float (&v)[E]) {
+    float w[E], b[E];
+    values(at, v);
+    row_gain<true, V, E>(a.w, a.w_f32, at, w);
+    if (a.b) row_gain<true, V, E>(a.b, a.w_f32, at, b);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float xh = ((v[e] - m) - e0) * r;
+      v[e] = a.b ? fmaf(xh, w[e], b[e]) : xh * w[e];
+    }
   };
-  float top[1] = {0.f};
+  float scale = 1.f, inverse = 1.f;
   if (a.scale) {
-    for (int c = threadIdx.x; c < a.dim; c += 1024) top[0] = fmaxf(top[0], fabsf(result(c)));
+    float top[1] = {0.f};
+    for (int c = begin; c < a.dim; c += STEP) {
+      float v[E];
+      results(Place<true, E>(c, a.dim), v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) top[0] = fmaxf(top[0], fabsf(v[e]));
+    }
     turn = 0;
     unit_reduce<Max, 1024, 1>(top, tmp, turn);
+    scale = eight_scale(top[0]);
+    inverse = 1.f / scale;
+    if (threadIdx.x == 0) a.scale[row] = scale;
   }
-  const float scale = eight_scale(top[0]);
-  if (a.scale && threadIdx.x == 0) a.scale[row] = scale;
-  for (int c = threadIdx.x; c < a.dim; c += 1024) {
-    const float v[1] = {result(c)};
-    if (a.scale) store8<1>((unsigned char*)a.y + row * a.dim + c, v, scale);
-    else store<V, 1>((V*)a.y + row * a.dim + c, v);
+  for (int c = begin; c < a.dim; c += STEP) {
+    const Place<true, E> at(c, a.dim);
+    float v[E];
+    results(at, v);
+    if (a.scale) row_store8<true, E>((unsigned char*)a.y + row * a.dim, at, v, inverse);
+    else row_store<true, false, V, E>((V*)a.y + row * a.dim, at, v);
   }
 }
 
@@ -491,29 +516,51 @@ __global__ __launch_bounds__(1024) void layer_norm_dx_kernel(const LayerBackArgs
 // ... of rows that do not fit registers: two passes over the row, the second from cache as a rule
 template <class V>
 __global__ __launch_bounds__(1024) void layer_norm_dx_long_kernel(const LayerBackArgs a) {
+  constexpr int E = width<V>(), STEP = 1024 * E;
   __shared__ float tmp[4 * 16];
   const long row = blockIdx.x;
-  const V* const dy = (const V*)a.dy + row * a.lddy;
-  const V* const h = (const V*)a.h + row * a.ldh;
   const float *const of = a.stats + row * STATS, m = of[0], e0 = of[1], r = of[2];
+  const int begin = (int)threadIdx.x * E;
+  // u = gain dy and xh
+  const auto terms = [&](const Place<true, E>& at, float (&u)[E], float (&xh)[E]) {
+    float w[E];
+    row_load<true, false, V, E>((const V*)a.dy + row * a.lddy, at, u);
+    row_load<true, false, V, E>((const V*)a.h + row * a.ldh, at, xh);
+    row_gain<true, V, E>(a.w, a.w_f32, at, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      u[e] *= w[e];
+      xh[e] = ((xh[e] - m) - e0) * r;
+    }
+  };
   float two[2] = {0.f, 0.f};
   int turn = 0;
-  for (int c = threadIdx.x; c < a.dim; c += 1024) {
-    float w[1];
-    load_gain<V, 1>(a.w, a.w_f32, c, w);
-    const float xh = ((Element<V>::get(h[c]) - m) - e0) * r, u = w[0] * Element<V>::get(dy[c]);
-    two[0] += u;
-    two[1] = fmaf(u, xh, two[1]);
+  for (int c = begin; c < a.dim; c += STEP) {
+    const Place<true, E> at(c, a.dim);
+    float u[E], xh[E];
+    terms(at, u, xh);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float one = at.of_row(e) ? u[e] : 0.f;
+      two[0] += one;
+      two[1] = fmaf(one, xh[e], two[1]);
+    }
   }
   unit_reduce<Sum, 1024, 2>(two, tmp, turn);
-  const float mean = two[0] / (float)a.dim, along = two[1] / (float)a.dim;
-  for (int c = threadIdx.x; c < a.dim; c += 1024) {
-    float w[1];
-    load_gain<V, 1>(a.w, a.w_f32, c, w);
-    const float xh = ((Element<V>::get(h[c]) - m) - e0) * r;
-    float d = r * fmaf(-xh, along, w[0] * Element<V>::get(dy[c]) - mean);
-    if (a.dh) d += Element<V>::get(((const V*)a.dh)[row * a.lddh + c]);
-    ((V*)a.dx)[row * a.dim + c] = Element<V>::put(d);
+  const float inv_dim = 1.f / (float)a.dim, mean = two[0] * inv_dim, along = two[1] * inv_dim;
+  for (int c = begin; c < a.dim; c += STEP) {
+    const Place<true, E> at(c, a.dim);
+    float u[E], xh[E], d[E];
+    terms(at, u, xh);
+#pragma unroll
+    for (int e = 0; e < E; ++e) d[e] = r * fmaf(-xh[e], along, u[e] - mean);
+    if (a.dh) {
+      float b[E];
+      row_load<true, false, V, E>((const V*)a.dh + row * a.lddh, at, b);
+#pragma unroll
+      for (int e = 0; e < E; ++e) d[e] += b[e];
+    }
+    row_store<true, false, V, E>((V*)a.dx + row * a.dim, at, d);
   }
 }
 
@@ -583,7 +630,8 @@ BackShape layer_backward_shape(int n) {
   if (n <= 16) return BackShape{64, 4096};
   for (const BackShape& s : LAYER_BACK_SHAPES)
     if (n <= s.threads) return s;
-  return BackShape{1024, 256};
+  // (rows whose sums are formed apart: fewer units for more columns, as the partial sums are a row each)
+  return BackShape{1024, n <= 2048 ? 256 : std::max(8, (1 << 19) / n)};
 }
 
 // `n` rows of `a` from `first` on
