@@ -33,8 +33,8 @@ def test_argument_errors_are_codes():
     assert need(0, 4, 8, 2, 1, 0) > 0 and need(0, 4, 8, 3, 1, 0) == 0 and need(0, 0, 8, 1, 1, 0) == 0
     assert need(0, 4, 8, 2, 0, 0) == 0 and need(0, 4, 8, 2, 3, 0) == 0
     assert need(0, 999, 8, 3, 2, 0) == 2 * need(0, 999, 8, 3, 1, 0)
-    # a whole sample's sum and its square are kept by the units where samples are shorter than their rows
-    assert need(0, 1 << 20, 8, 1 << 20, 2, 1) == 3 * need(0, 1 << 20, 8, 1 << 20, 2, 0)
+    # units of whole samples leave their samples' sums and squares
+    assert need(0, 1 << 20, 8, 1 << 20, 2, 1) == 2 * need(0, 1 << 20, 8, 1 << 20, 2, 0)
 
 
 def test_refusals():
