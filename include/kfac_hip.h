@@ -546,7 +546,8 @@ int kfac_muon_update_batched(int count, const int* rows, const int* cols, int ty
  *   mix(x): x ^= x >> 16; x *= 0x9E3779B1; x ^= x >> 15; x *= 0xB504F333; x ^= x >> 16
  *   w_0 = mix(mix(mix(mix(seed) + t) + i) + u),  w_(k+1) = w_k after w ^= w << 13; w ^= w >> 17; w ^= w << 5
  * the upper 16 for m, the lower for v, except that a v above 0 becomes at least the smallest number.
- * eps >= 0, in 8 bits at least 1e-12.  A call may hold one tensor once.
+ * eps >= 0, in 8 bits at least 1e-12; lr / (1 - beta1^t) below 1e-30 leaves p as it is.  A call may hold one tensor once;
+ * parameters, states and counters lie apart from each other.
  * counters != NULL (steps NULL then): device addresses of int32 numbers of updates so far, which the call raises by
  * one and goes by, so that a recorded call counts on when it is replayed; lr_on_device != NULL (only with them): a
  * float that is read in the place of lr.  Either needs the workspace.
@@ -593,7 +594,7 @@ int kfac_rms_norm_backward(int type, int gain_is_float, int64_t rows, int dim, i
 /* h = x + residual, rounded to its type;  y = (h - mean(h)) / sqrt(var(h) + eps) * gain + bias,  with the
  * arguments of kfac_rms_norm (a scale is at least 2^-120) and bias of the gain's type, or NULL (gain NULL: no bias either).  stats != NULL:
  * receives what the backward pass needs of each row, 3 floats [rows][3]: a mean m of h, the mean e of
- * h - m (what rounding has lost of m), and 1 / sqrt(var + eps); y may be NULL then.
+ * h - m (what rounding has lost of m), and 1 / sqrt(var + eps); y may be NULL then.  Results lie apart from the inputs.
  * The normalisation in front of the layers of a decoder, as the reference has BatchNorm in front of
  * its (curv/cov/batchnorm.py:10-49). */
 int kfac_layer_norm(int type, int gain_is_float, int64_t rows, int dim, const void* x, int64_t ldx,
@@ -609,7 +610,7 @@ int kfac_layer_norm(int type, int gain_is_float, int64_t rows, int dim, const vo
  *        and bias, scaled as kfac_rms_norm_backward's (curvature.py:154-158)
  * vectors: 2 with the sums of dy, 1 without (dbias NULL then).  The sums over rows are formed in an order that
  * depends on the sizes alone.  `squares` of the workspace query: whether a curvature is wanted; without dgain,
- * dbias and curvature no workspace is. */
+ * dbias and curvature no workspace is.  Results lie apart from the inputs. */
 size_t kfac_layer_norm_backward_workspace_bytes(int type, int64_t rows, int dim, int samples, int vectors, int squares);
 int kfac_layer_norm_backward(int type, int gain_is_float, int64_t rows, int dim, int samples, int vectors,
                              const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh,
