@@ -125,11 +125,19 @@ class AdamW(Optimizer):
 
     def load_state_dict(self, state_dict):
         """What state_dict of this class has saved, or of torch.optim.AdamW (states that are neither float32 nor 8 bits
-        become float32)."""
+        become float32).  States in 8 bits, whose blocks are those of a memory order, have to be in their parameter's."""
         for group in state_dict['param_groups']:
             for name in ('amsgrad', 'maximize'):
                 if group.get(name):
                     raise ValueError('AdamW has no option {}'.format(name))
+        # (what the base class numbers as it does here)
+        own = [p for group in self.param_groups for p in group['params']]
+        for p, i in zip(own, (i for group in state_dict['param_groups'] for i in group['params'])):
+            saved = state_dict['state'].get(i) or {}
+            for name in ('exp_avg', 'exp_avg_sq'):
+                if name + '_scale' in saved and _ops._strides(saved[name]) != _ops._strides(p):
+                    raise ValueError('a state in 8 bits with strides {} does not lie in memory as its parameter, {}'.format(
+                        saved[name].stride(), p.stride()))
         super(AdamW, self).load_state_dict(state_dict)
         for group in self.param_groups:
             for name, value in self.defaults.items():

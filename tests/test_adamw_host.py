@@ -266,6 +266,24 @@ def test_state_dict_keeps_types(monkeypatch, capturable, tmp_path):
     assert a.data_ptr() != b.data_ptr()
 
 
+def test_states_in_8_bits_of_another_order_of_memory_are_refused(monkeypatch):
+    """The blocks that have a scale each are runs of memory: numbers put into another order would lie under others' scales."""
+    monkeypatch.setattr(_ops, 'adamw', lambda *a: True)
+    p = torch.nn.Parameter(torch.zeros(8, 4, 16, 16).contiguous(memory_format=torch.channels_last))
+    q = torch.nn.Parameter(p.detach().contiguous())
+    for bits in (8, 32):
+        opt, other = (torchsso.optim.AdamW([t], state_bits=bits) for t in (p, q))
+        p.grad = torch.ones_like(p)
+        opt.step()
+        if bits == 32:
+            other.load_state_dict(opt.state_dict())
+            assert other.state[q]['exp_avg'].stride() == q.stride()
+        else:
+            with pytest.raises(ValueError, match='lie in memory'):
+                other.load_state_dict(opt.state_dict())
+            assert not other.state
+
+
 def test_states_of_torchs_class_are_taken(monkeypatch):
     calls = []
     monkeypatch.setattr(_ops, 'adamw', fake_update(calls))
