@@ -77,18 +77,29 @@ struct WithoutInterpreter {
   ~WithoutInterpreter() { PyEval_RestoreThread(state); }
 };
 
-// No element is written twice.
-bool apart(const std::vector<Tensor>& written) {
-  std::vector<std::pair<const char*, const char*>> ranges;
+// A gradient is read where it is: its elements lie as its parameter's do, with their own sign.
+bool read_in_place(const Tensor& grad, const Tensor& p) { return lies_as(grad, p) && !grad.is_neg(); }
+
+// No element is written twice, or is one of a gradient that is read in place (another thread's, perhaps).
+bool apart(const std::vector<Tensor>& written, const std::vector<Tensor>& params, const std::vector<Tensor>& grads) {
+  typedef std::pair<const char*, const char*> Range;
+  const auto range = [](const Tensor& t) {
+    const char* const at = (const char*)t.const_data_ptr();
+    return Range(at, at + t.numel() * (int64_t)t.element_size());
+  };
+  std::vector<Range> ranges;
   ranges.reserve(written.size());
   for (const Tensor& t : written)
-    if (t.numel() > 0) {
-      const char* const at = (const char*)t.const_data_ptr();
-      ranges.emplace_back(at, at + t.numel() * (int64_t)t.element_size());
-    }
+    if (t.numel() > 0) ranges.push_back(range(t));
   std::sort(ranges.begin(), ranges.end());
   for (size_t i = 1; i < ranges.size(); ++i)
     if (ranges[i].first < ranges[i - 1].second) return false;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (grads[i].numel() == 0 || !read_in_place(grads[i], params[i])) continue;
+    const Range g = range(grads[i]);
+    const auto behind = std::lower_bound(ranges.begin(), ranges.end(), Range(g.second, nullptr));
+    if (behind != ranges.begin() && (behind - 1)->second > g.first) return false;
+  }
   return true;
 }
 
@@ -175,7 +186,7 @@ PyObject* host_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       }
     }
     written.insert(written.end(), counters.begin(), counters.end());
-    if (!apart(written)) Py_RETURN_FALSE;
+    if (!apart(written, params, grads)) Py_RETURN_FALSE;
     int status;
     {
       const WithoutInterpreter released;
@@ -186,7 +197,7 @@ PyObject* host_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       for (auto& a : at) a.resize(n);
       for (size_t i = 0; i < n; ++i) {
         Tensor& grad = grads[i];
-        if (!lies_as(grad, params[i]) || grad.is_neg()) {
+        if (!read_in_place(grad, params[i])) {
           Tensor copy = at::empty_strided(params[i].sizes(), params[i].strides(), grad.options());
           copy.copy_(grad.detach());
           grad = copy;

@@ -962,6 +962,10 @@ def check_adamw(params, grads, ms, vs, m_scales, v_scales, steps, lr):
     ranges = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written)
     if any(b[0] < a[1] for a, b in zip(ranges, ranges[1:])):
         raise _hip.KfacHipError('parameters, states or steps share memory, or one is in the list twice')
+    for i, (p, g) in enumerate(zip(params, grads)):
+        begin, end = g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()
+        if _strides(g) == _strides(p) and any(a < end and begin < b for a, b in ranges):
+            raise _hip.KfacHipError('gradient %d shares memory with what the update writes' % i)
     raise _hip.KfacHipError('adamw cannot take these arguments')
 
 

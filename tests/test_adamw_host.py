@@ -143,6 +143,16 @@ def test_what_is_refused_is_named(reason):
     assert 'cannot take' in reason(m=Fake((10, 20), address=(1 << 20) + 800))
 
 
+def test_gradients_in_memory_that_is_written_are_named(reason):
+    for base in (1, 2, 3):
+        for offset in (-796, 0, 796):
+            assert 'gradient 0 shares memory' in reason(g=Fake((10, 20), address=(base << 20) + offset))
+        for offset in (-800, 800):
+            assert 'cannot take' in reason(g=Fake((10, 20), address=(base << 20) + offset))
+    # (one that lies otherwise is copied first)
+    assert 'cannot take' in reason(g=Fake((10, 20), strides=(1, 10), address=1 << 20))
+
+
 def test_random_numbers():
     """16 bits for m and 16 for v of every element: uniform, and no two of them that a rounding meets go together.
     (Over n numbers a mean of uniform ones is off by 0.29 / sqrt(n) on average, a correlation by 1 / sqrt(n): 5 times that.)"""

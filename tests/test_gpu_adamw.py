@@ -367,6 +367,29 @@ def test_refusals():
     assert int(count) == 1 and not torch.equal(p, before[0])
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_gradients_in_memory_that_is_written(bits):
+    """Refused where another thread may have written them already; a copy is made of those that lie otherwise."""
+    buffer = random((3 * 4096,))
+    p, q = buffer[:4096].view(64, 64), buffer[4096:8192].view(64, 64)
+    states = [torchsso.optim.adamw_states(t, bits) for t in (p, q)]
+    m, v = zip(*states)
+    free = random((64, 64), seed=1)
+    before = buffer.clone()
+    for g in (q, p, buffer[100:4196].view(64, 64), buffer[8191:12287].view(64, 64)):
+        with pytest.raises(_hip.KfacHipError):
+            torchsso.optim.adamw([p, q], [g, free], m, v, 1)
+    if bits == 32:
+        with pytest.raises(_hip.KfacHipError):
+            torchsso.optim.adamw([p, q], [free, v[0]], m, v, 1)
+    assert torch.equal(buffer, before)
+    want = [p.clone(), q.clone()]
+    copies = [torchsso.optim.adamw_states(t, bits) for t in want]
+    torchsso.optim.adamw(want, [q.t().contiguous(), buffer[8192:].view(64, 64)], *zip(*copies), 1)
+    torchsso.optim.adamw([p, q], [q.t(), buffer[8192:].view(64, 64)], m, v, 1)
+    assert torch.equal(p, want[0]) and torch.equal(q, want[1])
+
+
 def test_an_update_is_a_change_in_place_that_autograd_sees():
     p = torch.nn.Parameter(random((4, 6)))
     x = random((3, 6)).requires_grad_()
