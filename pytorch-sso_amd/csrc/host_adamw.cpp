@@ -173,12 +173,12 @@ PyObject* host_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     std::vector<Tensor> written(params);
     for (size_t i = 0; i < n; ++i) {
       const Tensor& p = params[i];
-      if (!strided_on(p, device, type) || !p.unsafeGetTensorImpl()->is_non_overlapping_and_dense() ||
+      if (!strided_on(p, device, type) || p.is_neg() || !p.unsafeGetTensorImpl()->is_non_overlapping_and_dense() ||
           !strided_on(grads[i], device, type) || grads[i].sizes() != p.sizes())
         Py_RETURN_FALSE;
       for (int k = 0; k < (eight ? 4 : 2); ++k) {
         const Tensor& t = states[k][i];
-        if (!strided_on(t, device, state_types[k])) Py_RETURN_FALSE;
+        if (!strided_on(t, device, state_types[k]) || t.is_neg()) Py_RETURN_FALSE;
         if (k < 2 ? !lies_as(t, p)
                   : t.dim() != 1 || !t.is_contiguous() || t.size(0) != (p.numel() + STATE_BLOCK - 1) / STATE_BLOCK)
           Py_RETURN_FALSE;

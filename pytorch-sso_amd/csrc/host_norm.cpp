@@ -35,16 +35,17 @@ int type_code(at::ScalarType t) {
 }
 bool on_device(const Tensor& t) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided; }
 
-// rows of `dim` elements that lie side by side
+// rows of `dim` elements that lie side by side (a view may have its sign still to be applied, as imaginary parts of
+// conjugates do)
 Tensor rows_of(const Tensor& t, int64_t dim) {
-  Tensor r = t.reshape({-1, dim});
+  Tensor r = (t.is_neg() ? t.resolve_neg() : t).reshape({-1, dim});
   return dim > 1 && r.stride(1) != 1 ? r.contiguous() : r;
 }
 hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 bool gain_ok(const Tensor& gain, const Tensor& x) {
   return !gain.defined() || (on_device(gain) && gain.device() == x.device() && gain.dim() == 1 &&
-                             gain.size(0) == x.size(-1) && gain.is_contiguous() &&
+                             gain.size(0) == x.size(-1) && gain.is_contiguous() && !gain.is_neg() &&
                              (gain.scalar_type() == at::kFloat || gain.scalar_type() == x.scalar_type()));
 }
 // (the entry points take 32 bits of a row's length)
@@ -60,7 +61,7 @@ bool takes(const Tensor& x, const Tensor& residual, const Tensor& gain, const Te
   const int vectors = bias.defined() ? 2 : 1;
   if (curvature.defined() && (!on_device(curvature) || curvature.device() != x.device() || curvature.dim() != vectors ||
                               curvature.size(-1) != x.size(-1) || (vectors == 2 && curvature.size(0) != 2) ||
-                              curvature.scalar_type() != at::kFloat || !curvature.is_contiguous()))
+                              curvature.scalar_type() != at::kFloat || !curvature.is_contiguous() || curvature.is_neg()))
     return false;
   if (bias.defined() && (!gain.defined() || !gain_ok(bias, x) || bias.scalar_type() != gain.scalar_type())) return false;
   return gain_ok(gain, x);

@@ -982,6 +982,8 @@ def _rows(t, dim):
     t = t.reshape(-1, dim)
     if dim > 1 and t.stride(1) != 1:
         t = t.contiguous()
+    if isinstance(t, torch.Tensor) and t.is_neg():
+        t = t.resolve_neg()
     return t, t.stride(0)
 
 

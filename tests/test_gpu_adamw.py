@@ -350,6 +350,7 @@ def test_refusals():
                 lambda: adamw([p], [g], [(m8[0], m8[1][:-1])], [v8], 1), lambda: adamw([p], [g], [v8], [m8], 1),
                 lambda: adamw([p], [g], [(m8[0], v8[1])], [v8], 1),
                 lambda: adamw([p[:30], p[20:]], [g[:30], g[20:]], [m[:30], m[20:].clone()], [v[:30], v[20:].clone()], 1),
+                lambda: adamw([torch._neg_view(p)], [g], [m], [v], 1), lambda: adamw([p], [g], [torch._neg_view(m)], [v], 1),
                 lambda: adamw([p], [g], [m], [v], [count.long()]), lambda: adamw([p], [g], [m], [v], [count.cpu()]),
                 lambda: adamw([p, p.clone()], [g, g], [m, m.clone()], [v, v.clone()], [count, count]),
                 lambda: adamw([p], [g], [m], [v], 1, lr=torch.tensor(1., device='cuda')),

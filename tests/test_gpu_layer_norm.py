@@ -275,6 +275,28 @@ def test_the_same_tensor_twice():
     check(dgain, want.dgain + want.dbias, torch.float32, 2e-6, want.dgain.norm().item() + want.dbias.norm().item())
 
 
+@pytest.mark.parametrize('norm', ['layer_norm', 'rms_norm'])
+def test_views_whose_sign_is_still_to_be_applied(norm):
+    gen = torch.Generator().manual_seed(0)
+    one, two, three = [torch.complex(*torch.randn(2, 6, 40, generator=gen)).cuda().conj().imag for _ in range(3)]
+    assert one.is_neg() and two.is_neg()
+    gain = torch.rand(40, generator=gen).cuda()
+    results = []
+    for x, r, dy in ((one, two, three), (one.resolve_neg(), two.resolve_neg(), three.resolve_neg())):
+        x, r = x.detach().requires_grad_(), r.detach().requires_grad_()
+        y, h = getattr(torchsso.nn, 'add_' + norm)(x, r, gain)
+        results.append([y, h] + list(torch.autograd.grad([y, h], [x, r], [dy, dy])))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    with pytest.raises(_hip.KfacHipError):
+        getattr(torchsso.nn, norm)(one, torch._neg_view(gain))
+    backward = getattr(_ops, norm + '_backward')
+    kept = (lambda x: _ops.layer_norm_stats(x, 1e-5)) if norm == 'layer_norm' else lambda x: None
+    for a, b in zip(*[backward(dy, dy, x, *((kept(x), gain, 2) if norm == 'layer_norm' else (gain, 1e-5, 2)))
+                      for x, dy in ((one, three), (one.resolve_neg(), three.resolve_neg()))]):
+        assert torch.equal(a, b)
+
+
 def test_empty():
     gain, bias = (random((50,), seed=i).requires_grad_() for i in range(2))
     x = torch.zeros(0, 4, 50, device='cuda', requires_grad=True)
