@@ -10,9 +10,11 @@
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros_like.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/kfac_hip.h"
@@ -73,6 +75,21 @@ void check(int status, const char* what) {
 const void* address(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* writable(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
+// A backward pass that is being recorded cannot hand its gradients to leaves that belong to a graph from outside as well:
+// autograd would bring the default stream, on which that one was built, into the recording, and the process would end.
+void leaves_take_recorded_gradients(const char* what) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& edge : node->next_edges()) {
+    auto* const leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
+    const auto stream = leaf ? leaf->stream() : std::nullopt;
+    // (by their numbers: autograd has the device's type otherwise than c10::hip)
+    TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(stream->device_index()).id(), what,
+                ": its backward pass cannot be recorded while another graph of its leaves, built on the default stream, lives");
+  }
+}
+
 struct Normed {
   Tensor y, h, scale;
 };
@@ -111,6 +128,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "rms_norm has no second derivative (create_graph)");
+    leaves_take_recorded_gradients("rms_norm");
     const auto saved = ctx->get_saved_variables();
     const Tensor h = saved[0], gain = saved[1], curvature = ctx->saved_data["curvature"].toTensor();
     const bool residual = ctx->saved_data["residual"].toBool();
@@ -199,6 +217,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm has no second derivative (create_graph)");
+    leaves_take_recorded_gradients("layer_norm");
     const auto saved = ctx->get_saved_variables();
     const Tensor h = saved[0], gain = saved[1], stats = saved[2], curvature = ctx->saved_data["curvature"].toTensor();
     const bool residual = ctx->saved_data["residual"].toBool(), bias = ctx->saved_data["bias"].toBool();

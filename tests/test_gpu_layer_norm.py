@@ -394,6 +394,31 @@ def test_in_a_recorded_graph_and_on_another_stream():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize('norm', ['layer_norm', 'rms_norm'])
+def test_recording_while_an_eager_graph_of_the_leaves_lives_is_refused(norm):
+    x, gain, dy = random((6, 20, 300)), random((300,), seed=1), random((6, 20, 300), seed=2)
+    gain.requires_grad_()
+
+    def work():
+        y = getattr(torchsso.nn, norm)(x, gain)
+        return torch.autograd.grad(y, gain, dy)[0]
+    eager = getattr(torchsso.nn, norm)(x, gain)
+    side = torch.cuda.Stream()
+    with pytest.raises(RuntimeError, match='cannot be recorded'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            work()
+    assert torch.equal(eager, getattr(torchsso.nn, norm)(x, gain).detach())
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        recorded = work()
+    for seed in range(3):
+        x.copy_(random((6, 20, 300), seed=30 + seed))
+        graph.replay()
+        got = recorded.clone()
+        assert torch.equal(got, work())
+
+
 def test_two_threads_at_once():
     inputs = [[random((7, 33, 1024), seed=2 * i + k) for k in range(2)] for i in range(2)]
 
