@@ -77,12 +77,14 @@ void* writable(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nu
 
 // A backward pass that is being recorded cannot hand its gradients to leaves that belong to a graph from outside as well:
 // autograd would bring the default stream, on which that one was built, into the recording, and the process would end.
+// (Leaves that this backward pass is not asked for get nothing from it, and may belong to any graph.)
 void leaves_take_recorded_gradients(const char* what) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
-  for (const auto& edge : node->next_edges()) {
-    auto* const leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    if (!node->task_should_compute_output(i)) continue;
+    auto* const leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(node->next_edge(i).function.get());
     const auto stream = leaf ? leaf->stream() : std::nullopt;
     // (by their numbers: autograd has the device's type otherwise than c10::hip)
     TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(stream->device_index()).id(), what,

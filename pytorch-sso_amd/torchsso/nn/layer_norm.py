@@ -7,8 +7,8 @@ The reference's networks normalise with BatchNorm and its curvature (curv/cov/ba
 this is the norm of a decoder's blocks that are centred as well.  Its backward pass forms the diagonal
 curvature of gain and bias in the same pass over memory as the gradients (curv/cov/layer_norm.py hands
 it to an optimizer).  Forward and backward passes can be recorded into a graph; a backward pass is refused there while
-another graph of its inputs or parameters, built on the default stream, lives (autograd cannot hand gradients on from the
-one to the other).
+another graph of inputs or parameters whose gradients it is asked for, built on the default stream, lives (autograd cannot
+hand gradients on from the one to the other).
 """
 import torch
 import torch.nn as nn

@@ -6,6 +6,9 @@
 The reference's networks normalise with BatchNorm and its curvature (curv/cov/batchnorm.py:10-49);
 this is the norm of a decoder's blocks.  Its backward pass forms the diagonal curvature of the gain
 in the same pass over memory as the gradients (curv/cov/rms_norm.py hands it to an optimizer).
+Forward and backward passes can be recorded into a graph; a backward pass is refused there while another graph of inputs
+or parameters whose gradients it is asked for, built on the default stream, lives (autograd cannot hand gradients on from
+the one to the other).
 """
 import torch
 import torch.nn as nn

@@ -419,6 +419,31 @@ def test_recording_while_an_eager_graph_of_the_leaves_lives_is_refused(norm):
         assert torch.equal(got, work())
 
 
+@pytest.mark.parametrize('norm', ['layer_norm', 'rms_norm'])
+@pytest.mark.parametrize('ask', ['input', 'gain'])
+def test_recording_while_an_eager_graph_of_leaves_that_get_nothing_lives(norm, ask):
+    """... of the gain, where the gradient of the input alone is asked for, and the other way round"""
+    x, gain, dy = random((6, 20, 300)), random((300,), seed=1), random((6, 20, 300), seed=2)
+    other = (gain if ask == 'input' else x).requires_grad_()
+
+    def work():
+        leaf = (x if ask == 'input' else gain).detach().requires_grad_()
+        y = getattr(torchsso.nn, norm)(*((leaf, gain) if ask == 'input' else (x, leaf)))
+        return torch.autograd.grad(y, leaf, dy)[0]
+    eager = getattr(torchsso.nn, norm)(x, gain)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        recorded = work()
+    for seed in range(3):
+        with torch.no_grad():
+            dy.copy_(random((6, 20, 300), seed=30 + seed))
+        graph.replay()
+        got = recorded.clone()
+        assert torch.equal(got, work())
+    # (the graph from outside is whole)
+    assert torch.autograd.grad(eager, other, dy)[0].shape == other.shape
+
+
 def test_two_threads_at_once():
     inputs = [[random((7, 33, 1024), seed=2 * i + k) for k in range(2)] for i in range(2)]
 
