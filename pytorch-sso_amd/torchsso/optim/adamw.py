@@ -163,14 +163,15 @@ class AdamW(Optimizer):
     def _first_state(self, p, group, capturing):
         if capturing:
             raise RuntimeError('AdamW: a step has to be taken before one is recorded (it makes the states)')
-        state = self.state[p]
-        state['step'] = torch.zeros((), dtype=torch.int32, device=p.device) if group['capturable'] else 0
+        state = {'step': torch.zeros((), dtype=torch.int32, device=p.device) if group['capturable'] else 0}
         eight = group['state_bits'] == 8 and p.numel() >= group['min_8bit_size']
         m, v = adamw_states(p, 8 if eight else 32)
         if eight:
             (state['exp_avg'], state['exp_avg_scale']), (state['exp_avg_sq'], state['exp_avg_sq_scale']) = m, v
         else:
             state['exp_avg'], state['exp_avg_sq'] = m, v
+        # (kept once it is whole: a step that runs out of memory here can be taken again)
+        self.state[p] = state
         return state
 
     def step(self, closure=None):

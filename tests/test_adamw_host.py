@@ -334,3 +334,28 @@ def test_lr_scheduler(monkeypatch):
         opt.step()
         sched.step()
     assert [c[3] for c in calls] == [1., .5, .25]
+
+
+@pytest.mark.parametrize('capturable', [False, True])
+def test_a_step_that_ran_out_of_memory_can_be_taken_again(monkeypatch, capturable):
+    """(where the states are made: none of a parameter, or all)"""
+    calls = []
+    monkeypatch.setattr(_ops, 'adamw', fake_update(calls))
+    p = torch.nn.Parameter(torch.zeros(5000))
+    p.grad = torch.ones_like(p)
+    opt = torchsso.optim.AdamW([p], state_bits=8, capturable=capturable)
+    zeros_like, made = torch.zeros_like, []
+
+    def full(*args, **more):
+        if made:
+            raise torch.OutOfMemoryError('no memory')
+        made.append(1)
+        return zeros_like(*args, **more)
+    monkeypatch.setattr(torch, 'zeros_like', full)
+    with pytest.raises(torch.OutOfMemoryError):
+        opt.step()
+    assert made and not calls and not opt.state_dict()['state']
+    monkeypatch.setattr(torch, 'zeros_like', zeros_like)
+    opt.step()
+    assert len(calls) == 1 and int(calls[0][2][0]) == (0 if capturable else 1)
+    assert sorted(opt.state[p]) == ['exp_avg', 'exp_avg_scale', 'exp_avg_sq', 'exp_avg_sq_scale', 'step']
