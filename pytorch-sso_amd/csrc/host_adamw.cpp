@@ -221,8 +221,10 @@ PyObject* host_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                            c10::hip::getCurrentHIPStream(device.index()).stream());
     }
     TORCH_CHECK(status == KFAC_OK, "kfac_adamw_batched failed (code ", status, ")");
-    // (a graph from before the update that goes through these is refused by its backward pass)
-    for (const Tensor& t : written) t.unsafeGetTensorImpl()->bump_version();
+    // (a graph from before the update that goes through these is refused by its backward pass; inference tensors are in
+    // no graph and have no version, and what has been updated is not to end in an error)
+    for (const Tensor& t : written)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     Py_RETURN_TRUE;
   } catch (...) {
     torch::translate_exception_to_python(std::current_exception());      // (each as torch's own calls raise it)

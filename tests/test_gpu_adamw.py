@@ -530,6 +530,34 @@ def test_beside_muon_and_a_curvature():
         assert torch.isfinite(p).all() and not torch.equal(p, b)
 
 
+@BITS
+@pytest.mark.parametrize('capturable', [False, True])
+def test_states_made_in_inference_mode(bits, capturable):
+    """Such tensors have no version to raise: what has been updated is not reported as an error."""
+    p, g = random((70, 80)), random((70, 80), seed=1)
+    q, plain = p.clone(), torchsso.optim.adamw_states(p, bits)
+    with torch.inference_mode():
+        m, v = torchsso.optim.adamw_states(p, bits)
+        step = torch.zeros((), dtype=torch.int32, device='cuda')
+    for t in (1, 2):
+        torchsso.optim.adamw([p], [g], [m], [v], [step] if capturable else t, **OPTIONS)
+        torchsso.optim.adamw([q], [g], [plain[0]], [plain[1]], t, **OPTIONS)
+    assert p._version == 2 and (not capturable or int(step) == 2)
+    if capturable:
+        # (the device's logarithms may be off by some last bits of 64: no more than one of 32)
+        assert bool(((p - q).abs() <= 1e-6 * (q.abs() + 1)).all())
+    else:
+        assert torch.equal(p, q) and torch.equal(values(m), values(plain[0])) and torch.equal(values(v), values(plain[1]))
+    # a step of the class in that mode makes such states; it goes on outside
+    w = torch.nn.Parameter(random((70, 80)))
+    w.grad = g
+    opt = torchsso.optim.AdamW([w], state_bits=bits, capturable=capturable)
+    with torch.inference_mode():
+        opt.step()
+    opt.step()
+    assert int(opt.state[w]['step']) == 2
+
+
 # ---------------------------------------------------------------------------------------
 # large
 # ---------------------------------------------------------------------------------------
