@@ -111,14 +111,26 @@ class AdamW(Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_size=4096,
                  capturable=False, seed=0):
-        if isinstance(lr, torch.Tensor) and not capturable:
+        defaults = {'lr': lr, 'betas': betas, 'eps': eps, 'weight_decay': weight_decay, 'state_bits': state_bits,
+                    'min_8bit_size': min_8bit_size, 'capturable': capturable, 'seed': seed}
+        self._check_options(defaults)
+        if state_bits == 8:
+            _check(lr, betas, eps, weight_decay, True)
+        super(AdamW, self).__init__(params, defaults)
+
+    @staticmethod
+    def _check_options(group):
+        if isinstance(group['lr'], torch.Tensor) and not group['capturable']:
             raise ValueError('a learning rate on the device needs capturable=True')
-        if state_bits not in (8, 32):
-            raise ValueError('Invalid number of bits: {}'.format(state_bits))
-        _check(lr, betas, eps, weight_decay, state_bits == 8)
-        super(AdamW, self).__init__(params, {
-            'lr': lr, 'betas': betas, 'eps': eps, 'weight_decay': weight_decay, 'state_bits': state_bits,
-            'min_8bit_size': min_8bit_size, 'capturable': capturable, 'seed': seed})
+        if group['state_bits'] not in (8, 32):
+            raise ValueError('Invalid number of bits: {}'.format(group['state_bits']))
+        # (eps for 8 bits: of a group whose tensors may all be too small for those an update says more)
+        _check(group['lr'], group['betas'], group['eps'], group['weight_decay'])
+
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            self._check_options(dict(self.defaults, **param_group))
+        super(AdamW, self).add_param_group(param_group)
 
     _KEPT = {'exp_avg': (torch.float32, torch.float8_e4m3fn), 'exp_avg_sq': (torch.float32, torch.float8_e5m2),
              'exp_avg_scale': (torch.float32,), 'exp_avg_sq_scale': (torch.float32,)}
@@ -164,9 +176,9 @@ class AdamW(Optimizer):
         if capturing:
             raise RuntimeError('AdamW: a step has to be taken before one is recorded (it makes the states)')
         state = {'step': torch.zeros((), dtype=torch.int32, device=p.device) if group['capturable'] else 0}
-        eight = group['state_bits'] == 8 and p.numel() >= group['min_8bit_size']
-        m, v = adamw_states(p, 8 if eight else 32)
-        if eight:
+        bits = 32 if group['state_bits'] == 8 and p.numel() < group['min_8bit_size'] else group['state_bits']
+        m, v = adamw_states(p, bits)
+        if bits == 8:
             (state['exp_avg'], state['exp_avg_scale']), (state['exp_avg_sq'], state['exp_avg_sq_scale']) = m, v
         else:
             state['exp_avg'], state['exp_avg_sq'] = m, v

@@ -359,3 +359,30 @@ def test_a_step_that_ran_out_of_memory_can_be_taken_again(monkeypatch, capturabl
     opt.step()
     assert len(calls) == 1 and int(calls[0][2][0]) == (0 if capturable else 1)
     assert sorted(opt.state[p]) == ['exp_avg', 'exp_avg_scale', 'exp_avg_sq', 'exp_avg_sq_scale', 'step']
+
+
+def test_options_of_a_group_are_checked(monkeypatch):
+    calls = []
+    monkeypatch.setattr(_ops, 'adamw', fake_update(calls))
+    p, q = (torch.nn.Parameter(torch.zeros(n)) for n in (5000, 10))
+    AdamW = torchsso.optim.AdamW
+    for more in (dict(lr=-1.), dict(lr=float('nan')), dict(betas=(1., .9)), dict(eps=-1.), dict(weight_decay=-1.), dict(state_bits=16),
+                 dict(state_bits=4), dict(lr=torch.tensor(1e-3))):
+        with pytest.raises(ValueError):
+            AdamW([dict(params=[p], **more)])
+        opt = AdamW([q])
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=[p], **more))
+        assert len(opt.param_groups) == 1
+    opt = AdamW([dict(params=[p], lr=torch.tensor(1e-3), capturable=True), dict(params=[q], state_bits=8, eps=0.)])
+    opt.param_groups[0]['state_bits'] = 16            # (changed later: said where states are made)
+    for t in (p, q):
+        t.grad = torch.ones_like(t)
+    with pytest.raises(ValueError, match='16'):
+        opt.step()
+    opt.param_groups[0]['state_bits'] = 8
+    opt.step()
+    # (tensors too small for states in 8 bits take any eps)
+    assert [c[1] for c in calls] == [True, False]
+    with pytest.raises(TypeError):
+        AdamW([q]).add_param_group([p])
