@@ -368,7 +368,8 @@ __global__ __launch_bounds__(ADAM_THREADS) void adamw_kernel(const AdamList<BITS
 
 // ---- numbers of the update on the device -----------------------------------------
 
-// (an update by less than LEAST_SIZE is none: the quotients above would leave float32)
+// (an update by less than LEAST_SIZE is none: the quotients above would leave float32.  eps' is infinite then, and root 1: 0
+// would make a number that is none of it where v has overflowed)
 constexpr double LEAST_SIZE = 1e-30;
 __host__ __device__ inline AdamScalars scalars_of(double t, unsigned step, double lr, double b1, double b2, double eps,
                                                   double decay, unsigned seed) {
@@ -376,7 +377,7 @@ __host__ __device__ inline AdamScalars scalars_of(double t, unsigned step, doubl
   const double size = lr / (b1 > 0. ? -expm1(t * log(b1)) : 1.);
   const bool some = !(fabs(size) < LEAST_SIZE);
   s.keep = (float)(1. - lr * decay);
-  s.root = some ? (float)(1. / (size * sqrt(b2 > 0. ? -expm1(t * log(b2)) : 1.))) : 0.f;
+  s.root = some ? (float)(1. / (size * sqrt(b2 > 0. ? -expm1(t * log(b2)) : 1.))) : 1.f;
   s.eps = some ? (float)(eps / size) : INFINITY;
   s.key = update_key(seed, step);
   return s;

@@ -531,6 +531,22 @@ def test_beside_muon_and_a_curvature():
 
 
 @BITS
+@pytest.mark.parametrize('on_device', [False, True])
+@pytest.mark.parametrize('lr', [0., 1e-35])
+def test_an_update_by_nothing_leaves_parameters_whose_v_overflows(bits, on_device, lr):
+    """The first steps of a schedule from 0: m is a number, the root of v infinite, and the update 0."""
+    p, g = random((300,)), random((300,), seed=1)
+    g[::7] = 1e25
+    before = p.clone()
+    m, v = torchsso.optim.adamw_states(p, bits)
+    step = [torch.zeros((), dtype=torch.int32, device='cuda')] if on_device else 1
+    torchsso.optim.adamw([p], [g], [m], [v], step, **dict(OPTIONS, lr=torch.tensor(lr, device='cuda') if on_device else lr))
+    assert bool(torch.isinf(flat(v[0] if bits == 8 else v)[::7]).all())
+    # (1 - lr weight_decay is 1 in float32)
+    assert torch.equal(p, before)
+
+
+@BITS
 @pytest.mark.parametrize('capturable', [False, True])
 def test_states_made_in_inference_mode(bits, capturable):
     """Such tensors have no version to raise: what has been updated is not reported as an error."""
