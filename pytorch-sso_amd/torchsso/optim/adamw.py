@@ -147,6 +147,9 @@ class AdamW(Optimizer):
         for p, i in zip(own, (i for group in state_dict['param_groups'] for i in group['params'])):
             saved = state_dict['state'].get(i) or {}
             for name in ('exp_avg', 'exp_avg_sq'):
+                if name in saved and saved[name].numel() != p.numel():
+                    raise ValueError('a state of shape {} is not that of a parameter of shape {}'.format(
+                        tuple(saved[name].shape), tuple(p.shape)))
                 if name + '_scale' in saved and _ops._strides(saved[name]) != _ops._strides(p):
                     raise ValueError('a state in 8 bits with strides {} does not lie in memory as its parameter, {}'.format(
                         saved[name].stride(), p.stride()))

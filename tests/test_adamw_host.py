@@ -386,3 +386,19 @@ def test_options_of_a_group_are_checked(monkeypatch):
     assert [c[1] for c in calls] == [True, False]
     with pytest.raises(TypeError):
         AdamW([q]).add_param_group([p])
+
+
+@pytest.mark.parametrize('bits', [8, 32])
+def test_states_of_another_shape_are_refused(monkeypatch, bits):
+    """(not spread over the parameter: a vector's state over the rows of a matrix)"""
+    monkeypatch.setattr(_ops, 'adamw', lambda *a: True)
+    make = lambda shape: torchsso.optim.AdamW([torch.nn.Parameter(torch.zeros(shape))], state_bits=bits, min_8bit_size=1)
+    opt, other = make((20,)), make((3, 20))
+    p, q = (o.param_groups[0]['params'][0] for o in (opt, other))
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(ValueError, match='shape'):
+        other.load_state_dict(opt.state_dict())
+    assert not other.state
+    for shape in ((20,), (1, 20)):
+        make(shape).load_state_dict(opt.state_dict())
