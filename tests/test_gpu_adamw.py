@@ -615,3 +615,28 @@ def test_more_elements_than_32_bits_count(bits):
         assert bool((m[1][blocks] > 0).all())
     # what has no gradient has not moved
     assert not p[400:1 << 31].any()
+
+
+def test_states_in_8_bits_behind_more_elements_than_32_bits_count():
+    """Codes and scales there are those of their own places: of the blocks, and of the random numbers' units."""
+    n = (1 << 32) + 5 * BLOCK + 77
+    p = torch.zeros(n, device='cuda', dtype=torch.bfloat16)
+    g = torch.zeros_like(p)
+    m, v = torchsso.optim.adamw_states(p, 8)
+    parts = [slice(0, 300), slice((1 << 31) - 40 * BLOCK, (1 << 31) + 70), slice((n - 205) // BLOCK * BLOCK, n)]
+    for i, s in enumerate(parts):
+        k = s.stop - s.start
+        p[s], g[s] = random((k,), torch.bfloat16, 2 * i), random((k,), torch.bfloat16, 2 * i + 1)
+    for t in (1, 2):
+        blocks = [slice(s.start // BLOCK, -(-s.stop // BLOCK)) for s in parts]
+        part = lambda state: [(state[0][s], state[1][b]) for s, b in zip(parts, blocks)]
+        before = [(flat(p[s]), flat(g[s]), values(a), values(b)) for s, a, b in zip(parts, part(m), part(v))]
+        torchsso.optim.adamw([p], [g], [m], [v], t, seed=3, **OPTIONS)
+        for s, was, (mq, ms), (vq, vs) in zip(parts, before, part(m), part(v)):
+            u = Update(*was, t, *(OPTIONS[k] for k in ('lr', 'betas', 'eps', 'weight_decay')))
+            w = words(s.stop - s.start, 3, t, 0, s.start)
+            check_p(flat(p[s]), u, p.dtype)
+            check_8(mq, ms, u.m, 'm', w >> 16)
+            check_8(vq, vs, u.v, 'v', w & 0xffff)
+    # (and nothing beside them)
+    assert not m[1][3:parts[1].start // BLOCK].any() and not v[1][parts[1].stop // BLOCK + 1:parts[2].start // BLOCK].any()
