@@ -162,7 +162,7 @@ PyObject* host_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     for (const int64_t t : steps)
       if (t < 1) Py_RETURN_FALSE;
     for (const Tensor& t : counters)
-      if (!strided_on(t, device, at::kInt) || t.numel() != 1) Py_RETURN_FALSE;
+      if (!strided_on(t, device, at::kInt) || t.numel() != 1 || t.is_neg()) Py_RETURN_FALSE;
     Tensor rate;
     if (lr_on_device) {
       rate = THPVariable_Unpack(args[5]);
@@ -207,6 +207,8 @@ PyObject* host_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         at[0][i] = params[i].mutable_data_ptr();
         for (int k = 0; k < (eight ? 4 : 2); ++k) at[1 + k][i] = states[k][i].mutable_data_ptr();
       }
+      // (a view may have its sign still to be applied)
+      if (rate.defined()) rate = rate.detach().resolve_neg();
       std::vector<int*> counter(counters.size());
       for (size_t i = 0; i < counters.size(); ++i) counter[i] = (int*)counters[i].mutable_data_ptr();
       Tensor scratch;

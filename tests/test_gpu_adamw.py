@@ -530,6 +530,22 @@ def test_beside_muon_and_a_curvature():
         assert torch.isfinite(p).all() and not torch.equal(p, b)
 
 
+def test_numbers_on_the_device_whose_sign_is_still_to_be_applied():
+    """A learning rate is read with it; a counter, which is written, is refused."""
+    p, g = random((300,)), random((300,), seed=1)
+    q = p.clone()
+    step = lambda: torch.zeros((), dtype=torch.int32, device='cuda')
+    rate = torch.tensor(1e-2, device='cuda')
+    for t, lr in ((p, torch._neg_view(-rate)), (q, rate)):
+        m, v = torchsso.optim.adamw_states(t)
+        torchsso.optim.adamw([t], [g], [m], [v], [step()], **dict(OPTIONS, lr=lr))
+    assert torch.equal(p, q)
+    m, v = torchsso.optim.adamw_states(p)
+    with pytest.raises(_hip.KfacHipError):
+        torchsso.optim.adamw([p], [g], [m], [v], [torch._neg_view(step())], **OPTIONS)
+    assert torch.equal(p, q)
+
+
 @BITS
 @pytest.mark.parametrize('on_device', [False, True])
 @pytest.mark.parametrize('lr', [0., 1e-35])
