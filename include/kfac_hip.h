@@ -546,7 +546,7 @@ int kfac_muon_update_batched(int count, const int* rows, const int* cols, int ty
  *   mix(x): x ^= x >> 16; x *= 0x9E3779B1; x ^= x >> 15; x *= 0xB504F333; x ^= x >> 16
  *   w_0 = mix(mix(mix(mix(seed) + t) + i) + u),  w_(k+1) = w_k after w ^= w << 13; w ^= w >> 17; w ^= w << 5
  * the upper 16 for m, the lower for v, except that a v above 0 becomes at least the smallest number.
- * eps >= 0, in 8 bits at least 1e-12; lr / (1 - beta1^t) below 1e-30 leaves p as it is.  A call may hold one tensor once;
+ * eps >= 0, in 8 bits at least 1e-12; lr / (1 - beta1^t) below 1e-30 leaves p as it is (the decay aside).  A call may hold one tensor once;
  * parameters, states and counters lie apart from each other and from the gradients.
  * counters != NULL (steps NULL then): device addresses of int32 numbers of updates so far, which the call raises by
  * one and goes by, so that a recorded call counts on when it is replayed; lr_on_device != NULL (only with them): a

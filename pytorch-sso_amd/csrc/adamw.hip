@@ -14,7 +14,7 @@
 // Bound by memory: 3 s + 16 bytes an element with states in 32 bits (s: a parameter's), 3 s + 4.25 in 8.  A thread takes
 // 8 consecutive elements, so 16 threads hold a block, and every stream is read and written once, 16 bytes at a time (8
 // of an 8-bit state).  The list travels as a kernel argument, as that of the other element-wise passes (elementwise.hip).
-// 244 million bfloat16 parameters: 958 us in 32 bits, 5.6 TB/s, and 383 in 8, 6.5, where a large copy reaches 5.2; a
+// 244 million bfloat16 parameters: 991 us in 32 bits, 5.4 TB/s, and 388 in 8, 6.4, where a large copy reaches 5.2; a
 // ResNet-50 in float32 142 us, 5.0 TB/s.  With twice and four times the elements to a workgroup the last takes 3 and 6 % longer.
 #include <cmath>
 
@@ -154,7 +154,7 @@ __device__ __forceinline__ void block_scale(unsigned top_bits, float largest, fl
 // ---- the update --------------------------------------------------------------
 
 // ONCE: past the caches.  States in 8 bits of calls that access more than the last cache holds: 244 million bfloat16
-// parameters 435 us without that, 390 with it.  (In 32 bits it costs: 958 and 977.)
+// parameters 435 us without that, 390 with it.  (In 32 bits it costs: on one card 958 without and 977 with it.)
 constexpr double LAST_CACHE = 256. * (1 << 20);
 template <bool ONCE>
 __device__ __forceinline__ u4 load16(const void* p) {

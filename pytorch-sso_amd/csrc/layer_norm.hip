@@ -238,8 +238,10 @@ __global__ __launch_bounds__(block_threads(T)) void layer_norm_kernel(const Laye
   }
 }
 
-// Rows that do not fit registers: three passes over the row, or four, from cache as a rule, 16 bytes an access wherever a row
-// begins (1024 bfloat16 rows of 65536 with their residual: 167 us, one element an access 380).
+// Rows of more than four accesses a thread of 1024, which the kernel above does not hold as floats: three passes over the
+// row, or four, from cache as a rule, 16 bytes an access wherever a row begins (1024 bfloat16 rows of 65536 with their residual:
+// 167 us, one element an access 380; the streams alone 104).  Packed in their 16-bit type rows of up to 65536 elements would
+// fit registers; that is not built.
 template <class V>
 __global__ __launch_bounds__(1024) void layer_norm_long_kernel(const LayerNormArgs a) {
   constexpr int E = width<V>(), STEP = 1024 * E;
@@ -514,8 +516,8 @@ __global__ __launch_bounds__(1024) void layer_norm_dx_kernel(const LayerBackArgs
   }
 }
 
-// ... of rows that do not fit registers: two passes over the row, the second from cache as a rule (the backward pass of 1024
-// rows of 65536: 244 us with the sums over rows, one element an access 474)
+// ... of rows of more than four accesses a thread: two passes over the row, the second from cache as a rule (the backward pass
+// of 1024 rows of 65536: 244 us with the sums over rows, one element an access 474; the streams alone 104)
 template <class V>
 __global__ __launch_bounds__(1024) void layer_norm_dx_long_kernel(const LayerBackArgs a) {
   constexpr int E = width<V>(), STEP = 1024 * E;
